@@ -76,7 +76,8 @@ const char* b200lut_last_error(void);
  * non-zero = a bounded wait inside a kernel ran out (the kernel then returned early
  * with its tensor memory freed and its output undefined). Synchronises the device
  * read; clears the word. No counterpart in the reference (its kernels never wait).
- * 0x6000: an embedding gather met an id outside its table (that row was written as zeros). */
+ * 0x6000: an embedding gather met an id outside its table (that row was written as zeros);
+ * 0x6100: a slot, 0x6200: a page outside a key/value cache. */
 int b200lut_device_status(void);
 
 /* Number of SMs of the current device (used by the split policy). */
@@ -535,6 +536,111 @@ enum {
 int b200lut_fht(const void* x, void* out, const float* signs, const float* scale,
                 int M, int K, int64_t ldx, int64_t ldo, int dtype, int mode, int block,
                 void* stream);
+
+/* ------------------------------------------------------------------------- *
+ * The attention side: positions, the 4-bit key/value cache, attention over it
+ * ------------------------------------------------------------------------- */
+
+/* Rotary positions over several axes. q [T, n_heads, D] and k [T, n_kv_heads, D] (strides in
+ * elements, multiples of 8; the last dimension contiguous) -> q_out, k_out, contiguous.
+ * Elements (i, i + R/2), i < R/2, of each head turn by 2 pi * positions[axis[i], t] * turns[i]
+ * (turns: theta^(-2i/R) / (2 pi), fp64); the other D - R elements pass. With q_gain and k_gain
+ * ([D], dtype) each head is first divided by its root mean square (eps inside the root) and
+ * multiplied by the gain. fp32 inside, one rounding. D in {64, 128, 256}, R a multiple of 16. */
+typedef struct b200lut_rotary_args {
+  const void* q;
+  const void* k;
+  void* q_out;
+  void* k_out;
+  const void* q_gain;          /* NULL: no norm (both or neither) */
+  const void* k_gain;
+  const void* positions;       /* [axes, T] int32 (or int64 with pos64) */
+  const double* turns;         /* [R / 2] */
+  const int32_t* axis;         /* [R / 2], each below the number of rows of positions */
+  int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride;
+  int64_t pos_stride;          /* elements between the axes' rows (0: one row serves all) */
+  int T, n_heads, n_kv_heads, D, R;
+  int pos64, dtype;
+  float eps;
+} b200lut_rotary_args;
+int b200lut_rotary(const b200lut_rotary_args* args, void* stream);
+
+/* A paged cache of 4-bit keys and values. A row is the D elements of one token and key/value
+ * head: lo and hi, its smallest and largest element, are kept exactly, an element is
+ * rint(15 (x - lo) / (hi - lo)) (half to even) and stands for lo + code (hi - lo) / 15. A row
+ * with a NaN, an infinity or a range of 2^120 and more reads as NaN. Slot = page * page_size +
+ * offset. k_codes, v_codes: n_pages * n_kv_heads * page_size * head_dim / 2 bytes each; k_pairs,
+ * v_pairs: n_pages * n_kv_heads * page_size * 4 bytes each; 16-byte aligned. */
+typedef struct b200lut_kv_cache {
+  void* k_codes;
+  void* v_codes;
+  void* k_pairs;
+  void* v_pairs;
+  int n_pages, page_size;      /* page_size: 16, 32, 64, 128 or 256; n_pages * page_size < 2^31 */
+  int n_kv_heads, head_dim;    /* head_dim: 64, 128 or 256 */
+  int dtype;
+} b200lut_kv_cache;
+
+/* What a step of a paged cache needs, from the requests' lengths on the device, in one launch.
+ * Request b has cached[b] tokens and brings fresh[b] more (negative counts as 0). In the order of
+ * the requests, pages that it does not have yet are taken from free_pages[*taken ..] and entered
+ * into its row of block_table. A request whose pages do not fit its row or the free list, or whose
+ * rows would end behind max_tokens, is not served: it gets no page and its slots are -1.
+ * Results: row_start [B + 1] (clamped to max_tokens), kv_len [B] (cached + fresh where served, else
+ * cached), positions and slots [max_tokens] (0 and -1 behind the last row; -1 also where the row
+ * holds a negative page), taken_out [1], served [B] (bytes, 0 or 1). Calling it again with the same
+ * inputs gives the same results. B <= 8192; cached + fresh < 2^31. */
+typedef struct b200lut_kv_plan_args {
+  const int32_t* cached;
+  const int32_t* fresh;
+  int32_t* block_table;        /* [B, width] */
+  const int32_t* free_pages;   /* [free_count] */
+  const int32_t* taken;        /* [1] */
+  int32_t* row_start;
+  int32_t* kv_len;
+  int32_t* positions;
+  int32_t* slots;
+  int32_t* taken_out;
+  uint8_t* served;
+  int B, width, free_count, page_size, max_tokens;
+} b200lut_kv_plan_args;
+int b200lut_kv_plan(const b200lut_kv_plan_args* args, void* stream);
+
+/* Rows k, v [tokens, n_kv_heads, head_dim] (strides in elements, multiples of 8) into the slots of
+ * the cache; a negative slot is skipped, one outside the cache too, and raises the device status
+ * (0x6100). Slots of one call must differ. */
+int b200lut_kv_write(const b200lut_kv_cache* cache, const void* k, const void* v, int64_t k_token_stride,
+                     int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride,
+                     const int32_t* slots, int tokens, void* stream);
+
+/* The values of slots, rounded to dtype, into contiguous k, v [tokens, n_kv_heads, head_dim];
+ * zeros for a negative slot and for one outside the cache, which raises the device status. */
+int b200lut_kv_read(const b200lut_kv_cache* cache, void* k, void* v, const int32_t* slots, int tokens,
+                    void* stream);
+
+/* Attention of q [T, n_heads, D] over the cache. Rows row_start[b] .. row_start[b + 1] of q are the
+ * last tokens of request b, whose kv_len[b] tokens lie in the pages of its row of block_table; the
+ * row at position p sees the tokens j <= p with window == 0, j > p - window or j < sinks. Query
+ * head h reads key/value head h / (n_heads / n_kv_heads). out = softmax(scale q k^T) v, times
+ * sigmoid(gate) with a gate; zeros where nothing is visible. Rows of q that belong to no request
+ * are not written. row_start NULL: one row per request (T == B). Tokens on a page outside the
+ * cache count as hidden and raise the device status (0x6200). */
+typedef struct b200lut_attend_args {
+  const b200lut_kv_cache* cache;
+  const void* q;
+  const void* gate;            /* [T, n_heads, D] or NULL */
+  void* out;
+  const int32_t* block_table;  /* [B, width], rows table_stride elements apart */
+  const int32_t* kv_len;       /* [B] */
+  const int32_t* row_start;    /* [B + 1] or NULL */
+  int64_t q_token_stride, q_head_stride, gate_token_stride, gate_head_stride;
+  int64_t out_token_stride, out_head_stride, table_stride;
+  int T, B, width, n_heads;
+  int window, sinks;
+  float scale;
+} b200lut_attend_args;
+size_t b200lut_attend_workspace_bytes(int n_heads, int n_kv_heads, int head_dim);
+int b200lut_attend(const b200lut_attend_args* args, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

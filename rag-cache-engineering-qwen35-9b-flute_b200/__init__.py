@@ -5,7 +5,7 @@ SplitQKV / FusedPalettizedMLP; compute: libb200lut.so (hand-written sm_100a CUDA
 behind a C ABI, see include/b200_lut.h). Import of this package does not load
 the library; the first compute call does, and fails loudly if it is not built.
 """
-from . import _lib, fht, idxN, synthetic                                    # noqa: F401
+from . import _lib, fht, idxN, kvcache, rotary, synthetic                  # noqa: F401
 from .palettized_modules import (FusedPalettizedMLP, KGroupedPalettizedLinear,  # noqa: F401
                                  PalettizedEmbedding, PalettizedLinear,
                                  SplitQKV,
@@ -19,4 +19,4 @@ from . import flute_extended                                                    
 __all__ = ["load_quant_model", "load_palettized_weight", "replace_linear_with_palettized",
            "load_palettized_embedding", "load_tied_pair", "export_luts", "import_luts",
            "iter_palettized_linears", "load_metadata", "PalettizedLinear", "PalettizedEmbedding", "KGroupedPalettizedLinear", "SplitQKV", "FusedPalettizedMLP", "reference_dequant",
-           "set_programmatic_launch", "fht", "idxN", "synthetic", "flute_extended"]
+           "set_programmatic_launch", "fht", "kvcache", "rotary", "idxN", "synthetic", "flute_extended"]

@@ -38,6 +38,8 @@ EXPORTS = (
     "b200lut_embed_gather", "b200lut_embed_gather_checked", "b200lut_round_rows", "b200lut_gemv_kgrouped",
     "b200lut_gemv_kgrouped_split", "b200lut_gemv_kgrouped_workspace_bytes", "b200lut_gemm_kgrouped", "b200lut_gemv_exchange", "b200lut_peer_export", "b200lut_peer_open", "b200lut_peer_close",
     "b200lut_gemv_noalloc", "b200lut_gemv_noalloc_reset", "b200lut_gemv_launch_blocks", "b200lut_gemv_input", "b200lut_plan_bytes", "b200lut_plan_build", "b200lut_plan_run", "b200lut_plan_status", "b200lut_plan_form", "b200lut_plan_release",
+    "b200lut_rotary", "b200lut_kv_plan", "b200lut_kv_write", "b200lut_kv_read", "b200lut_attend_workspace_bytes",
+    "b200lut_attend",
 )
 
 
@@ -84,6 +86,38 @@ class Input(ctypes.Structure):
     _fields_ = [("x_mul", ctypes.c_void_p), ("rot_signs", ctypes.c_void_p), ("awq_scale", ctypes.c_void_p),
                 ("per_segment", ctypes.c_int), ("seg_rot_signs", ctypes.c_void_p * 8),
                 ("seg_awq_scale", ctypes.c_void_p * 8)]
+
+
+class RotaryArgs(ctypes.Structure):
+    """struct b200lut_rotary_args."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "q_out", "k_out", "q_gain", "k_gain", "positions", "turns", "axis")]
+                + [(n, ctypes.c_int64) for n in ("q_token_stride", "q_head_stride", "k_token_stride", "k_head_stride",
+                                                 "pos_stride")]
+                + [(n, ctypes.c_int) for n in ("T", "n_heads", "n_kv_heads", "D", "R", "pos64", "dtype")]
+                + [("eps", ctypes.c_float)])
+
+
+class KVCacheView(ctypes.Structure):
+    """struct b200lut_kv_cache."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("k_codes", "v_codes", "k_pairs", "v_pairs")]
+                + [(n, ctypes.c_int) for n in ("n_pages", "page_size", "n_kv_heads", "head_dim", "dtype")])
+
+
+class KVPlanArgs(ctypes.Structure):
+    """struct b200lut_kv_plan_args."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("cached", "fresh", "block_table", "free_pages", "taken", "row_start",
+                                                "kv_len", "positions", "slots", "taken_out", "served")]
+                + [(n, ctypes.c_int) for n in ("B", "width", "free_count", "page_size", "max_tokens")])
+
+
+class AttendArgs(ctypes.Structure):
+    """struct b200lut_attend_args."""
+    _fields_ = ([("cache", ctypes.POINTER(KVCacheView))]
+                + [(n, ctypes.c_void_p) for n in ("q", "gate", "out", "block_table", "kv_len", "row_start")]
+                + [(n, ctypes.c_int64) for n in ("q_token_stride", "q_head_stride", "gate_token_stride", "gate_head_stride",
+                                                 "out_token_stride", "out_head_stride", "table_stride")]
+                + [(n, ctypes.c_int) for n in ("T", "B", "width", "n_heads", "window", "sinks")]
+                + [("scale", ctypes.c_float)])
 
 
 class LibraryError(RuntimeError):
@@ -194,6 +228,18 @@ def lib() -> ctypes.CDLL:
     L.b200lut_plan_form.argtypes = [vp]
     L.b200lut_plan_release.restype = i32
     L.b200lut_plan_release.argtypes = [vp]
+    L.b200lut_rotary.restype = i32
+    L.b200lut_rotary.argtypes = [ctypes.POINTER(RotaryArgs), vp]
+    L.b200lut_kv_plan.restype = i32
+    L.b200lut_kv_plan.argtypes = [ctypes.POINTER(KVPlanArgs), vp]
+    L.b200lut_kv_write.restype = i32
+    L.b200lut_kv_write.argtypes = [ctypes.POINTER(KVCacheView), vp, vp, i64, i64, i64, i64, vp, i32, vp]
+    L.b200lut_kv_read.restype = i32
+    L.b200lut_kv_read.argtypes = [ctypes.POINTER(KVCacheView), vp, vp, vp, i32, vp]
+    L.b200lut_attend_workspace_bytes.restype = sz
+    L.b200lut_attend_workspace_bytes.argtypes = [i32, i32, i32]
+    L.b200lut_attend.restype = i32
+    L.b200lut_attend.argtypes = [ctypes.POINTER(AttendArgs), vp, sz, vp]
     _lib = L
     return L
 

@@ -1,0 +1,612 @@
+// Attention over the 4-bit cache for few rows per request (single tokens): mma.sync on codes, split over tokens.
+//
+// A work item is 8 NT rows (query heads of one key/value head, times new tokens) of one request. Its visible
+// tokens are cut into tiles of 16; all items' tiles form one line that is dealt to the blocks in equal
+// contiguous shares, whatever the requests' lengths. The warps of a block take the tiles of its share in turn,
+// each with a running maximum and sum of its own, and join in shared memory; items that span blocks are
+// joined by a second kernel in the order of the blocks (deterministic, no atomics).
+//
+// Operands: the tokens are the M = 16 side of mma.m16n8k16, the rows its N = 8 side, so a tile of codes is
+// unpacked once and eight rows ride for free.
+//   S^T[token, row] = K[token, :] q[row, :]     A = keys: lane (g, t) holds 16 tokens' rows g and g + 8
+//   O^T[dim, row]  += V^T[dim, token] P^T       A = values: lane (g, t) holds elements 8 g .. 8 g + 7 of four tokens
+// Row s of A stands for token pi(s) = 4 (s / 2 % 4) + s % 2 + 2 (s / 8) of the tile, so that the four tokens of a
+// value lane are adjacent in memory; P^T comes out of S^T by two 8 x 8 transposes of half pairs.
+// Every lane copies exactly the 16-byte pieces it will read (cp.async into a ring of its own): no barrier in
+// the loop.
+#include "attend.cuh"
+
+namespace b200lut {
+namespace {
+
+__device__ int g_attend_status = 0;
+constexpr int kBadPage = 0x6200;
+constexpr int kWarps = 8;
+constexpr int kTile = 16;
+constexpr float kLazy = 8.f;           // the running maximum may lag by this many powers of two
+constexpr float kMinStep = 7.888609e-31f;   // 2^-100
+
+template <int D, int NT>
+struct Shape {
+  static constexpr int kRows = 8 * NT;
+  static constexpr int kWords = D / 32;                        // 32-bit words of a key row per lane
+  static constexpr int kPieces = D >= 128 ? D / 64 : 1;        // 16-byte key pieces per lane and tile
+  static constexpr int kStage = 16 * D + 512;                  // bytes of a tile: keys, values, pairs
+  static constexpr int kStages = D == 256 ? 2 : D == 128 ? 4 : 6;
+  static constexpr int kFold = kRows * (D + 4) * 4;            // a warp's partial result, in its ring's place
+  static constexpr int kRing = kStages * kStage > kFold ? kStages * kStage : kFold;
+  static constexpr int kQ = NT * D * 16;                       // query fragments
+  static constexpr int kSmem = kQ + kWarps * kRing + kRows * 8 + kWarps * kRows * 8;
+};
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp8(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 r;
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a) : "memory");
+  return r;
+}
+__device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                      uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t half2_of(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// the power of two >= x (x > 0, normal)
+__device__ __forceinline__ float pow2_above(float x) {
+  return __uint_as_float((__float_as_uint(x) + 0x007FFFFFu) & 0x7F800000u);
+}
+
+// Tiles of all items of request b (its row tiles are equal but for what they see).
+template <int kRows>
+__device__ __forceinline__ long long request_tiles(const AttendParams& p, int b) {
+  const Request r = request_of(p, b);
+  long long sum = 0;
+  const long long rows = (long long)r.rows * p.G;
+  for (long long r0 = 0; r0 < rows; r0 += kRows) {
+    const int last = int((min(r0 + kRows, rows) - 1) / p.G), base = r.len - r.rows;
+    sum += Span<kTile>(base + int(r0 / p.G), base + last, r.len, p.window, p.sinks).tiles;
+  }
+  return sum * p.c.heads;
+}
+
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) attend_rows_kernel(const __grid_constant__ AttendParams p) {
+  using S = Shape<D, NT>;
+  constexpr int kRows = S::kRows;
+  extern __shared__ __align__(128) uint8_t sm[];
+  uint16_t* sq = reinterpret_cast<uint16_t*>(sm);
+  uint8_t* ring = sm + S::kQ;
+  float2* row_k = reinterpret_cast<float2*>(sm + S::kQ + kWarps * S::kRing);     // factor of q.c, scaled sum of q
+  float2* warp_ml = row_k + kRows;                                               // [kWarps][kRows]
+  __shared__ long long scan[kWarps];
+  __shared__ long long first_tile;
+  __shared__ int first_b;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
+
+  // ---- this block's share of the line of tiles
+  long long total = 0, mine_before = 0;
+  const int per = (p.B + kWarps * 32 - 1) / (kWarps * 32);
+  long long mine = 0;
+  for (int i = 0; i < per; ++i) {
+    const int b = tid * per + i;
+    if (b < p.B) mine += request_tiles<kRows>(p, b);
+  }
+  long long inc = mine;
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += v;
+  }
+  if (lane == 31) scan[warp] = inc;
+  if (tid == 0) first_b = p.B;
+  __syncthreads();
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) mine_before += scan[w];
+    total += scan[w];
+  }
+  mine_before += inc - mine;
+  long long share = (total + gridDim.x - 1) / gridDim.x;
+  share = max((long long)kWarps, (share + kWarps - 1) / kWarps * kWarps);
+  const long long begin = share * blockIdx.x, stop = min(total, begin + share);
+  if (begin >= mine_before && begin < mine_before + mine) {
+    long long at = mine_before;
+    for (int i = 0; i < per; ++i) {
+      const int b = tid * per + i;
+      if (b >= p.B) break;
+      const long long n = request_tiles<kRows>(p, b);
+      if (begin < at + n) {
+        first_b = b;
+        first_tile = at;
+        break;
+      }
+      at += n;
+    }
+  }
+  __syncthreads();
+  if (tid == 0) p.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
+  if (begin >= stop) return;
+
+  const uint32_t ring_at = uint32_t(__cvta_generic_to_shared(ring + warp * S::kRing));
+  const uint32_t q_at = uint32_t(__cvta_generic_to_shared(sq)) + lane * 16;
+  const int tok0 = 4 * (g >> 1) + (g & 1);       // tokens of this lane's rows g and g + 8: tok0, tok0 + 2
+  long long cur = begin, req_at = first_tile;
+  for (int b = first_b; cur < stop && b < p.B; ++b) {
+    const Request rq = request_of(p, b);
+    const long long rows = (long long)rq.rows * p.G;
+    const int base = rq.len - rq.rows;
+    for (int h = 0; h < p.c.heads && cur < stop; ++h) {
+      for (long long r0 = 0; r0 < rows && cur < stop; r0 += kRows) {
+        const int n_rows = int(min((long long)kRows, rows - r0));
+        const int first_pos = base + int(r0 / p.G), last_pos = base + int((r0 + n_rows - 1) / p.G);
+        const Span<kTile> span(first_pos, last_pos, rq.len, p.window, p.sinks);
+        if (req_at + span.tiles <= cur) {
+          req_at += span.tiles;
+          continue;
+        }
+        const int i0 = int(cur - req_at), i1 = int(min((long long)span.tiles, stop - req_at));
+
+        // ---- the item's rows as fp16 fragments
+        __syncthreads();
+        for (int r = warp; r < kRows; r += kWarps) {
+          float v[D / 32], top = 0.f, sum = 0.f;
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i) v[i] = 0.f;
+          if (r < n_rows) {
+            const long long tok = rq.row0 + (r0 + r) / p.G;
+            const uint16_t* x = p.q + tok * p.q_token + (long long)(h * p.G + int((r0 + r) % p.G)) * p.q_head;
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) v[i] = DType<T>::to_float(x[lane * (D / 32) + i]);
+          }
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i) top = fmaxf(top, fabsf(v[i])), sum += v[i];
+          for (int o = 16; o; o >>= 1) {
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            sum += __shfl_xor_sync(0xffffffffu, sum, o);
+          }
+          const int ex = int(__float_as_uint(top) >> 23);                // exponent of the largest element
+          const int fe = ex == 255 || top == 0.f ? 127 : min(254, 127 + 13 + 127 - ex);
+          const float f = __uint_as_float(uint32_t(fe) << 23);
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i) {
+            const int d = lane * (D / 32) + i;
+            const int tig = D == 64 ? d / 16 : (d % 128) / 32, nib = d % 8;
+            const int w = D == 64 ? (d % 16) / 8 : (d / 128) * 4 + (d % 32) / 8;
+            const float x = v[i] * f * (nib & 1 ? 0.0625f : 1.f);
+            sq[((((r >> 3) * S::kWords + w) * 32 + (r & 7) * 4 + tig) * 4 + (nib & 3)) * 2 + (nib >> 2)] =
+                __half_as_ushort(__float2half_rn(x));
+          }
+          if (lane == 0) row_k[r] = make_float2(p.scale * 16777216.f / f, p.scale * sum);
+        }
+        __syncthreads();
+
+        float qf[NT][2], qs[NT][2], m[NT][2], l[NT][2], pm[NT][2];
+        int pos[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int r = n * 8 + 2 * t4 + e;
+            const float2 k = row_k[r];
+            qf[n][e] = k.x, qs[n][e] = k.y;
+            m[n][e] = -INFINITY, l[n][e] = 0.f, pm[n][e] = 0.f;
+            pos[n][e] = r < n_rows ? base + int((r0 + r) / p.G) : -1;
+          }
+        float o[NT][D / 16][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[n][i][e] = 0.f;
+        float sig = 0.f, inv_sig = 0.f;
+
+        // ---- the ring
+        const int iters = i1 - i0 > warp ? (i1 - i0 - warp + kWarps - 1) / kWarps : 0;
+        const int* table = p.table + (long long)b * p.table_ld;
+        int pages = -1;              // lane x: the page of iteration 32 * (k / 32) + x
+        uint32_t bad = 0;            // bit of a stage: its page is not one of the cache
+        auto load = [&](int k) {
+          if (k < iters) {
+            if ((k & 31) == 0) {
+              const int kk = k + lane;
+              pages = -1;
+              if (kk < iters) {
+                const int first = span.id(i0 + warp + kk * kWarps) * kTile;
+                if (first < rq.len) pages = table[first >> p.c.page_log2];
+              }
+            }
+            const int page = __shfl_sync(0xffffffffu, pages, k & 31);
+            const int first = span.id(i0 + warp + k * kWarps) * kTile;
+            const int stage = k % S::kStages;
+            const bool ok = page >= 0 && page < p.c.n_pages;
+            if (ok) {
+              bad &= ~(1u << stage);
+              const int off = first & ((1 << p.c.page_log2) - 1);
+              const long long codes = cache_codes_at(page, h, p.c.heads, p.c.page_log2, D) + (long long)off * (D / 2);
+              const uint32_t dst = ring_at + stage * S::kStage + lane * 16;
+              const uint8_t* kp = p.c.k + codes;
+              if constexpr (D == 64) {
+                cp8(dst, kp + tok0 * 32 + t4 * 8);
+                cp8(dst + 8, kp + (tok0 + 2) * 32 + t4 * 8);
+              } else {
+#pragma unroll
+                for (int i = 0; i < S::kPieces; ++i)
+                  cp16(dst + i * 512, kp + (tok0 + 2 * (i & 1)) * (D / 2) + (i >> 1) * 64 + t4 * 16);
+              }
+              const uint8_t* vp = p.c.v + codes + (t4 * 8 + g) * 16;
+#pragma unroll
+              for (int i = 0; i < D / 64; ++i) cp16(dst + S::kPieces * 512 + i * 512, vp + i * 512);
+              const long long pair = cache_pair_at(page, h, p.c.heads, p.c.page_log2, off) + tok0;
+              const uint32_t pd = dst + 16 * D;
+              cp4(pd, p.c.k_pair + pair);
+              cp4(pd + 4, p.c.k_pair + pair + 2);
+              cp4(pd + 8, p.c.v_pair + pair);
+              cp4(pd + 12, p.c.v_pair + pair + 2);
+            } else {
+              bad |= 1u << stage;
+              if (first < rq.len && lane == 0) atomicExch(&g_attend_status, kBadPage);
+            }
+          }
+          cp_commit();
+        };
+#pragma unroll
+        for (int k = 0; k < S::kStages - 1; ++k) load(k);
+
+        for (int k = 0; k < iters; ++k) {
+          cp_wait<S::kStages - 2>();
+          const int stage = k % S::kStages;
+          const bool missing = (bad >> stage) & 1u;
+          load(k + S::kStages - 1);
+          const uint32_t at = ring_at + stage * S::kStage + lane * 16;
+
+          // ---- scores
+          float acc[NT][2][4];
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) acc[n][i >> 2][i & 3] = 0.f;
+          const uint4 pr = lds128(at + 16 * D);
+          auto qk = [&](uint32_t x, uint32_t y, int w) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              const uint4 q = lds128(q_at + (n * S::kWords + w) * 512);
+              mma16(acc[n][0], x & 0x000F000Fu, y & 0x000F000Fu, x & 0x00F000F0u, y & 0x00F000F0u, q.x, q.y);
+              mma16(acc[n][1], (x >> 8) & 0x000F000Fu, (y >> 8) & 0x000F000Fu, (x >> 8) & 0x00F000F0u,
+                    (y >> 8) & 0x00F000F0u, q.z, q.w);
+            }
+          };
+          if constexpr (D == 64) {
+            const uint4 a = lds128(at);
+            qk(a.x, a.z, 0);
+            qk(a.y, a.w, 1);
+          } else {
+#pragma unroll
+            for (int i = 0; i < S::kPieces; i += 2) {
+              const uint4 a = lds128(at + i * 512), c = lds128(at + (i + 1) * 512);
+              qk(a.x, c.x, i * 2);
+              qk(a.y, c.y, i * 2 + 1);
+              qk(a.z, c.z, i * 2 + 2);
+              qk(a.w, c.w, i * 2 + 3);
+            }
+          }
+
+          // ---- probabilities
+          const int first = span.id(i0 + warp + k * kWarps) * kTile;
+          const float2 k0 = lo_step<T>(pr.x), k1 = lo_step<T>(pr.y);
+          float2 v0 = lo_step<T>(pr.z), v1 = lo_step<T>(pr.w);
+          float x[NT][4];
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float2 kk = e < 2 ? k0 : k1;
+              x[n][e] = fmaf(kk.y, (acc[n][0][e] + acc[n][1][e]) * qf[n][e & 1], kk.x * qs[n][e & 1]);
+            }
+          const bool whole = !missing && first + kTile <= first_pos + 1 && first + kTile <= rq.len &&
+                             (p.window == 0 || first > last_pos - p.window || first + kTile <= p.sinks);
+          bool seen0 = true, seen1 = true;       // some row of this lane sees the token
+          uint32_t hidden = 0;
+          if (!whole) {
+            seen0 = seen1 = false;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int j = first + tok0 + (e < 2 ? 0 : 2);
+                const bool see = !missing && token_seen(j, pos[n][e & 1], rq.len, p.window, p.sinks);
+                if (!see) x[n][e] = -INFINITY, hidden |= 1u << (4 * n + e);
+                else if (e < 2) seen0 = true;
+                else seen1 = true;
+              }
+            // what lies in hidden places may be anything, NaN too
+            if (!seen0) v0 = make_float2(0.f, 0.f);
+            if (!seen1) v1 = make_float2(0.f, 0.f);
+          }
+          bool grow = fmaxf(v0.y, v1.y) > sig || sig == 0.f;
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) grow |= x[n][e] > m[n][e & 1] + kLazy;
+          if (__any_sync(0xffffffffu, grow)) {
+            float vs = fmaxf(fmaxf(v0.y, v1.y), kMinStep);
+#pragma unroll
+            for (int s = 16; s; s >>= 1) vs = fmaxf(vs, __shfl_xor_sync(0xffffffffu, vs, s));
+            const float sig_new = fmaxf(sig, pow2_above(vs));
+            const float beta = sig / sig_new;
+            sig = sig_new;
+            inv_sig = 1.f / sig;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                float top = fmaxf(x[n][e], x[n][e + 2]);
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                const float m_new = fmaxf(m[n][e], top);
+                const float alpha = m_new == -INFINITY ? 1.f : ex2(m[n][e] - m_new);
+                m[n][e] = m_new;
+                l[n][e] *= alpha;
+                pm[n][e] *= alpha;
+                const float ab = alpha * beta;
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) o[n][i][e] *= ab, o[n][i][e + 2] *= ab;
+              }
+          }
+          uint32_t bf[NT][2];
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            float w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float2 vv = e < 2 ? v0 : v1;
+              const float mm = m[n][e & 1];
+              const float pr_ = ex2(x[n][e] - (mm == -INFINITY ? 0.f : mm));
+              const bool none = (hidden >> (4 * n + e)) & 1u;
+              l[n][e & 1] += pr_;
+              pm[n][e & 1] += none ? 0.f : pr_ * vv.x;
+              w[e] = none ? 0.f : pr_ * (vv.y * inv_sig);
+            }
+            bf[n][0] = transpose8x8(half2_of(w[0], w[1]));
+            bf[n][1] = transpose8x8(half2_of(w[2], w[3]));
+          }
+
+          // ---- values
+#pragma unroll
+          for (int i = 0; i < D / 64; ++i) {
+            const uint4 v = lds128(at + S::kPieces * 512 + i * 512);
+            uint32_t x01 = __byte_perm(v.x, v.y, 0x5410), y01 = __byte_perm(v.x, v.y, 0x7632);
+            uint32_t x23 = __byte_perm(v.z, v.w, 0x5410), y23 = __byte_perm(v.z, v.w, 0x7632);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+#pragma unroll
+              for (int n = 0; n < NT; ++n) {
+                mma16(o[n][i * 4 + 2 * j], x01 & 0x000F000Fu, y01 & 0x000F000Fu, x23 & 0x000F000Fu, y23 & 0x000F000Fu,
+                      bf[n][0], bf[n][1]);
+                mma16(o[n][i * 4 + 2 * j + 1], x01 & 0x00F000F0u, y01 & 0x00F000F0u, x23 & 0x00F000F0u,
+                      y23 & 0x00F000F0u, bf[n][0], bf[n][1]);
+              }
+              x01 >>= 8, y01 >>= 8, x23 >>= 8, y23 >>= 8;
+            }
+          }
+        }
+        cp_wait<0>();
+
+        // ---- the warps' results joined
+        float* fold = reinterpret_cast<float*>(ring + warp * S::kRing);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+#pragma unroll
+            for (int s = 4; s < 32; s <<= 1) {
+              l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], s);
+              pm[n][e] += __shfl_xor_sync(0xffffffffu, pm[n][e], s);
+            }
+            const int r = n * 8 + 2 * t4 + e;
+            if (g == 0) warp_ml[warp * kRows + r] = make_float2(m[n][e], l[n][e]);
+            const float back = 16777216.f * sig;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+              const float f = i & 1 ? back * 0.0625f : back;
+              const int d = (i >> 2) * 64 + 8 * g + (i & 3);
+              fold[r * (D + 4) + d] = fmaf(o[n][i][e], f, pm[n][e]);
+              fold[r * (D + 4) + d + 4] = fmaf(o[n][i][e + 2], f, pm[n][e]);
+            }
+          }
+        __syncthreads();
+        const bool starts = i0 == 0, ends = i1 == span.tiles;
+        const long long slot = 2LL * blockIdx.x + (starts ? 1 : 0);
+        for (int i = tid; i < n_rows * (D / 2); i += kWarps * 32) {
+          const int r = i / (D / 2), d = 2 * (i % (D / 2));
+          float top = -INFINITY;
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) top = fmaxf(top, warp_ml[w * kRows + r].x);
+          float sum = 0.f, a = 0.f, c = 0.f;
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) {
+            const float2 ml = warp_ml[w * kRows + r];
+            const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : ex2(ml.x - top);
+            const float* part = reinterpret_cast<const float*>(ring + w * S::kRing) + r * (D + 4) + d;
+            sum = fmaf(ml.y, f, sum);
+            a = fmaf(part[0], f, a);
+            c = fmaf(part[1], f, c);
+          }
+          if (starts && ends) {
+            const long long tok = rq.row0 + (r0 + r) / p.G;
+            const int head = h * p.G + int((r0 + r) % p.G);
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            const uint32_t lo = DType<T>::from_float(gated<T>(a * inv, p, tok, head, d));
+            const uint32_t hi = DType<T>::from_float(gated<T>(c * inv, p, tok, head, d + 1));
+            *reinterpret_cast<uint32_t*>(p.out + tok * p.out_token + (long long)head * p.out_head + d) = lo | (hi << 16);
+          } else {
+            *reinterpret_cast<float2*>(p.part_o + (slot * kRows + r) * D + d) = make_float2(a, c);
+            if (d == 0) p.part_ml[slot * kRows + r] = make_float2(top, sum);
+          }
+        }
+        if (starts && !ends && tid == 0) {
+          const long long last = (req_at + span.tiles - 1) / share;
+          p.meta[blockIdx.x] = make_int4(int(last), b, h, int(r0 / kRows));
+        }
+        req_at += span.tiles;
+        cur = min(req_at, stop);
+      }
+    }
+  }
+}
+
+// Joins the parts of the item that block blockIdx.x began and others went on with; one row per block of threads.
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(D / 2) attend_join_kernel(const __grid_constant__ AttendParams p) {
+  constexpr int kRows = 8 * NT;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int4 meta = p.meta[blockIdx.x];
+  if (meta.x == 0) return;
+  const int c0 = blockIdx.x, c1 = meta.x, b = meta.y, h = meta.z, r = blockIdx.y, d = 2 * threadIdx.x;
+  const Request rq = request_of(p, b);
+  const long long row = (long long)meta.w * kRows + r;
+  if (row >= (long long)rq.rows * p.G) return;
+  auto slot = [&](int c) { return (c == c0 ? 2LL * c + 1 : 2LL * c) * kRows + r; };
+  float top = -INFINITY;
+  for (int c = c0; c <= c1; ++c) top = fmaxf(top, p.part_ml[slot(c)].x);
+  float sum = 0.f, x = 0.f, y = 0.f;
+  for (int c = c0; c <= c1; ++c) {
+    const float2 ml = p.part_ml[slot(c)];
+    const float2 o = *reinterpret_cast<const float2*>(p.part_o + slot(c) * D + d);
+    const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : ex2(ml.x - top);
+    sum = fmaf(ml.y, f, sum);
+    x = fmaf(o.x, f, x);
+    y = fmaf(o.y, f, y);
+  }
+  const long long tok = rq.row0 + row / p.G;
+  const int head = h * p.G + int(row % p.G);
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const uint32_t lo = DType<T>::from_float(gated<T>(x * inv, p, tok, head, d));
+  const uint32_t hi = DType<T>::from_float(gated<T>(y * inv, p, tok, head, d + 1));
+  *reinterpret_cast<uint32_t*>(p.out + tok * p.out_token + (long long)head * p.out_head + d) = lo | (hi << 16);
+}
+
+template <typename T, int D, int NT>
+int launch(AttendParams p, int blocks, cudaStream_t st) {
+  using S = Shape<D, NT>;
+  B200LUT_CUDA_OK(cudaFuncSetAttribute(attend_rows_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+  attend_rows_kernel<T, D, NT><<<unsigned(blocks), kWarps * 32, S::kSmem, st>>>(p);
+  B200LUT_CUDA_OK(cudaGetLastError());
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(blocks), S::kRows);
+  cfg.blockDim = dim3(D / 2);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr, cfg.numAttrs = 1;
+  B200LUT_CUDA_OK(cudaLaunchKernelEx(&cfg, attend_join_kernel<T, D, NT>, p));
+  return B200LUT_OK;
+}
+
+template <typename T, int D>
+int pick_rows(const AttendParams& p, int blocks, cudaStream_t st) {
+  return p.G <= 8 && !p.row_start ? launch<T, D, 1>(p, blocks, st) : launch<T, D, 2>(p, blocks, st);
+}
+
+template <typename T>
+int pick_dim(const AttendParams& p, int blocks, cudaStream_t st) {
+  return p.c.D == 64 ? pick_rows<T, 64>(p, blocks, st) : p.c.D == 128 ? pick_rows<T, 128>(p, blocks, st)
+                                                                      : pick_rows<T, 256>(p, blocks, st);
+}
+
+int blocks_of(int sms) { return 2 * sms; }
+
+}  // namespace
+
+int attend_status_take() {
+  int v = 0, zero = 0;
+  if (cudaMemcpyFromSymbol(&v, g_attend_status, sizeof(int)) != cudaSuccess) return -1;
+  if (v != 0) cudaMemcpyToSymbol(g_attend_status, &zero, sizeof(int));
+  return v;
+}
+
+size_t attend_rows_workspace(int D, int sms) {
+  const size_t n = size_t(blocks_of(sms));
+  return n * 16 + 2 * n * 16 * 8 + 2 * n * 16 * size_t(D) * 4;
+}
+
+int attend_rows(const AttendParams& q, int dtype, int sms, void* ws, void* stream) {
+  AttendParams p = q;
+  const int blocks = blocks_of(sms);
+  p.meta = static_cast<int4*>(ws);
+  p.part_ml = reinterpret_cast<float2*>(p.meta + blocks);
+  p.part_o = reinterpret_cast<float*>(p.part_ml + 2LL * blocks * 16);
+  const cudaStream_t st = cudaStream_t(stream);
+  return dtype == B200LUT_BF16 ? pick_dim<__nv_bfloat16>(p, blocks, st) : pick_dim<__half>(p, blocks, st);
+}
+
+}  // namespace b200lut
+
+using namespace b200lut;
+
+extern "C" size_t b200lut_attend_workspace_bytes(int n_heads, int n_kv_heads, int head_dim) {
+  if (n_heads < 1 || n_kv_heads < 1 || n_heads % n_kv_heads || (head_dim != 64 && head_dim != 128 && head_dim != 256)) return 0;
+  return attend_rows_workspace(head_dim, b200lut_sm_count());
+}
+
+extern "C" int b200lut_attend(const b200lut_attend_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+  B200LUT_REQUIRE(a, B200LUT_ERR_INVALID, "attend: null argument");
+  AttendParams p = {};
+  const int rc = check_cache(a->cache, "attend", &p.c);
+  if (rc != B200LUT_OK) return rc;
+  B200LUT_REQUIRE(a->T >= 0 && a->B >= 0, B200LUT_ERR_INVALID, "attend: T and B must not be negative");
+  B200LUT_REQUIRE(a->n_heads >= 1 && a->n_heads % p.c.heads == 0, B200LUT_ERR_INVALID,
+                  "attend: n_heads %d is not a multiple of the cache's %d heads", a->n_heads, p.c.heads);
+  B200LUT_REQUIRE(a->n_heads / p.c.heads <= 64, B200LUT_ERR_UNSUPPORTED,
+                  "attend: at most 64 query heads per key/value head (got %d)", a->n_heads / p.c.heads);
+  B200LUT_REQUIRE(a->window >= 0 && a->sinks >= 0 && a->width >= 1 && a->B <= 65536, B200LUT_ERR_INVALID,
+                  "attend: window and sinks must not be negative, width must be positive, B at most 65536");
+  if (a->T == 0 || a->B == 0) return B200LUT_OK;
+  B200LUT_REQUIRE(a->q && a->out && a->block_table && a->kv_len, B200LUT_ERR_INVALID, "attend: null argument");
+  B200LUT_REQUIRE(a->row_start || a->T == a->B, B200LUT_ERR_INVALID,
+                  "attend: without row_start there is one row per request (T %d, B %d)", a->T, a->B);
+  B200LUT_REQUIRE(aligned16(a->q) && aligned16(a->out) && (!a->gate || aligned16(a->gate)) && a->q_token_stride % 8 == 0 &&
+                      a->q_head_stride % 8 == 0 && a->out_token_stride % 8 == 0 && a->out_head_stride % 8 == 0 &&
+                      (!a->gate || (a->gate_token_stride % 8 == 0 && a->gate_head_stride % 8 == 0)),
+                  B200LUT_ERR_ALIGN, "attend: rows must be 16-byte aligned (pointers and strides)");
+  const int sms = b200lut_sm_count();
+  B200LUT_REQUIRE(workspace && aligned16(workspace) &&
+                      workspace_bytes >= attend_rows_workspace(p.c.D, sms),
+                  B200LUT_ERR_WORKSPACE, "attend: workspace of b200lut_attend_workspace_bytes() wanted");
+  p.q = static_cast<const uint16_t*>(a->q), p.gate = static_cast<const uint16_t*>(a->gate);
+  p.out = static_cast<uint16_t*>(a->out);
+  p.q_token = a->q_token_stride, p.q_head = a->q_head_stride;
+  p.gate_token = a->gate_token_stride, p.gate_head = a->gate_head_stride;
+  p.out_token = a->out_token_stride, p.out_head = a->out_head_stride;
+  p.table = a->block_table, p.table_ld = a->table_stride, p.kv_len = a->kv_len, p.row_start = a->row_start;
+  p.T = a->T, p.B = a->B, p.Hq = a->n_heads, p.G = a->n_heads / p.c.heads, p.width = a->width;
+  p.window = a->window, p.sinks = a->sinks;
+  p.scale = a->scale * 1.4426950408889634f;
+  return attend_rows(p, a->cache->dtype, sms, workspace, stream);
+}

@@ -1,0 +1,82 @@
+// Shared by the kernels that attend over the 4-bit cache.
+//
+//   s_rj = scale * q_r . k_j,  k_j = lo_j + step_j c_j  =>  s_rj = scale * (step_j (q_r . c_j) + lo_j sum(q_r))
+//   o_r  = sum_j p_rj v_j / sum_j p_rj                  =   (sum_j (p_rj step_j) c_j + sum_j p_rj lo_j) / sum_j p_rj
+//
+// so the matrix products run on the 4-bit codes themselves and a token's two parameters enter the scores and
+// the probabilities, not the elements: nothing of K or V is rounded. A code needs one AND to become an
+// operand: in the low bits of a half it is the subnormal c * 2^-24, four bits higher c * 2^-20, both exact,
+// and the powers of two go into q and the result.
+// q is multiplied by the power of two that puts its row's largest element into [2^13, 2^14): fp16 then
+// holds bf16's eight bits exactly down to 2^-28 of the largest element (and fp16's eleven to 2^-25).
+// p * step is rounded to fp16 (2^-12) after division by a power of two >= the largest step so far.
+#pragma once
+
+#include "kvcache.cuh"
+
+namespace b200lut {
+
+struct AttendParams {
+  const uint16_t* q;
+  const uint16_t* gate;        // or null
+  uint16_t* out;
+  long long q_token, q_head, gate_token, gate_head, out_token, out_head;    // strides in elements
+  CacheView c;
+  const int* table;
+  const int* kv_len;
+  const int* row_start;        // or null: one row per request
+  long long table_ld;
+  int T, B, Hq, G, width, window, sinks;
+  float scale;                 // scale * log2(e)
+  // workspace of the split kernel
+  int4* meta;
+  float2* part_ml;
+  float* part_o;
+};
+
+// The requests' rows and lengths as the kernels read them (device data: clamped, never trusted).
+struct Request {
+  int row0, rows, len;         // first row, rows, cached tokens with them
+};
+__device__ __forceinline__ Request request_of(const AttendParams& p, int b) {
+  Request r;
+  r.row0 = p.row_start ? min(max(0, p.row_start[b]), p.T) : b;
+  r.rows = p.row_start ? max(0, min(p.row_start[b + 1], p.T) - r.row0) : 1;
+  const long long room = (long long)p.width << p.c.page_log2;
+  const int len = max(0, p.kv_len[b]);
+  r.len = int(min((long long)len, room));
+  return r;
+}
+
+// Tiles of kTile tokens that rows at positions [first, last] of a request see: ids 0 .. sink_tiles - 1, then from
+// main0 on. At least one, so that a row that sees nothing is written.
+template <int kTile>
+struct Span {
+  int sink_tiles, main0, tiles;
+  __device__ __forceinline__ Span(int first, int last, int len, int window, int sinks) {
+    const int hi = min(len, last + 1);                       // tokens below hi
+    const int lo = window ? max(0, first - window + 1) : 0;
+    const int s = min(min(sinks, lo), max(hi, 0));
+    sink_tiles = (s + kTile - 1) / kTile;
+    main0 = max(lo / kTile, sink_tiles);
+    const int main1 = (max(hi, 0) + kTile - 1) / kTile;
+    tiles = max(1, sink_tiles + max(0, main1 - main0));
+  }
+  __device__ __forceinline__ int id(int i) const { return i < sink_tiles ? i : main0 + i - sink_tiles; }
+};
+
+__device__ __forceinline__ bool token_seen(int j, int pos, int len, int window, int sinks) {
+  return j <= pos && j < len && (window == 0 || j > pos - window || j < sinks);
+}
+
+template <typename T>
+__device__ __forceinline__ float gated(float o, const AttendParams& p, long long token, int head, int d) {
+  if (!p.gate) return o;
+  const float g = DType<T>::to_float(p.gate[token * p.gate_token + (long long)head * p.gate_head + d]);
+  return o / (1.f + __expf(-g));
+}
+
+int attend_rows(const AttendParams& p, int dtype, int sms, void* ws, void* stream);
+size_t attend_rows_workspace(int D, int sms);
+
+}  // namespace b200lut

@@ -1045,7 +1045,9 @@ extern "C" int b200lut_device_status(void) {
   const int e = b200lut::exchange_status_take();
   const int g = b200lut::embed_status_take();
   const int c = b200lut::gemm_cluster_status_take();
-  return v != 0 ? v : (c != 0 ? c : (e != 0 ? e : g));
+  const int s = b200lut::kv_status_take();
+  const int a = b200lut::attend_status_take();
+  return v != 0 ? v : c != 0 ? c : e != 0 ? e : g != 0 ? g : s != 0 ? s : a;
 }
 
 namespace {

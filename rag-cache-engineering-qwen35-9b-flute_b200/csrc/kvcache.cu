@@ -1,0 +1,302 @@
+// The paged 4-bit key/value cache: the step plan (row starts, positions, page assignment and slots from the
+// requests' lengths, on the device), rows written and rows read back. Layout: kvcache.cuh.
+#include "kvcache.cuh"
+
+namespace b200lut {
+namespace {
+
+__device__ int g_kv_status = 0;
+constexpr int kBadSlot = 0x6100;
+
+// ---- step plan ------------------------------------------------------------------------------------------
+// One launch: every block scans all requests (two sums: new tokens and pages wanted; a scan over 1024
+// requests is one block-wide scan), then fills its share of the tokens. A token's page is either an entry of
+// the request's row or, past the pages it has, the next of the free list, so no block waits for another; the
+// entry of a fresh page is written by the thread of that page's first token.
+struct PlanParams {
+  const int *cached, *fresh;
+  int* table;
+  const int *free_pages, *taken;
+  int *row_start, *kv_len, *positions, *slots, *taken_out;
+  uint8_t* served;
+  int B, width, free_count, page_log2, max_tokens;
+};
+
+constexpr int kUnserved = INT32_MIN;
+
+__global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ PlanParams p) {
+  extern __shared__ int sm[];
+  int* end = sm;                 // [B] tokens up to and with request b, clamped to 2^31 - 1
+  int* base = sm + p.B;          // [B] free-list index of page j of request b, less j; kUnserved
+  __shared__ long long warp_tokens[32], warp_pages[32];
+  __shared__ int taken_max;
+  const int n = blockDim.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, P = 1 << p.page_log2;
+  const int taken = max(0, *p.taken);
+  if (tid == 0) taken_max = taken;
+  long long carry_tokens = 0, carry_pages = taken;
+  for (int b0 = 0; b0 < p.B; b0 += n) {
+    const int b = b0 + tid;
+    long long cached = 0, fresh = 0;
+    if (b < p.B) cached = max(0, p.cached[b]), fresh = max(0, p.fresh[b]);
+    // tokens first: whether a request fits depends on where its rows end
+    long long tok = fresh;
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long v = __shfl_up_sync(0xffffffffu, tok, o);
+      if (lane >= o) tok += v;
+    }
+    if (lane == 31) warp_tokens[warp] = tok;
+    __syncthreads();
+    long long before = carry_tokens;
+    for (int w = 0; w < n / 32; ++w) {
+      if (w < warp) before += warp_tokens[w];
+      carry_tokens += warp_tokens[w];
+    }
+    tok += before;
+    const long long have = (cached + P - 1) >> p.page_log2, want = (cached + fresh + P - 1) >> p.page_log2;
+    const bool fits = b < p.B && want <= p.width && tok <= p.max_tokens;
+    const long long need = fits ? want - have : 0;
+    long long pg = need;
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long v = __shfl_up_sync(0xffffffffu, pg, o);
+      if (lane >= o) pg += v;
+    }
+    if (lane == 31) warp_pages[warp] = pg;
+    __syncthreads();
+    long long used = carry_pages;
+    for (int w = 0; w < n / 32; ++w) {
+      if (w < warp) used += warp_pages[w];
+      carry_pages += warp_pages[w];
+    }
+    pg += used;
+    if (b < p.B) {
+      const bool served = fits && (need == 0 || pg <= p.free_count);
+      end[b] = int(min(tok, (long long)INT32_MAX));
+      base[b] = served ? int(pg - need - have) : kUnserved;
+      if (served && need > 0) atomicMax(&taken_max, int(pg));
+      if (blockIdx.x == 0) {
+        p.row_start[b] = int(min(tok - fresh, (long long)p.max_tokens));
+        if (b == p.B - 1) p.row_start[p.B] = int(min(tok, (long long)p.max_tokens));
+        p.kv_len[b] = int(served ? cached + fresh : cached);
+        p.served[b] = served ? 1 : 0;
+      }
+    }
+    __syncthreads();
+  }
+  if (blockIdx.x == 0 && tid == 0) *p.taken_out = taken_max;
+  const int total = end[p.B - 1];
+  for (int t = blockIdx.x * n + tid; t < p.max_tokens; t += gridDim.x * n) {
+    int pos = 0, slot = -1;
+    if (t < total) {
+      int lo = 0, hi = p.B - 1;                  // first request that ends behind t
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (end[mid] > t) hi = mid;
+        else lo = mid + 1;
+      }
+      const int b = lo, cached = max(0, p.cached[b]);
+      // of a request that is not the first in a clamped sum, the start is exact whenever t lies in it
+      const int start = b ? end[b - 1] : 0;
+      pos = cached + (t - start);
+      if (base[b] != kUnserved) {
+        const int j = pos >> p.page_log2;
+        int* entry = p.table + (long long)b * p.width + j;
+        int page;
+        if (j >= int(((long long)cached + P - 1) >> p.page_log2)) {
+          page = p.free_pages[base[b] + j];
+          if ((pos & (P - 1)) == 0) *entry = page;
+        } else {
+          page = *entry;
+        }
+        if (page >= 0) slot = (page << p.page_log2) + (pos & (P - 1));
+      }
+    }
+    p.positions[t] = pos;
+    p.slots[t] = slot;
+  }
+}
+
+// ---- rows in ------------------------------------------------------------------------------------------
+// A row is D/8 lanes of eight elements: two shuffle reductions give lo and hi, then each lane writes the one
+// 32-bit word of codes its elements make. 15 (x - lo) / (hi - lo) is an IEEE division: codes on a border
+// (frequent with 8-bit significands) are decided as the definition does, half to even. Bound by memory: the
+// rows are read once.
+constexpr int kRowWarps = 8;
+constexpr float kRangeLimit = 1.329227996e36f;     // 2^120: 15 times a range below it is finite
+
+template <typename T>
+__global__ void __launch_bounds__(kRowWarps * 32) kv_write_kernel(const uint16_t* k, const uint16_t* v, long long kt,
+                                                                  long long kh, long long vt, long long vh,
+                                                                  const int* slots, int tokens, CacheView c) {
+  const int lane = threadIdx.x & 31, lanes = c.D >> 3, per = 32 / lanes, at = lane % lanes;
+  const long long row = ((long long)blockIdx.x * kRowWarps + (threadIdx.x >> 5)) * per + lane / lanes;
+  const long long rows = (long long)tokens * c.heads * 2;
+  const bool in = row < rows;
+  const bool value = row >= rows / 2;
+  const long long r = in ? (value ? row - rows / 2 : row) : 0;
+  const long long t = r / c.heads;
+  const int h = int(r - t * c.heads);
+  const int slot = in ? slots[t] : -1;
+  uint4 raw = make_uint4(0, 0, 0, 0);
+  if (slot >= 0) raw = __ldg(reinterpret_cast<const uint4*>(value ? v + t * vt + h * vh : k + t * kt + h * kh) + at);
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  float x[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = DType<T>::to_float(uint16_t(w[e >> 1] >> (16 * (e & 1))));
+  float lo = x[0], hi = x[0], bad = x[0] - x[0];         // 0, or NaN where an element is not finite
+#pragma unroll
+  for (int e = 1; e < 8; ++e) lo = fminf(lo, x[e]), hi = fmaxf(hi, x[e]), bad += x[e] - x[e];
+  for (int o = lanes >> 1; o; o >>= 1) {
+    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    bad += __shfl_xor_sync(0xffffffffu, bad, o);
+  }
+  const float range = hi - lo;
+  const bool finite = bad == 0.f && range < kRangeLimit;
+  uint32_t word = 0;
+  if (finite && range > 0.f) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) word |= uint32_t(rintf(__fdiv_rn(15.f * (x[e] - lo), range))) << (4 * e);
+  }
+  if (slot < 0) return;
+  if (slot >= (c.n_pages << c.page_log2)) {
+    if (at == 0) atomicExch(&g_kv_status, kBadSlot);
+    return;
+  }
+  const int page = slot >> c.page_log2, offset = slot & ((1 << c.page_log2) - 1);
+  uint8_t* codes = (value ? c.v : c.k) + cache_codes_at(page, h, c.heads, c.page_log2, c.D);
+  *reinterpret_cast<uint32_t*>(codes + (value ? value_word_at(offset, at, c.D) : key_word_at(offset, at, c.D))) = word;
+  if (at == 0)
+    (value ? c.v_pair : c.k_pair)[cache_pair_at(page, h, c.heads, c.page_log2, offset)] =
+        finite ? uint32_t(DType<T>::from_float(lo)) | (uint32_t(DType<T>::from_float(hi)) << 16) : 0x7FFF7FFFu;
+}
+
+// ---- rows out -----------------------------------------------------------------------------------------
+template <typename T>
+__global__ void __launch_bounds__(kRowWarps * 32) kv_read_kernel(uint16_t* k, uint16_t* v, const int* slots, int tokens,
+                                                                 CacheView c) {
+  const int lane = threadIdx.x & 31, lanes = c.D >> 3, per = 32 / lanes, at = lane % lanes;
+  const long long row = ((long long)blockIdx.x * kRowWarps + (threadIdx.x >> 5)) * per + lane / lanes;
+  const long long rows = (long long)tokens * c.heads * 2;
+  if (row >= rows) return;
+  const bool value = row >= rows / 2;
+  const long long r = value ? row - rows / 2 : row, t = r / c.heads;
+  const int h = int(r - t * c.heads), slot = slots[t];
+  uint32_t out[4] = {0, 0, 0, 0};
+  if (slot >= (c.n_pages << c.page_log2)) {
+    if (at == 0) atomicExch(&g_kv_status, kBadSlot);
+  } else if (slot >= 0) {
+    const int page = slot >> c.page_log2, offset = slot & ((1 << c.page_log2) - 1);
+    const uint8_t* codes = (value ? c.v : c.k) + cache_codes_at(page, h, c.heads, c.page_log2, c.D);
+    const uint32_t word = *reinterpret_cast<const uint32_t*>(
+        codes + (value ? value_word_at(offset, at, c.D) : key_word_at(offset, at, c.D)));
+    const float2 ls = lo_step<T>((value ? c.v_pair : c.k_pair)[cache_pair_at(page, h, c.heads, c.page_log2, offset)]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      out[e >> 1] |= uint32_t(DType<T>::from_float(fmaf(float((word >> (4 * e)) & 15u), ls.y, ls.x))) << (16 * (e & 1));
+  }
+  reinterpret_cast<uint4*>((value ? v : k) + r * c.D)[at] = make_uint4(out[0], out[1], out[2], out[3]);
+}
+
+}  // namespace
+
+int kv_status_take() {
+  int v = 0, zero = 0;
+  if (cudaMemcpyFromSymbol(&v, g_kv_status, sizeof(int)) != cudaSuccess) return -1;
+  if (v != 0) cudaMemcpyToSymbol(g_kv_status, &zero, sizeof(int));
+  return v;
+}
+
+int check_cache(const b200lut_kv_cache* c, const char* who, CacheView* v) {
+  B200LUT_REQUIRE(c && c->k_codes && c->v_codes && c->k_pairs && c->v_pairs, B200LUT_ERR_INVALID, "%s: null cache", who);
+  B200LUT_REQUIRE(c->dtype == B200LUT_BF16 || c->dtype == B200LUT_F16, B200LUT_ERR_INVALID,
+                  "%s: dtype must be B200LUT_BF16 or B200LUT_F16", who);
+  B200LUT_REQUIRE(c->head_dim == 64 || c->head_dim == 128 || c->head_dim == 256, B200LUT_ERR_UNSUPPORTED,
+                  "%s: head_dim must be 64, 128 or 256 (got %d)", who, c->head_dim);
+  B200LUT_REQUIRE(c->page_size >= 16 && c->page_size <= 256 && (c->page_size & (c->page_size - 1)) == 0,
+                  B200LUT_ERR_UNSUPPORTED, "%s: page_size must be 16, 32, 64, 128 or 256 (got %d)", who, c->page_size);
+  B200LUT_REQUIRE(c->n_kv_heads >= 1 && c->n_kv_heads <= 4096 && c->n_pages >= 1 &&
+                      (long long)c->n_pages * c->page_size <= 0x7fffffffLL,
+                  B200LUT_ERR_INVALID, "%s: 1 to 4096 heads and fewer than 2^31 slots wanted", who);
+  B200LUT_REQUIRE(aligned16(c->k_codes) && aligned16(c->v_codes) && aligned16(c->k_pairs) && aligned16(c->v_pairs),
+                  B200LUT_ERR_ALIGN, "%s: cache buffers must be 16-byte aligned", who);
+  v->k = static_cast<uint8_t*>(c->k_codes), v->v = static_cast<uint8_t*>(c->v_codes);
+  v->k_pair = static_cast<uint32_t*>(c->k_pairs), v->v_pair = static_cast<uint32_t*>(c->v_pairs);
+  v->n_pages = c->n_pages, v->heads = c->n_kv_heads, v->D = c->head_dim;
+  v->page_log2 = 31 - __builtin_clz(unsigned(c->page_size));
+  return B200LUT_OK;
+}
+
+}  // namespace b200lut
+
+using namespace b200lut;
+
+extern "C" int b200lut_kv_plan(const b200lut_kv_plan_args* a, void* stream) {
+  B200LUT_REQUIRE(a && a->cached && a->fresh && a->block_table && a->free_pages && a->taken && a->row_start && a->kv_len &&
+                      a->positions && a->slots && a->taken_out && a->served,
+                  B200LUT_ERR_INVALID, "kv_plan: null argument");
+  B200LUT_REQUIRE(a->B >= 1 && a->B <= 8192, B200LUT_ERR_UNSUPPORTED, "kv_plan: 1 to 8192 requests (got %d)", a->B);
+  B200LUT_REQUIRE(a->width >= 1 && a->free_count >= 0 && a->max_tokens >= 1, B200LUT_ERR_INVALID,
+                  "kv_plan: width and max_tokens must be positive, free_count not negative");
+  B200LUT_REQUIRE(a->page_size >= 16 && a->page_size <= 256 && (a->page_size & (a->page_size - 1)) == 0,
+                  B200LUT_ERR_UNSUPPORTED, "kv_plan: page_size must be 16, 32, 64, 128 or 256 (got %d)", a->page_size);
+  PlanParams p;
+  p.cached = a->cached, p.fresh = a->fresh, p.table = a->block_table, p.free_pages = a->free_pages, p.taken = a->taken;
+  p.row_start = a->row_start, p.kv_len = a->kv_len, p.positions = a->positions, p.slots = a->slots;
+  p.taken_out = a->taken_out, p.served = a->served;
+  p.B = a->B, p.width = a->width, p.free_count = a->free_count, p.max_tokens = a->max_tokens;
+  p.page_log2 = 31 - __builtin_clz(unsigned(a->page_size));
+  const int n = a->B <= 128 ? 128 : a->B <= 512 ? 512 : 1024;
+  long long grid = ((long long)a->max_tokens + n - 1) / n;
+  if (grid > 148) grid = 148;
+  const size_t smem = size_t(a->B) * 8;
+  if (smem > 40 * 1024)
+    B200LUT_CUDA_OK(cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 8192 * 8));
+  plan_kernel<<<unsigned(grid), n, smem, cudaStream_t(stream)>>>(p);
+  B200LUT_CUDA_OK(cudaGetLastError());
+  return B200LUT_OK;
+}
+
+extern "C" int b200lut_kv_write(const b200lut_kv_cache* cache, const void* k, const void* v, int64_t k_token_stride,
+                                int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride,
+                                const int32_t* slots, int tokens, void* stream) {
+  CacheView c;
+  const int rc = check_cache(cache, "kv_write", &c);
+  if (rc != B200LUT_OK) return rc;
+  B200LUT_REQUIRE(tokens >= 0 && (tokens == 0 || (k && v && slots)), B200LUT_ERR_INVALID, "kv_write: null argument");
+  B200LUT_REQUIRE(aligned16(k) && aligned16(v) && k_token_stride % 8 == 0 && k_head_stride % 8 == 0 &&
+                      v_token_stride % 8 == 0 && v_head_stride % 8 == 0,
+                  B200LUT_ERR_ALIGN, "kv_write: rows must be 16-byte aligned (pointers and strides)");
+  if (tokens == 0) return B200LUT_OK;
+  const long long rows = 2LL * tokens * c.heads, per = (256 / c.D) * kRowWarps, grid = (rows + per - 1) / per;
+  B200LUT_REQUIRE(grid <= 0x7fffffffLL, B200LUT_ERR_UNSUPPORTED, "kv_write: too many rows");
+  const auto* kk = static_cast<const uint16_t*>(k);
+  const auto* vv = static_cast<const uint16_t*>(v);
+  if (cache->dtype == B200LUT_BF16)
+    kv_write_kernel<__nv_bfloat16><<<unsigned(grid), kRowWarps * 32, 0, cudaStream_t(stream)>>>(
+        kk, vv, k_token_stride, k_head_stride, v_token_stride, v_head_stride, slots, tokens, c);
+  else
+    kv_write_kernel<__half><<<unsigned(grid), kRowWarps * 32, 0, cudaStream_t(stream)>>>(
+        kk, vv, k_token_stride, k_head_stride, v_token_stride, v_head_stride, slots, tokens, c);
+  B200LUT_CUDA_OK(cudaGetLastError());
+  return B200LUT_OK;
+}
+
+extern "C" int b200lut_kv_read(const b200lut_kv_cache* cache, void* k, void* v, const int32_t* slots, int tokens,
+                               void* stream) {
+  CacheView c;
+  const int rc = check_cache(cache, "kv_read", &c);
+  if (rc != B200LUT_OK) return rc;
+  B200LUT_REQUIRE(tokens >= 0 && (tokens == 0 || (k && v && slots)), B200LUT_ERR_INVALID, "kv_read: null argument");
+  B200LUT_REQUIRE(aligned16(k) && aligned16(v), B200LUT_ERR_ALIGN, "kv_read: outputs must be 16-byte aligned");
+  if (tokens == 0) return B200LUT_OK;
+  const long long rows = 2LL * tokens * c.heads, per = (256 / c.D) * kRowWarps, grid = (rows + per - 1) / per;
+  B200LUT_REQUIRE(grid <= 0x7fffffffLL, B200LUT_ERR_UNSUPPORTED, "kv_read: too many rows");
+  auto* kk = static_cast<uint16_t*>(k);
+  auto* vv = static_cast<uint16_t*>(v);
+  if (cache->dtype == B200LUT_BF16)
+    kv_read_kernel<__nv_bfloat16><<<unsigned(grid), kRowWarps * 32, 0, cudaStream_t(stream)>>>(kk, vv, slots, tokens, c);
+  else
+    kv_read_kernel<__half><<<unsigned(grid), kRowWarps * 32, 0, cudaStream_t(stream)>>>(kk, vv, slots, tokens, c);
+  B200LUT_CUDA_OK(cudaGetLastError());
+  return B200LUT_OK;
+}
