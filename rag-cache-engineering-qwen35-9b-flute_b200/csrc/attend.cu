@@ -24,6 +24,7 @@ constexpr int kBadPage = 0x6200;
 constexpr int kWarps = 8;
 constexpr int kTile = 16;
 constexpr float kLazy = 8.f;           // the running maximum may lag by this many powers of two
+constexpr uint32_t kOnes = 0x3C003C00u;     // two halves of 1
 constexpr float kMinStep = 7.888609e-31f;   // 2^-100
 
 template <int D, int NT>
@@ -223,6 +224,11 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) attend_rows_kern
           for (int i = 0; i < D / 16; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[n][i][e] = 0.f;
+        float ws[NT][4];             // sums of the rounded weights (every row of A is ones)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) ws[n][e] = 0.f;
         float sig = 0.f, inv_sig = 0.f;
 
         // ---- the ring
@@ -376,6 +382,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) attend_rows_kern
                 const float ab = alpha * beta;
 #pragma unroll
                 for (int i = 0; i < D / 16; ++i) o[n][i][e] *= ab, o[n][i][e + 2] *= ab;
+                ws[n][e] *= ab;
               }
           }
           uint32_t bf[NT][2];
@@ -389,11 +396,12 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) attend_rows_kern
               const float pr_ = ex2(x[n][e] - (mm == -INFINITY ? 0.f : mm));
               const bool none = (hidden >> (4 * n + e)) & 1u;
               l[n][e & 1] += pr_;
-              pm[n][e & 1] += none ? 0.f : pr_ * vv.x;
+              pm[n][e & 1] += none ? 0.f : pr_ * fmaf(7.5f, vv.y, vv.x);
               w[e] = none ? 0.f : pr_ * (vv.y * inv_sig);
             }
             bf[n][0] = transpose8x8(half2_of(w[0], w[1]));
             bf[n][1] = transpose8x8(half2_of(w[2], w[3]));
+            mma16(ws[n], kOnes, kOnes, kOnes, kOnes, bf[n][0], bf[n][1]);
           }
 
           // ---- values
@@ -430,13 +438,13 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) attend_rows_kern
             }
             const int r = n * 8 + 2 * t4 + e;
             if (g == 0) warp_ml[warp * kRows + r] = make_float2(m[n][e], l[n][e]);
-            const float back = 16777216.f * sig;
+            const float back = 16777216.f * sig, mid = fmaf(-7.5f * sig, ws[n][e], pm[n][e]);
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) {
               const float f = i & 1 ? back * 0.0625f : back;
               const int d = (i >> 2) * 64 + 8 * g + (i & 3);
-              fold[r * (D + 4) + d] = fmaf(o[n][i][e], f, pm[n][e]);
-              fold[r * (D + 4) + d + 4] = fmaf(o[n][i][e + 2], f, pm[n][e]);
+              fold[r * (D + 4) + d] = fmaf(o[n][i][e], f, mid);
+              fold[r * (D + 4) + d + 4] = fmaf(o[n][i][e + 2], f, mid);
             }
           }
         __syncthreads();
@@ -514,7 +522,13 @@ __global__ void __launch_bounds__(D / 2) attend_join_kernel(const __grid_constan
 template <typename T, int D, int NT>
 int launch(AttendParams p, int blocks, cudaStream_t st) {
   using S = Shape<D, NT>;
-  B200LUT_CUDA_OK(cudaFuncSetAttribute(attend_rows_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+  static bool configured[64] = {false};
+  int dev = 0;
+  B200LUT_CUDA_OK(cudaGetDevice(&dev));
+  if (dev >= 64 || !configured[dev]) {
+    B200LUT_CUDA_OK(cudaFuncSetAttribute(attend_rows_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+    if (dev < 64) configured[dev] = true;
+  }
   attend_rows_kernel<T, D, NT><<<unsigned(blocks), kWarps * 32, S::kSmem, st>>>(p);
   B200LUT_CUDA_OK(cudaGetLastError());
   cudaLaunchConfig_t cfg = {};

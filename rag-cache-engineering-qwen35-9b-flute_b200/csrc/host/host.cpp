@@ -5,8 +5,10 @@
 // here do the same work for the shapes and dtypes that need no conversion: look the module's native
 // description up, allocate the outputs, call the C entries. They return None, having launched
 // nothing, when a call is not one of those; the Python route then runs.
+#include <cmath>
 #include <cstring>
 
+#include "attention.h"
 #include "merged.h"
 
 using namespace b200host;
@@ -37,6 +39,7 @@ static PyObject* reduce_none(PyObject*, PyObject*) {
 static PyMethodDef reduce_methods[] = {{"__reduce__", reduce_none, METH_NOARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
 
 PyTypeObject LayerType = {PyVarObject_HEAD_INIT(nullptr, 0)};
+PyTypeObject CacheType = {PyVarObject_HEAD_INIT(nullptr, 0)};
 
 static int ready_type(PyTypeObject* t, const char* name, size_t size, destructor d) {
   t->tp_name = name;
@@ -390,6 +393,18 @@ static PyObject* workspace(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// ---- the attention side (attention.h) -----------------------------------------------------------------
+#define ATTENTION_SIDE(f)                                                              \
+  static PyObject* f##_entry(PyObject*, PyObject* const* a, Py_ssize_t n) {            \
+    return f([](auto&& body) { return guarded(body); }, context, a, n);                \
+  }
+ATTENTION_SIDE(kv_write)
+ATTENTION_SIDE(kv_read)
+ATTENTION_SIDE(kv_plan)
+ATTENTION_SIDE(attend)
+ATTENTION_SIDE(rotary)
+#undef ATTENTION_SIDE
+
 static PyObject* set_library_error(PyObject*, PyObject* type) {
   Py_INCREF(type);
   Py_XDECREF(g_library_error);
@@ -406,6 +421,12 @@ static PyMethodDef methods[] = {{"bind", FAST(bind)},
                                 {"embed", FAST(embed)},
                                 {"fht", FAST(fht)},
                                 {"workspace", FAST(workspace)},
+                                {"bind_cache", FAST(bind_cache)},
+                                {"kv_write", FAST(kv_write_entry)},
+                                {"kv_read", FAST(kv_read_entry)},
+                                {"kv_plan", FAST(kv_plan_entry)},
+                                {"attend", FAST(attend_entry)},
+                                {"rotary", FAST(rotary_entry)},
                                 {"set_library_error", set_library_error, METH_O, nullptr},
                                 {nullptr, nullptr, 0, nullptr}};
 static PyModuleDef module = {PyModuleDef_HEAD_INIT, "_b200lut_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
@@ -414,5 +435,6 @@ static PyModuleDef module = {PyModuleDef_HEAD_INIT, "_b200lut_host", nullptr, -1
 
 PyMODINIT_FUNC PyInit__b200lut_host(void) {
   if (ready_type(&LayerType, "_b200lut_host.Layer", sizeof(Layer), layer_dealloc) < 0) return nullptr;
+  if (ready_type(&CacheType, "_b200lut_host.Cache", sizeof(Cache), cache_dealloc) < 0) return nullptr;
   return PyModule_Create(&module);
 }

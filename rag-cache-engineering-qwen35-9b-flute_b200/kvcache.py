@@ -58,6 +58,11 @@ def plan_step(cached: torch.Tensor, fresh: torch.Tensor, block_table: torch.Tens
     of the free list, or whose rows would end behind max_tokens, is not served: it takes no page and its slots are
     -1. The caller goes on with the returned kv_len and taken; the same call again gives the same result."""
     _lib._need_cuda(cached, "cached")
+    done = _lib.host.kv_plan(cached, fresh, block_table, free_pages, taken, page_size, max_tokens) \
+        if page_size in PAGE_SIZES else None
+    if done is not None:
+        row_start, kv_len, positions, slots, taken, served = done
+        return StepPlan(row_start, kv_len, positions, slots, taken, served)
     dev = cached.device
     _ints("cached", cached, (None,), dev)
     B = cached.shape[0]
@@ -72,6 +77,11 @@ def plan_step(cached: torch.Tensor, fresh: torch.Tensor, block_table: torch.Tens
     if B < 1 or B > 8192 or block_table.shape[1] < 1 or max_tokens < 1:
         raise ValueError(f"plan_step: 1 to 8192 requests, a block_table of some width and max_tokens >= 1 wanted, "
                          f"got {B}, {block_table.shape[1]}, {max_tokens}")
+    return _plan_route(cached, fresh, block_table, free_pages, taken, page_size, max_tokens)
+
+
+def _plan_route(cached, fresh, block_table, free_pages, taken, page_size, max_tokens):
+    B, dev = cached.shape[0], cached.device
     cached, fresh, free_pages = cached.contiguous(), fresh.contiguous(), free_pages.contiguous()
     ints = torch.empty(2 * B + 2 + 2 * max_tokens, dtype=torch.int32, device=dev)
     row_start, kv_len, taken_out, positions, slots = ints.split((B + 1, B, 1, max_tokens, max_tokens))
@@ -106,12 +116,19 @@ class KVCache4:
         self.n_pages, self.n_kv_heads, self.head_dim = int(n_pages), int(n_kv_heads), int(head_dim)
         self.page_size, self.dtype = int(page_size), dtype
         codes = (2, n_pages, n_kv_heads, page_size * head_dim // 2)
-        self.k_codes, self.v_codes = torch.zeros(codes, dtype=torch.uint8, device=device)
-        self.k_pairs, self.v_pairs = torch.zeros((2, n_pages, n_kv_heads, page_size, 2), dtype=dtype, device=device)
+        self._buffers = (*torch.zeros(codes, dtype=torch.uint8, device=device),
+                         *torch.zeros((2, n_pages, n_kv_heads, page_size, 2), dtype=dtype, device=device))
         self.device = self.k_codes.device
         self._view = _lib.KVCacheView(self.k_codes.data_ptr(), self.v_codes.data_ptr(), self.k_pairs.data_ptr(),
                                       self.v_pairs.data_ptr(), self.n_pages, self.page_size, self.n_kv_heads,
                                       self.head_dim, _lib.dtype_id(dtype))
+        self._native = _lib.host.bind_cache(*self._buffers, self.n_pages, self.page_size, self.n_kv_heads, self.head_dim)
+
+    # codes: uint8 [n_pages, n_kv_heads, page_size * head_dim / 2]; pairs (lo, hi): [n_pages, n_kv_heads, page_size, 2]
+    k_codes = property(lambda self: self._buffers[0])
+    v_codes = property(lambda self: self._buffers[1])
+    k_pairs = property(lambda self: self._buffers[2])
+    v_pairs = property(lambda self: self._buffers[3])
 
     def __reduce__(self):
         raise TypeError("a KVCache4 is bound to its device buffers: it is neither copied nor pickled")
@@ -130,6 +147,8 @@ class KVCache4:
     def write(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
         """Rows k, v [tokens, n_kv_heads, head_dim] into `slots` (int32 [tokens], all different; negative: not
         written). A slot outside the cache is skipped and raises the device status (0x6100)."""
+        if _lib.host.kv_write(self._native, k, v, slots):
+            return
         k, v = self._rows("k", k, self.n_kv_heads), self._rows("v", v, self.n_kv_heads)
         T = k.shape[0]
         if v.shape[0] != T:
@@ -144,6 +163,9 @@ class KVCache4:
     def read(self, slots: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
         """Keys and values [tokens, n_kv_heads, head_dim] that `slots` (int32 [tokens]) stand for, rounded to the
         cache's dtype; zeros for negative slots and for those outside the cache (device status 0x6100)."""
+        done = _lib.host.kv_read(self._native, slots)
+        if done is not None:
+            return done
         if slots.dim() != 1:
             raise ValueError(f"slots must be an int32 tensor [*] on {self.device}, got {tuple(slots.shape)}")
         slots = _ints("slots", slots, (None,), self.device).contiguous()
@@ -167,6 +189,10 @@ class KVCache4:
         h // (n_heads / n_kv_heads). scale: head_dim ** -0.5 unless given. gate: the result is multiplied by
         sigmoid(gate). Where nothing is visible the result is zero; rows that belong to no request are not written.
         A token on a page outside the cache counts as hidden and raises the device status (0x6200)."""
+        done = _lib.host.attend(self._native, q, block_table, kv_len, row_start,
+                                self.head_dim ** -0.5 if scale is None else scale, window, sinks, gate, out)
+        if done is not None:
+            return done
         if q.dim() != 3 or q.shape[1] < 1 or q.shape[1] % self.n_kv_heads:
             raise ValueError(f"q must be [tokens, a multiple of {self.n_kv_heads} heads, {self.head_dim}], got {tuple(q.shape)}")
         q = self._rows("q", q, q.shape[1])

@@ -99,6 +99,11 @@ class AxisRotary:
         """q [tokens, heads, D] and k [tokens, kv_heads, D], D in {64, 128, 256}, rotated into new
         contiguous tensors. positions: int32 or int64, [axes, tokens] or [tokens]. q_gain, k_gain: [D] in
         q's dtype, both or neither."""
+        tables = self._tables.get(q.device)
+        if tables is not None:
+            done = _lib.host.rotary(q, k, positions, q_gain, k_gain, eps, *tables, self.axes)
+            if done is not None:
+                return done
         check_heads("q", q, None, None)
         check_heads("k", k, None, q.shape[2])
         T, Hq, D = q.shape
