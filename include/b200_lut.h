@@ -77,7 +77,7 @@ const char* b200lut_last_error(void);
  * with its tensor memory freed and its output undefined). Synchronises the device
  * read; clears the word. No counterpart in the reference (its kernels never wait).
  * 0x6000: an embedding gather met an id outside its table (that row was written as zeros);
- * 0x6100: a slot, 0x6200: a page outside a key/value cache. */
+ * 0x6100: a slot, 0x6200: a page outside a key/value cache; 0x63xx: a wait of the attention over it. */
 int b200lut_device_status(void);
 
 /* Number of SMs of the current device (used by the split policy). */
@@ -639,7 +639,8 @@ typedef struct b200lut_attend_args {
   int window, sinks;
   float scale;
 } b200lut_attend_args;
-size_t b200lut_attend_workspace_bytes(int n_heads, int n_kv_heads, int head_dim);
+/* one_row_each: the call comes without row_start. 0 on invalid sizes. */
+size_t b200lut_attend_workspace_bytes(int n_heads, int n_kv_heads, int head_dim, int one_row_each);
 int b200lut_attend(const b200lut_attend_args* args, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus

@@ -237,7 +237,7 @@ def lib() -> ctypes.CDLL:
     L.b200lut_kv_read.restype = i32
     L.b200lut_kv_read.argtypes = [ctypes.POINTER(KVCacheView), vp, vp, vp, i32, vp]
     L.b200lut_attend_workspace_bytes.restype = sz
-    L.b200lut_attend_workspace_bytes.argtypes = [i32, i32, i32]
+    L.b200lut_attend_workspace_bytes.argtypes = [i32, i32, i32, i32]
     L.b200lut_attend.restype = i32
     L.b200lut_attend.argtypes = [ctypes.POINTER(AttendArgs), vp, sz, vp]
     _lib = L

@@ -14,6 +14,8 @@
 // value lane are adjacent in memory; P^T comes out of S^T by two 8 x 8 transposes of half pairs.
 // Every lane copies exactly the 16-byte pieces it will read (cp.async into a ring of its own): no barrier in
 // the loop.
+#include <climits>
+
 #include "attend.cuh"
 
 namespace b200lut {
@@ -84,9 +86,14 @@ __device__ __forceinline__ float pow2_above(float x) {
 }
 
 // Tiles of all items of request b (its row tiles are equal but for what they see).
+__device__ __forceinline__ Request rows_request(const AttendParams& p, int b) {
+  Request r = request_of(p, b);
+  if ((long long)r.rows * p.G > p.rows_limit) r.rows = 0;        // the tile kernel's
+  return r;
+}
 template <int kRows>
 __device__ __forceinline__ long long request_tiles(const AttendParams& p, int b) {
-  const Request r = request_of(p, b);
+  const Request r = rows_request(p, b);
   long long sum = 0;
   const long long rows = (long long)r.rows * p.G;
   for (long long r0 = 0; r0 < rows; r0 += kRows) {
@@ -157,7 +164,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) attend_rows_kern
   const int tok0 = 4 * (g >> 1) + (g & 1);       // tokens of this lane's rows g and g + 8: tok0, tok0 + 2
   long long cur = begin, req_at = first_tile;
   for (int b = first_b; cur < stop && b < p.B; ++b) {
-    const Request rq = request_of(p, b);
+    const Request rq = rows_request(p, b);
     const long long rows = (long long)rq.rows * p.G;
     const int base = rq.len - rq.rows;
     for (int h = 0; h < p.c.heads && cur < stop; ++h) {
@@ -488,35 +495,80 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) attend_rows_kern
   }
 }
 
-// Joins the parts of the item that block blockIdx.x began and others went on with; one row per block of threads.
-template <typename T, int D, int NT>
-__global__ void __launch_bounds__(D / 2) attend_join_kernel(const __grid_constant__ AttendParams p) {
-  constexpr int kRows = 8 * NT;
+// Joins the parts of the item that block blockIdx.x began and others went on with. `Ways` warps share a row: each
+// adds every Ways-th part, then the first adds the warps' sums in their order.
+constexpr int kJoinWarps = 8;
+template <typename T, int D, int kRows, int Ways>
+__global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const __grid_constant__ AttendParams p) {
+  constexpr int kPer = D / 32;
+  __shared__ float part[kJoinWarps][D + 2];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int4 meta = p.meta[blockIdx.x];
   if (meta.x == 0) return;
-  const int c0 = blockIdx.x, c1 = meta.x, b = meta.y, h = meta.z, r = blockIdx.y, d = 2 * threadIdx.x;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, way = warp % Ways;
+  const int c0 = blockIdx.x, c1 = meta.x, b = meta.y, h = meta.z, r = blockIdx.y * (kJoinWarps / Ways) + warp / Ways;
   const Request rq = request_of(p, b);
   const long long row = (long long)meta.w * kRows + r;
-  if (row >= (long long)rq.rows * p.G) return;
+  if (row - r + blockIdx.y * (kJoinWarps / Ways) >= (long long)rq.rows * p.G) return;      // none of the block's rows
+  const bool live = row < (long long)rq.rows * p.G;
   auto slot = [&](int c) { return (c == c0 ? 2LL * c + 1 : 2LL * c) * kRows + r; };
-  float top = -INFINITY;
-  for (int c = c0; c <= c1; ++c) top = fmaxf(top, p.part_ml[slot(c)].x);
-  float sum = 0.f, x = 0.f, y = 0.f;
-  for (int c = c0; c <= c1; ++c) {
-    const float2 ml = p.part_ml[slot(c)];
-    const float2 o = *reinterpret_cast<const float2*>(p.part_o + slot(c) * D + d);
-    const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : ex2(ml.x - top);
-    sum = fmaf(ml.y, f, sum);
-    x = fmaf(o.x, f, x);
-    y = fmaf(o.y, f, y);
+  float top = -INFINITY, sum = 0.f, x[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) x[i] = 0.f;
+  if (live) {
+    for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, p.part_ml[slot(c)].x);
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+#pragma unroll 4
+    for (int c = c0 + way; c <= c1; c += Ways) {
+      const float2 ml = p.part_ml[slot(c)];
+      const float* o = p.part_o + slot(c) * D + lane * kPer;
+      float v[kPer];
+#pragma unroll
+      for (int i = 0; i < kPer; i += 2) {
+        const float2 y = *reinterpret_cast<const float2*>(o + i);
+        v[i] = y.x, v[i + 1] = y.y;
+      }
+      const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : ex2(ml.x - top);
+      sum = fmaf(ml.y, f, sum);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) x[i] = fmaf(v[i], f, x[i]);
+    }
   }
+  if constexpr (Ways > 1) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) part[warp][lane * kPer + i] = x[i];
+    if (lane == 0) part[warp][D] = sum;
+    __syncthreads();
+    if (way != 0) return;
+    for (int w = 1; w < Ways; ++w) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) x[i] += part[warp + w][lane * kPer + i];
+      sum += part[warp + w][D];
+    }
+  }
+  if (!live) return;
   const long long tok = rq.row0 + row / p.G;
-  const int head = h * p.G + int(row % p.G);
+  const int head = h * p.G + int(row % p.G), d = lane * kPer;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  const uint32_t lo = DType<T>::from_float(gated<T>(x * inv, p, tok, head, d));
-  const uint32_t hi = DType<T>::from_float(gated<T>(y * inv, p, tok, head, d + 1));
-  *reinterpret_cast<uint32_t*>(p.out + tok * p.out_token + (long long)head * p.out_head + d) = lo | (hi << 16);
+  uint32_t* to = reinterpret_cast<uint32_t*>(p.out + tok * p.out_token + (long long)head * p.out_head + d);
+#pragma unroll
+  for (int i = 0; i < kPer; i += 2)
+    to[i / 2] = uint32_t(DType<T>::from_float(gated<T>(x[i] * inv, p, tok, head, d + i))) |
+                (uint32_t(DType<T>::from_float(gated<T>(x[i + 1] * inv, p, tok, head, d + i + 1))) << 16);
+}
+
+template <typename T, int D, int kRows, int Ways>
+int join(const AttendParams& p, int blocks, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(blocks), kRows * Ways / kJoinWarps);
+  cfg.blockDim = dim3(kJoinWarps * 32);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr, cfg.numAttrs = 1;
+  B200LUT_CUDA_OK(cudaLaunchKernelEx(&cfg, attend_join_kernel<T, D, kRows, Ways>, p));
+  return B200LUT_OK;
 }
 
 template <typename T, int D, int NT>
@@ -531,30 +583,46 @@ int launch(AttendParams p, int blocks, cudaStream_t st) {
   }
   attend_rows_kernel<T, D, NT><<<unsigned(blocks), kWarps * 32, S::kSmem, st>>>(p);
   B200LUT_CUDA_OK(cudaGetLastError());
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(blocks), S::kRows);
-  cfg.blockDim = dim3(D / 2);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr, cfg.numAttrs = 1;
-  B200LUT_CUDA_OK(cudaLaunchKernelEx(&cfg, attend_join_kernel<T, D, NT>, p));
-  return B200LUT_OK;
+  return join<T, D, S::kRows, 8>(p, blocks, st);
+}
+
+// Blocks: two per SM with eight rows (fewer rows than that leave SMs without enough loads in flight), one with 16.
+int row_blocks(int sms, int G) { return G <= 8 ? 2 * sms : sms; }
+int rows_of(int G) { return G <= 8 ? 8 : 16; }
+
+// Workspace of a launch over `blocks` blocks of `rows` rows: what attend_*_kernel leave to the join.
+size_t workspace_of(int blocks, int rows, int D) { return size_t(blocks) * (16 + 2 * size_t(rows) * (8 + size_t(D) * 4)); }
+void lay_out(AttendParams* p, void* ws, int blocks, int rows) {
+  p->meta = static_cast<int4*>(ws);
+  p->part_ml = reinterpret_cast<float2*>(p->meta + blocks);
+  p->part_o = reinterpret_cast<float*>(p->part_ml + 2LL * blocks * rows);
 }
 
 template <typename T, int D>
-int pick_rows(const AttendParams& p, int blocks, cudaStream_t st) {
-  return p.G <= 8 && !p.row_start ? launch<T, D, 1>(p, blocks, st) : launch<T, D, 2>(p, blocks, st);
+int run(AttendParams p, int sms, void* ws, cudaStream_t st) {
+  const int blocks = row_blocks(sms, p.G), rows = rows_of(p.G);
+  p.rows_limit = INT_MAX;
+  if (p.row_start) {
+    // requests of many rows first, on the tensor cores; the others' launch follows
+    p.rows_limit = rows;
+    AttendParams t = p;
+    lay_out(&t, static_cast<char*>(ws) + workspace_of(blocks, rows, D), sms, 128);
+    int rc = attend_tiles(t, DType<T>::id, sms, st);
+    if (rc == B200LUT_OK) rc = join<T, D, 128, 1>(t, sms, st);
+    if (rc != B200LUT_OK) return rc;
+  }
+  lay_out(&p, ws, blocks, rows);
+  return rows == 8 ? launch<T, D, 1>(p, blocks, st) : launch<T, D, 2>(p, blocks, st);
 }
 
 template <typename T>
-int pick_dim(const AttendParams& p, int blocks, cudaStream_t st) {
-  return p.c.D == 64 ? pick_rows<T, 64>(p, blocks, st) : p.c.D == 128 ? pick_rows<T, 128>(p, blocks, st)
-                                                                      : pick_rows<T, 256>(p, blocks, st);
+int pick_dim(const AttendParams& p, int sms, void* ws, cudaStream_t st) {
+  return p.c.D == 64 ? run<T, 64>(p, sms, ws, st) : p.c.D == 128 ? run<T, 128>(p, sms, ws, st) : run<T, 256>(p, sms, ws, st);
 }
 
-int blocks_of(int sms) { return 2 * sms; }
+size_t workspace_bytes_of(int G, int D, bool one_row_each, int sms) {
+  return workspace_of(row_blocks(sms, G), rows_of(G), D) + (one_row_each ? 0 : workspace_of(sms, 128, D));
+}
 
 }  // namespace
 
@@ -565,28 +633,13 @@ int attend_status_take() {
   return v;
 }
 
-size_t attend_rows_workspace(int D, int sms) {
-  const size_t n = size_t(blocks_of(sms));
-  return n * 16 + 2 * n * 16 * 8 + 2 * n * 16 * size_t(D) * 4;
-}
-
-int attend_rows(const AttendParams& q, int dtype, int sms, void* ws, void* stream) {
-  AttendParams p = q;
-  const int blocks = blocks_of(sms);
-  p.meta = static_cast<int4*>(ws);
-  p.part_ml = reinterpret_cast<float2*>(p.meta + blocks);
-  p.part_o = reinterpret_cast<float*>(p.part_ml + 2LL * blocks * 16);
-  const cudaStream_t st = cudaStream_t(stream);
-  return dtype == B200LUT_BF16 ? pick_dim<__nv_bfloat16>(p, blocks, st) : pick_dim<__half>(p, blocks, st);
-}
-
 }  // namespace b200lut
 
 using namespace b200lut;
 
-extern "C" size_t b200lut_attend_workspace_bytes(int n_heads, int n_kv_heads, int head_dim) {
+extern "C" size_t b200lut_attend_workspace_bytes(int n_heads, int n_kv_heads, int head_dim, int one_row_each) {
   if (n_heads < 1 || n_kv_heads < 1 || n_heads % n_kv_heads || (head_dim != 64 && head_dim != 128 && head_dim != 256)) return 0;
-  return attend_rows_workspace(head_dim, b200lut_sm_count());
+  return workspace_bytes_of(n_heads / n_kv_heads, head_dim, one_row_each != 0, b200lut_sm_count());
 }
 
 extern "C" int b200lut_attend(const b200lut_attend_args* a, void* workspace, size_t workspace_bytes, void* stream) {
@@ -611,7 +664,7 @@ extern "C" int b200lut_attend(const b200lut_attend_args* a, void* workspace, siz
                   B200LUT_ERR_ALIGN, "attend: rows must be 16-byte aligned (pointers and strides)");
   const int sms = b200lut_sm_count();
   B200LUT_REQUIRE(workspace && aligned16(workspace) &&
-                      workspace_bytes >= attend_rows_workspace(p.c.D, sms),
+                      workspace_bytes >= workspace_bytes_of(a->n_heads / p.c.heads, p.c.D, !a->row_start, sms),
                   B200LUT_ERR_WORKSPACE, "attend: workspace of b200lut_attend_workspace_bytes() wanted");
   p.q = static_cast<const uint16_t*>(a->q), p.gate = static_cast<const uint16_t*>(a->gate);
   p.out = static_cast<uint16_t*>(a->out);
@@ -622,5 +675,7 @@ extern "C" int b200lut_attend(const b200lut_attend_args* a, void* workspace, siz
   p.T = a->T, p.B = a->B, p.Hq = a->n_heads, p.G = a->n_heads / p.c.heads, p.width = a->width;
   p.window = a->window, p.sinks = a->sinks;
   p.scale = a->scale * 1.4426950408889634f;
-  return attend_rows(p, a->cache->dtype, sms, workspace, stream);
+  p.wait_cycles = gemm_wait_cycles();
+  const cudaStream_t st = cudaStream_t(stream);
+  return a->cache->dtype == B200LUT_BF16 ? pick_dim<__nv_bfloat16>(p, sms, workspace, st) : pick_dim<__half>(p, sms, workspace, st);
 }

@@ -30,7 +30,11 @@ struct AttendParams {
   long long table_ld;
   int T, B, Hq, G, width, window, sinks;
   float scale;                 // scale * log2(e)
-  // workspace of the split kernel
+  // a request of at most so many rows (times query heads per key/value head) is the single-row kernel's, the
+  // others are the tile kernel's; INT_MAX: no tile kernel runs
+  int rows_limit;
+  long long wait_cycles;
+  // workspace: per block, what it left to be joined
   int4* meta;
   float2* part_ml;
   float* part_o;
@@ -78,7 +82,7 @@ __device__ __forceinline__ float gated(float o, const AttendParams& p, long long
   return o / (1.f + __expf(-g));
 }
 
-int attend_rows(const AttendParams& p, int dtype, int sms, void* ws, void* stream);
-size_t attend_rows_workspace(int D, int sms);
+// The tile kernel over `blocks` blocks (its joins are launched with those of the row kernel).
+int attend_tiles(const AttendParams& p, int dtype, int blocks, cudaStream_t stream);
 
 }  // namespace b200lut

@@ -1,0 +1,780 @@
+// Attention over the 4-bit cache for many rows per request (prompts, chunks of prompts): tcgen05 on codes.
+//
+// A work item is 128 rows (query heads of one key/value head, times new tokens) of one request; its visible
+// tokens are cut into tiles of 128. All items' tiles form one line that is dealt to the blocks (one per SM) in
+// equal contiguous shares; items that span blocks are joined by a second kernel in the order of the blocks.
+// Per tile, in the roles of one block:
+//   warp 14     parameters: pages, and what the tokens' pairs say (one tile ahead of everybody else).
+//   warps 12-13 keys: codes from global memory (fetched one tile ahead) into fp16 operands in shared memory, 128-byte
+//               swizzle, [token, dim] rows.
+//   warps 8-11  values: transposed, [dim, token] rows. A 16-byte piece holds four tokens' words side by side, two byte
+//               permutes make pairs of tokens. The words are rotated by the lane's group first, so that the
+//               eight rows a store hits differ in their swizzle.
+//   warp 15     one thread issues S = Q K^T (128 x 128, fp32 in tensor memory, two buffers) and O += P V (128 x D).
+//   warps 0-7   softmax, two threads a row (64 tokens each): scores from tensor memory, the token's two parameters
+//               applied as packed pairs, P back into the place of S as fp16 (the A operand of the second product).
+//               The running maximum may lag by 2^8 before O is rescaled, which then waits for the products in flight.
+// Tensor memory: O in columns 0 .. D - 1, S in 256 .. 383 and 384 .. 511.
+#include "attend.cuh"
+#include "tc05.cuh"
+
+namespace b200lut {
+namespace {
+
+__device__ int g_tiles_status = 0;
+constexpr int kRows = 128, kTile = 128;
+constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kValueWarp = 8, kKeyWarp = 12, kParamWarp = 14, kProductWarp = 15;
+constexpr int kParamStages = 4;
+constexpr float kLazy = 8.f;
+constexpr float kMinStep = 7.888609e-31f;   // 2^-100
+constexpr int kBadPage = 0x6200;
+
+template <int D>
+struct Shape {
+  static constexpr int kStages = D == 256 ? 1 : 2;
+  static constexpr int kOperand = 256 * D;                       // bytes of 128 x D halves
+  static constexpr int kQ = 0, kK = kOperand, kV = kK + kStages * kOperand;
+  static constexpr int kParam = kV + kStages * kOperand;         // [stage][64 token pairs] of a, a, lo, lo and s, s, mid, mid
+  static constexpr int kParamBytes = 2 * 64 * 16;
+  static constexpr int kEnd = kParam + kParamStages * kParamBytes;
+  static constexpr int kSmem = kEnd + 1024;                      // the base is rounded up to 1024
+};
+
+struct TileInfo {
+  float sig;                   // power of two >= the largest step so far
+  int whole;                   // every row sees every token
+  uint32_t valid[4];           // tokens that some row may see
+  int page[8];                 // of each 16 tokens; -1: none
+};
+
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float pow2_above(float x) {
+  return __uint_as_float((__float_as_uint(x) + 0x007FFFFFu) & 0x7F800000u);
+}
+__device__ __forceinline__ uint32_t half2_of(float2 a) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(a.y), "f"(a.x));
+  return r;
+}
+__device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+__device__ __forceinline__ uint32_t hadd2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+__device__ __forceinline__ void sts64(uint32_t a, uint32_t x, uint32_t y) {
+  asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(a), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t t, float* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+        "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]),
+        "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
+        "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+      : "r"(t)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t t, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(t),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+// D[d] (+)= A[desc a] B[desc b], one K = 16 step; one thread issues.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
+      "r"(accumulate), "r"(0u)
+      : "memory");
+}
+
+__device__ __forceinline__ float4 lds128f(uint32_t a) {
+  float4 r;
+  asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(r.x), "=f"(r.y), "=f"(r.z), "=f"(r.w) : "r"(a) : "memory");
+  return r;
+}
+__device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
+
+// ---- the line of tiles ---------------------------------------------------------------------------------------
+__device__ __forceinline__ Request tiles_request(const AttendParams& p, int b) {
+  Request r = request_of(p, b);
+  if ((long long)r.rows * p.G <= p.rows_limit) r.rows = 0;       // the other kernel's
+  return r;
+}
+__device__ __forceinline__ Span<kTile> span_of(const AttendParams& p, const Request& r, long long r0) {
+  const long long rows = (long long)r.rows * p.G;
+  const int base = r.len - r.rows;
+  const long long last = min(r0 + kRows, rows) - 1;
+  return Span<kTile>(base + int(r0 / p.G), base + int(last / p.G), r.len, p.window, p.sinks);
+}
+// Tiles of one head of request b, summed over its row tiles by a whole warp (all lanes get the sum).
+__device__ __forceinline__ long long head_tiles(const AttendParams& p, const Request& r, int lane) {
+  const long long n = ((long long)r.rows * p.G + kRows - 1) / kRows;
+  long long sum = 0;
+  for (long long i = lane; i < n; i += 32) sum += span_of(p, r, i * kRows).tiles;
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  return sum;
+}
+
+// A part of an item: tiles [i0, i1) of row tile rt of head h of request b.
+struct Work {
+  int b, h;
+  long long rt;
+  int i0, i1, tiles;
+  Request rq;
+  long long item_at;           // tiles of the line before the item
+};
+
+// What the roles need of it.
+struct Item {
+  Span<kTile> span;
+  long long r0;
+  int n_rows, base, first_pos, last_pos;
+  uint32_t n0;                 // tiles of this block before the item's
+  int count;
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_constant__ AttendParams p) {
+  using S = Shape<D>;
+  extern __shared__ uint8_t raw_sm[];
+  __shared__ __align__(8) uint64_t bars[24];
+  __shared__ uint32_t tmem_base;
+  __shared__ int abort_word;
+  __shared__ float2 row_k[kRows];              // factor of the scores, sum of the scaled row
+  __shared__ TileInfo info[kParamStages];
+  __shared__ float half_top[2][2][kRows];      // [tile & 1][half][row]
+  __shared__ float2 half_sum[kRows];
+  __shared__ long long scan[kWarps];
+  __shared__ long long first_at;
+  __shared__ int first_b;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t sm = (tc::smem_addr(raw_sm) + 1023u) & ~1023u;
+  volatile int* abort_flag = &abort_word;
+  const uint32_t bar0 = tc::smem_addr(bars);
+  auto bar = [&](int i) { return bar0 + 8u * uint32_t(i); };
+  constexpr int kKFull = 0, kKEmpty = 2, kVFull = 4, kVEmpty = 6, kSFull = 8, kPFull = 10, kPvDone = 12, kPrmFull = 14,
+                kPrmEmpty = 18;
+
+  // ---- this block's share
+  if (tid == 0) {
+    p.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
+    abort_word = 0;
+    first_b = p.B;
+  }
+  const int per = (p.B + kWarps - 1) / (kWarps);
+  long long mine = 0;
+  for (int i = 0; i < per; ++i) {
+    const int b = warp * per + i;
+    if (b < p.B) mine += head_tiles(p, tiles_request(p, b), lane) * p.c.heads;
+  }
+  if (lane == 0) scan[warp] = mine;
+  __syncthreads();
+  long long total = 0, before = 0;
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += scan[w];
+    total += scan[w];
+  }
+  const long long share = max(1LL, (total + gridDim.x - 1) / gridDim.x);
+  const long long begin = share * blockIdx.x, stop = min(total, begin + share);
+  if (begin >= stop) return;
+  if (begin >= before && begin < before + mine) {
+    long long at = before;
+    for (int i = 0; i < per; ++i) {
+      const int b = warp * per + i;
+      if (b >= p.B) break;
+      const long long n = head_tiles(p, tiles_request(p, b), lane) * p.c.heads;
+      if (begin < at + n) {
+        if (lane == 0) first_b = b, first_at = at;
+        break;
+      }
+      at += n;
+    }
+  }
+  if (warp == kProductWarp) tc::tmem_alloc(tc::smem_addr(&tmem_base), 512);
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(bar(kKFull + i), 2), tc::mbar_init(bar(kKEmpty + i), 1);
+      tc::mbar_init(bar(kVFull + i), 4), tc::mbar_init(bar(kVEmpty + i), 1);
+      tc::mbar_init(bar(kSFull + i), 1), tc::mbar_init(bar(kPFull + i), 8), tc::mbar_init(bar(kPvDone + i), 1);
+    }
+    for (int i = 0; i < kParamStages; ++i) tc::mbar_init(bar(kPrmFull + i), 1), tc::mbar_init(bar(kPrmEmpty + i), 14);
+    tc::mbar_init_fence();
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = tmem_base;
+  auto wait = [&](int i, uint32_t parity, int why) {
+    tc::mbar_wait(bar(i), parity, abort_flag, &g_tiles_status, why, p.wait_cycles);
+  };
+
+  // A wait names a phase by its parity alone: whoever waits must know that the phase before is complete and that
+  // the one after cannot be yet. Product P V of tile m reports to barrier m & 1: tile m - 2 is through when S of m is
+  // there, tile m + 2 waits for P of m.
+  auto wait_pv = [&](uint32_t m) { wait(kPvDone + int(m & 1), (m >> 1) & 1u, tc::kStatusWaitDone); };
+
+  // the first item (every warp finds it by itself)
+  Work w;
+  w.b = first_b;
+  {
+    w.rq = tiles_request(p, w.b);
+    const long long per_head = head_tiles(p, w.rq, lane);
+    long long off = begin - first_at;
+    w.h = int(off / per_head);
+    off -= w.h * per_head;
+    const long long n = ((long long)w.rq.rows * p.G + kRows - 1) / kRows;
+    w.rt = 0;
+    for (long long c0 = 0; c0 < n; c0 += 32) {
+      const long long tiles = c0 + lane < n ? span_of(p, w.rq, (c0 + lane) * kRows).tiles : 0;
+      long long inc = tiles;
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += v;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, off < inc);
+      if (hit) {
+        const int l = __ffs(int(hit)) - 1;
+        w.rt = c0 + l;
+        off -= __shfl_sync(0xffffffffu, inc - tiles, l);
+        break;
+      }
+      off -= __shfl_sync(0xffffffffu, inc, 31);
+    }
+    w.item_at = begin - off;
+  }
+
+  uint32_t n = 0;                              // tiles of this block so far
+  // Every role walks the block's items: the rows' operand is made by all warps, then `body` does the role's
+  // part of the item's tiles.
+  auto items = [&](auto&& body) {
+    long long cur = begin;
+    while (cur < stop) {
+      const Span<kTile> span = span_of(p, w.rq, w.rt * kRows);
+      w.tiles = span.tiles;
+      w.i0 = int(cur - w.item_at), w.i1 = int(min((long long)w.tiles, stop - w.item_at));
+      const long long r0 = w.rt * kRows, rows = (long long)w.rq.rows * p.G;
+      const int n_rows = int(min((long long)kRows, rows - r0)), base = w.rq.len - w.rq.rows;
+      const int first_pos = base + int(r0 / p.G), last_pos = base + int((r0 + n_rows - 1) / p.G);
+
+      // ---- the item's rows: fp16, scaled, in the order of the codes' pairs
+      for (int r = warp; r < kRows; r += kWarps) {
+        constexpr int kChunks = D / 8;           // 16-byte chunks of eight elements
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (r < n_rows && lane < kChunks) {
+          const long long tok = w.rq.row0 + (r0 + r) / p.G;
+          x = __ldg(reinterpret_cast<const uint4*>(p.q + tok * p.q_token +
+                                                   (long long)(w.h * p.G + int((r0 + r) % p.G)) * p.q_head) + lane);
+        }
+        const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+        float v[8], top = 0.f, sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          v[e] = DType<T>::to_float(uint16_t(u[e >> 1] >> (16 * (e & 1))));
+          top = fmaxf(top, fabsf(v[e])), sum += v[e];
+        }
+        for (int o = 16; o; o >>= 1) {
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        }
+        const int ex = int(__float_as_uint(top) >> 23);
+        const int fe = ex == 255 || top == 0.f ? 127 : max(24, min(254, 127 + 13 + 127 - ex));   // 2^24 / f stays finite
+        const float f = __uint_as_float(uint32_t(fe) << 23), fs = p.scale < 0.f ? -f : f;
+        if (lane < kChunks) {
+          uint32_t o[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float g = e & 1 ? fs * 0.0625f : fs;
+            o[e] = half2_of(make_float2(v[e] * g, v[e + 4] * g));
+          }
+          sts128(sm + S::kQ + (lane >> 3) * (kRows * 128) + r * 128 + (((lane & 7) ^ (r & 7)) << 4), o[0], o[1], o[2], o[3]);
+        }
+        if (lane == 0) row_k[r] = make_float2(fmaxf(fabsf(p.scale) * (16777216.f / f), 1.17549435e-38f), sum * fs * 5.9604645e-8f);
+      }
+      tc::fence_proxy_async();
+      __syncthreads();
+
+      const Item item{span, r0, n_rows, base, first_pos, last_pos, n, w.i1 - w.i0};
+      body(item);
+      n += uint32_t(item.count);
+      cur = w.item_at + w.i1;
+      // ---- on to the next item: the rows' operand and O are free once every role is through
+      if (cur < stop) {
+        w.item_at += w.tiles;
+        if ((w.rt + 1) * kRows < rows) {
+          ++w.rt;
+        } else {
+          w.rt = 0;
+          if (++w.h == p.c.heads) {
+            w.h = 0;
+            do w.rq = tiles_request(p, ++w.b);
+            while (w.rq.rows == 0);
+          }
+        }
+      }
+      __syncthreads();
+      tc::fence_after_sync();
+    }
+  };
+
+  if (warp < kValueWarp) {
+    // ================================================================ softmax: two threads a row
+    const int r = tid & 127, half = warp >> 2;
+    const uint32_t lane_base = tmem + (uint32_t((warp & 3) * 32) << 16);
+    items([&](const Item& it) {
+      const float2 rk = row_k[r];
+      const float2 qf = make_float2(rk.x, rk.x), qs = make_float2(rk.y, rk.y);
+      const int pos = r < it.n_rows ? it.base + int((it.r0 + r) / p.G) : -1;
+      float m_run = -INFINITY, sig_run = 0.f;
+      float2 l2 = make_float2(0.f, 0.f), pm2 = make_float2(0.f, 0.f);
+      for (int t = 0; t < it.count; ++t) {
+        const uint32_t m = it.n0 + uint32_t(t);
+        const int ps = int(m % kParamStages), first = it.span.id(w.i0 + t) * kTile + 64 * half;
+        wait(kPrmFull + ps, (m / kParamStages) & 1u, tc::kStatusWaitFull);
+        wait(kSFull + int(m & 1), (m >> 1) & 1u, tc::kStatusWaitDone);
+        tc::fence_after_sync();
+        const uint32_t s_at = lane_base + 256 + 128 * (m & 1);
+        float s[64];
+        tmem_ld32(s_at + 64 * half, s);
+        tmem_ld32(s_at + 64 * half + 32, s + 32);
+        tc::wait_ld();
+        const uint32_t prm = sm + S::kParam + ps * S::kParamBytes + half * 512;
+        float2 top2[2] = {make_float2(-INFINITY, -INFINITY), make_float2(-INFINITY, -INFINITY)};
+        uint32_t mask[2] = {0xffffffffu, 0xffffffffu};
+        const bool whole = info[ps].whole != 0;
+        if (!whole) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            auto below = [](int k) { return k <= 0 ? 0u : k >= 32 ? 0xffffffffu : (1u << k) - 1u; };
+            const int f = first + 32 * c;
+            mask[c] = below(pos + 1 - f) & info[ps].valid[2 * half + c];
+            if (p.window) mask[c] &= ~below(pos - p.window + 1 - f) | below(p.sinks - f);
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          const float4 k = lds128f(prm + 16 * c);
+          const float2 y = fma2(make_float2(k.x, k.y), make_float2(s[2 * c], s[2 * c + 1]), mul2(make_float2(k.z, k.w), qs));
+          s[2 * c] = y.x, s[2 * c + 1] = y.y;
+        }
+        if (!whole) {
+#pragma unroll
+          for (int c = 0; c < 64; ++c)
+            if (!((mask[c >> 5] >> (c & 31)) & 1u)) s[c] = -INFINITY;
+        }
+#pragma unroll
+        for (int c = 0; c < 64; c += 4) {
+          top2[0].x = fmaxf(top2[0].x, s[c]), top2[0].y = fmaxf(top2[0].y, s[c + 1]);
+          top2[1].x = fmaxf(top2[1].x, s[c + 2]), top2[1].y = fmaxf(top2[1].y, s[c + 3]);
+        }
+        float top = fmaxf(fmaxf(top2[0].x, top2[0].y), fmaxf(top2[1].x, top2[1].y));
+        half_top[m & 1][half][r] = top;
+        pair_sync(1 + (warp & 3));
+        top = fmaxf(top, half_top[m & 1][half ^ 1][r]) * qf.x;
+        const float sig_new = info[ps].sig;
+        if (__any_sync(0xffffffffu, top > m_run + kLazy || sig_new != sig_run)) {
+          const float m_new = fmaxf(m_run, top);
+          const float alpha = m_new == -INFINITY ? 1.f : ex2(m_run - m_new);
+          const float ab = alpha * (sig_run / sig_new);
+          m_run = m_new, sig_run = sig_new;
+          l2 = mul2(l2, make_float2(alpha, alpha));
+          pm2 = mul2(pm2, make_float2(alpha, alpha));
+          if (t > 0) {         // each of the two threads rescales half of the row
+            wait_pv(m - 1);
+            tc::fence_after_sync();
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t o[16];
+              const uint32_t at = lane_base + half * (D / 2) + 16 * c;
+              tc::tmem_ld_32x32b_x16(at, o);
+              tc::wait_ld();
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * ab);
+              tmem_st16(at, o);
+            }
+            tc::wait_st();
+          }
+        }
+        const float off = m_run == -INFINITY ? 0.f : -m_run;
+        const float2 off2 = make_float2(off, off);
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            const int c = part * 16 + k;
+            float4 v = lds128f(prm + 1024 + 16 * c);
+            if (!whole) {        // a hidden token may be poisoned: 0 times NaN
+              if (!((mask[part] >> (2 * k)) & 1u)) v.x = v.z = 0.f;
+              if (!((mask[part] >> (2 * k + 1)) & 1u)) v.y = v.w = 0.f;
+            }
+            const float2 x = fma2(make_float2(s[2 * c], s[2 * c + 1]), qf, off2);
+            const float2 e = make_float2(ex2(x.x), ex2(x.y));
+            l2 = add2(l2, e);
+            pm2 = fma2(e, make_float2(v.z, v.w), pm2);
+            pk[k] = half2_of(mul2(e, make_float2(v.x, v.y)));
+          }
+          tmem_st16(s_at + 32 * half + 16 * part, pk);
+        }
+        tc::wait_st();
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) {
+          tc::mbar_arrive(bar(kPFull + int(m & 1)));
+          tc::mbar_arrive(bar(kPrmEmpty + ps));
+        }
+      }
+      // ---- the item's result; each of the two threads writes half of the row
+      const uint32_t last = it.n0 + uint32_t(it.count) - 1;
+      wait_pv(last);
+      tc::fence_after_sync();
+      float l = l2.x + l2.y, pm = pm2.x + pm2.y;
+      if (half) half_sum[r] = make_float2(l, pm);
+      pair_sync(1 + (warp & 3));
+      if (!half) {
+        l += half_sum[r].x, pm += half_sum[r].y;
+        half_sum[r] = make_float2(l, pm);
+      }
+      pair_sync(1 + (warp & 3));
+      l = half_sum[r].x, pm = half_sum[r].y;
+      const float back = 16777216.f * sig_run, inv = l == 0.f ? 0.f : 1.f / l;
+      const bool starts = w.i0 == 0, ends = w.i1 == w.tiles;
+      const long long slot = 2LL * blockIdx.x + (starts ? 1 : 0);
+      const long long tok = w.rq.row0 + (it.r0 + r) / p.G;
+      const int head = w.h * p.G + int((it.r0 + r) % p.G);
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[16];
+        const int d = half * (D / 2) + 16 * c;
+        tc::tmem_ld_32x32b_x16(lane_base + d, o);
+        tc::wait_ld();
+        if (r < it.n_rows) {
+          float x[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) x[e] = fmaf(__uint_as_float(o[e]), back, pm);
+          if (starts && ends) {
+            uint4* to = reinterpret_cast<uint4*>(p.out + tok * p.out_token + (long long)head * p.out_head + d);
+            const uint4* gt = reinterpret_cast<const uint4*>(p.gate + tok * p.gate_token + (long long)head * p.gate_head + d);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const uint4 gv = p.gate ? __ldg(gt + e) : make_uint4(0, 0, 0, 0);
+              const uint32_t gw[4] = {gv.x, gv.y, gv.z, gv.w};
+              uint32_t out[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                float a = x[8 * e + 2 * k] * inv, b = x[8 * e + 2 * k + 1] * inv;
+                if (p.gate) {
+                  a /= 1.f + __expf(-DType<T>::to_float(uint16_t(gw[k] & 0xFFFFu)));
+                  b /= 1.f + __expf(-DType<T>::to_float(uint16_t(gw[k] >> 16)));
+                }
+                out[k] = uint32_t(DType<T>::from_float(a)) | (uint32_t(DType<T>::from_float(b)) << 16);
+              }
+              to[e] = make_uint4(out[0], out[1], out[2], out[3]);
+            }
+          } else {
+            float4* to = reinterpret_cast<float4*>(p.part_o + (slot * kRows + r) * D + d);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) to[e] = make_float4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
+          }
+        }
+      }
+      if (!(starts && ends) && !half) p.part_ml[slot * kRows + r] = make_float2(m_run, l);
+      if (starts && !ends && tid == 0)
+        p.meta[blockIdx.x] = make_int4(int((w.item_at + w.tiles - 1) / share), w.b, w.h, int(w.rt));
+      tc::fence_before_sync();
+    });
+  } else if (warp < kKeyWarp) {
+    // ================================================================ values: 32 tokens a warp
+    const int q = warp - kValueWarp, tg = lane >> 3, g = lane & 7;
+    constexpr int kLoads = D / 32;               // 16-byte loads per lane and tile
+    const int page_mask = (1 << p.c.page_log2) - 1;
+    items([&](const Item& it) {
+      uint4 vc[kLoads];
+      auto load = [&](int t) {
+        const uint32_t m = it.n0 + uint32_t(t);
+        const int ps = int(m % kParamStages), first = it.span.id(w.i0 + t) * kTile + 32 * q;
+        wait(kPrmFull + ps, (m / kParamStages) & 1u, tc::kStatusWaitFull);
+#pragma unroll
+        for (int blk = 0; blk < 2; ++blk) {
+          const int page = info[ps].page[2 * q + blk];
+          const bool ok = unsigned(page) < unsigned(p.c.n_pages);      // after a wait that gave up it may be anything
+          const uint4* at = reinterpret_cast<const uint4*>(p.c.v + cache_codes_at(page, w.h, p.c.heads, p.c.page_log2, D) +
+                                                           value_word_at((first + 16 * blk) & page_mask, 0, D)) + lane;
+#pragma unroll
+          for (int db = 0; db < D / 64; ++db) vc[blk * (D / 64) + db] = ok ? __ldg(at + 32 * db) : make_uint4(0, 0, 0, 0);
+        }
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(bar(kPrmEmpty + ps));
+      };
+      load(0);
+      for (int t = 0; t < it.count; ++t) {
+        const uint32_t m = it.n0 + uint32_t(t), use = m / S::kStages;
+        const int st = int(m % S::kStages);
+        if (use > 0) wait(kVEmpty + st, (use - 1) & 1u, tc::kStatusWaitEmpty);
+        const uint32_t at = sm + S::kV + st * S::kOperand;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+          const int blk = i / (D / 64), db = i % (D / 64);
+          const int tok = 32 * q + 16 * blk + 4 * tg;
+          const uint32_t a0 = __funnelshift_r(vc[i].x, vc[i].x, 4 * g), a1 = __funnelshift_r(vc[i].y, vc[i].y, 4 * g);
+          const uint32_t a2 = __funnelshift_r(vc[i].z, vc[i].z, 4 * g), a3 = __funnelshift_r(vc[i].w, vc[i].w, 4 * g);
+          const uint32_t row0 = at + (tok >> 6) * (D * 128) + (64 * db + 8 * g) * 128 + (tg & 1) * 8;
+          const uint32_t chunk = uint32_t(tok & 63) >> 3;
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            uint32_t x = __byte_perm(a0, a1, hf ? 0x7632 : 0x5410), y = __byte_perm(a2, a3, hf ? 0x7632 : 0x5410);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t dim = uint32_t(hf * 4 + e + g) & 7u;
+              const uint32_t to = row0 + dim * 128 + ((chunk ^ dim) << 4);
+              if (e & 1) {
+                sts64(to, hfma2(x & 0x00F000F0u, 0x2C002C00u, 0x80088008u), hfma2(y & 0x00F000F0u, 0x2C002C00u, 0x80088008u));
+                x >>= 8, y >>= 8;
+              } else {
+                sts64(to, hadd2(x & 0x000F000Fu, 0x80088008u), hadd2(y & 0x000F000Fu, 0x80088008u));
+              }
+            }
+          }
+        }
+        tc::fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(bar(kVFull + st));
+        if (t + 1 < it.count) load(t + 1);
+      }
+    });
+  } else if (warp < kParamWarp) {
+    // ================================================================ keys: 64 tokens a warp
+    const int q = warp - kKeyWarp;
+    constexpr int kLoads = D / 16;               // 16-byte loads per lane and tile
+    constexpr int kPieces = D / 32;              // 16-byte pieces of a row
+    const int page_mask = (1 << p.c.page_log2) - 1;
+    items([&](const Item& it) {
+      uint4 kc[kLoads];
+      // load i: piece e % kPieces of token 8 (e / kPieces) + lane % 8, e = 4 i + lane / 8
+      auto load = [&](int t) {
+        const uint32_t m = it.n0 + uint32_t(t);
+        const int ps = int(m % kParamStages), first = it.span.id(w.i0 + t) * kTile + 64 * q;
+        wait(kPrmFull + ps, (m / kParamStages) & 1u, tc::kStatusWaitFull);
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+          const int e = i * 4 + (lane >> 3), tok = (e / kPieces) * 8 + (lane & 7);
+          const int page = info[ps].page[4 * q + (tok >> 4)];
+          const uint4* at = reinterpret_cast<const uint4*>(p.c.k + cache_codes_at(page, w.h, p.c.heads, p.c.page_log2, D) +
+                                                           key_word_at((first + tok) & page_mask, (e % kPieces) * 4, D));
+          kc[i] = unsigned(page) < unsigned(p.c.n_pages) ? __ldg(at) : make_uint4(0, 0, 0, 0);
+        }
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(bar(kPrmEmpty + ps));
+      };
+      load(0);
+      for (int t = 0; t < it.count; ++t) {
+        const uint32_t m = it.n0 + uint32_t(t), use = m / S::kStages;
+        const int st = int(m % S::kStages);
+        if (use > 0) wait(kKEmpty + st, (use - 1) & 1u, tc::kStatusWaitEmpty);
+        const uint32_t at = sm + S::kK + st * S::kOperand;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+          const int e = i * 4 + (lane >> 3), tok = 64 * q + (e / kPieces) * 8 + (lane & 7);
+          const uint32_t u[4] = {kc[i].x, kc[i].y, kc[i].z, kc[i].w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int ch = (e % kPieces) * 4 + j;
+            const uint32_t x = u[j], y = x >> 8;
+            sts128(at + (ch >> 3) * (kTile * 128) + tok * 128 + (((ch & 7) ^ (tok & 7)) << 4), x & 0x000F000Fu,
+                   x & 0x00F000F0u, y & 0x000F000Fu, y & 0x00F000F0u);
+          }
+        }
+        tc::fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(bar(kKFull + st));
+        if (t + 1 < it.count) load(t + 1);
+      }
+    });
+  } else if (warp == kParamWarp) {
+    // ================================================================ parameters: tokens 32 j + lane
+    const int page_mask = (1 << p.c.page_log2) - 1;
+    items([&](const Item& it) {
+      const int* table = p.table + (long long)w.b * p.table_ld;
+      float sig = 0.f;                           // running power of two of the item
+      int page[4];
+      auto pages = [&](int t) {
+        const int first = it.span.id(w.i0 + t) * kTile;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int tok = first + 32 * j + lane;
+          page[j] = tok < w.rq.len ? table[tok >> p.c.page_log2] : -1;
+          if (tok < w.rq.len && (page[j] < 0 || page[j] >= p.c.n_pages)) {
+            atomicExch(&g_tiles_status, kBadPage);
+            page[j] = -1;
+          }
+        }
+      };
+      pages(0);
+      for (int t = 0; t < it.count; ++t) {
+        const uint32_t m = it.n0 + uint32_t(t);
+        const int ps = int(m % kParamStages), first = it.span.id(w.i0 + t) * kTile;
+        float2 kk[4], vv[4];
+        float top = kMinStep;
+        uint32_t valid[4];
+        bool all = true;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int tok = first + 32 * j + lane;
+          const bool see = page[j] >= 0 && tok <= it.last_pos &&
+                           (p.window == 0 || tok > it.first_pos - p.window || tok < p.sinks);
+          kk[j] = vv[j] = make_float2(0.f, 0.f);
+          if (see) {
+            const long long at = cache_pair_at(page[j], w.h, p.c.heads, p.c.page_log2, tok & page_mask);
+            kk[j] = lo_step<T>(__ldg(p.c.k_pair + at)), vv[j] = lo_step<T>(__ldg(p.c.v_pair + at));
+          }
+          valid[j] = __ballot_sync(0xffffffffu, see);
+          all = all && valid[j] == 0xffffffffu;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) top = fmaxf(top, vv[j].y);
+        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        sig = fmaxf(sig, pow2_above(top));
+        const float inv = 1.f / sig;
+        if (m >= kParamStages) wait(kPrmEmpty + ps, (m / kParamStages - 1) & 1u, tc::kStatusWaitEmpty);
+        float* prm = reinterpret_cast<float*>(raw_sm + (sm - tc::smem_addr(raw_sm)) + S::kParam + ps * S::kParamBytes);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int c = 32 * j + lane, at = (c >> 1) * 4 + (c & 1);
+          prm[at] = kk[j].y, prm[at + 2] = kk[j].x;
+          prm[256 + at] = vv[j].y * inv, prm[256 + at + 2] = fmaf(8.f, vv[j].y, vv[j].x);
+          if ((lane & 15) == 0) info[ps].page[2 * j + (lane >> 4)] = page[j];
+        }
+        if (lane == 0) {
+          info[ps].sig = sig;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) info[ps].valid[j] = valid[j];
+          info[ps].whole = all && first + kTile <= it.first_pos + 1 &&
+                           (p.window == 0 || first > it.last_pos - p.window || first + kTile <= p.sinks);
+        }
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(bar(kPrmFull + ps));
+        if (t + 1 < it.count) pages(t + 1);
+      }
+    });
+  } else {
+    // ================================================================ products
+    items([&](const Item& it) {
+      if (tc::elect_one()) {
+        const uint64_t tmpl = tc::smem_desc(0u, 16u, 1024u, 2u);
+        const uint32_t idesc_s = tc::instr_desc(0, 128, kTile), idesc_o = tc::instr_desc(0, 128, D);
+        auto scores = [&](uint32_t m) {
+          const int st = int(m % S::kStages);
+          wait(kKFull + st, (m / S::kStages) & 1u, tc::kStatusWaitFull);
+          // S's buffer held P of the tile before last: its product has to be through
+          if (m >= 2 + it.n0) wait_pv(m - 2);
+          tc::fence_after_sync();
+          const uint64_t a = tmpl | ((sm + S::kQ) >> 4), b = tmpl | ((sm + S::kK + st * S::kOperand) >> 4);
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+            mma_ss(tmem + 256 + 128 * (m & 1), a + (k >> 2) * 1024 + (k & 3) * 2, b + (k >> 2) * 1024 + (k & 3) * 2, idesc_s,
+                   k > 0);
+          tc::mma_commit(bar(kKEmpty + st));
+          tc::mma_commit(bar(kSFull + int(m & 1)));
+        };
+        scores(it.n0);
+        for (int t = 0; t < it.count; ++t) {
+          const uint32_t m = it.n0 + uint32_t(t);
+          if (t + 1 < it.count) scores(m + 1);
+          const int st = int(m % S::kStages);
+          wait(kVFull + st, (m / S::kStages) & 1u, tc::kStatusWaitFull);
+          wait(kPFull + int(m & 1), (m >> 1) & 1u, tc::kStatusWaitFull);
+          tc::fence_after_sync();
+          const uint64_t b = tmpl | ((sm + S::kV + st * S::kOperand) >> 4);
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            tc::mma_ts_kblock(tmem, tmem + 256 + 128 * (m & 1) + 32 * k, uint32_t(b) + k * (D * 8), uint32_t(b >> 32), idesc_o,
+                              t > 0 || k > 0);
+          tc::mma_commit(bar(kVEmpty + st));
+          tc::mma_commit(bar(kPvDone + int(m & 1)));
+        }
+      }
+      __syncwarp();
+    });
+  }
+  if (*abort_flag) {            // a wait gave up: products under way still read shared memory, for microseconds
+    const long long t0 = clock64();
+    while (clock64() - t0 < 400000) {
+    }
+    __syncthreads();
+  }
+  if (warp == kProductWarp) tc::tmem_dealloc(tmem, 512);
+}
+
+template <typename T, int D>
+int launch(const AttendParams& p, int blocks, cudaStream_t st) {
+  static bool configured[64] = {false};
+  int dev = 0;
+  B200LUT_CUDA_OK(cudaGetDevice(&dev));
+  if (dev >= 64 || !configured[dev]) {
+    B200LUT_CUDA_OK(cudaFuncSetAttribute(attend_tiles_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::kSmem));
+    if (dev < 64) configured[dev] = true;
+  }
+  attend_tiles_kernel<T, D><<<unsigned(blocks), kThreads, Shape<D>::kSmem, st>>>(p);
+  B200LUT_CUDA_OK(cudaGetLastError());
+  return B200LUT_OK;
+}
+
+}  // namespace
+
+int attend_tiles_status_take() {
+  int v = 0, zero = 0;
+  if (cudaMemcpyFromSymbol(&v, g_tiles_status, sizeof(int)) != cudaSuccess) return -1;
+  if (v != 0) cudaMemcpyToSymbol(g_tiles_status, &zero, sizeof(int));
+  return v == kBadPage || v == 0 ? v : 0x6300 + v;
+}
+
+int attend_tiles(const AttendParams& p, int dtype, int blocks, cudaStream_t st) {
+  const bool bf = dtype == B200LUT_BF16;
+  switch (p.c.D) {
+    case 64: return bf ? launch<__nv_bfloat16, 64>(p, blocks, st) : launch<__half, 64>(p, blocks, st);
+    case 128: return bf ? launch<__nv_bfloat16, 128>(p, blocks, st) : launch<__half, 128>(p, blocks, st);
+    default: return bf ? launch<__nv_bfloat16, 256>(p, blocks, st) : launch<__half, 256>(p, blocks, st);
+  }
+}
+
+}  // namespace b200lut

@@ -106,5 +106,6 @@ int embed_status_take();
 // Status words of the key/value cache (a slot outside it) and of the attention over it (a page outside it).
 int kv_status_take();
 int attend_status_take();
+int attend_tiles_status_take();
 
 }  // namespace b200lut

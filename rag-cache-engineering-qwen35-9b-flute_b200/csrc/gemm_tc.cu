@@ -1047,7 +1047,8 @@ extern "C" int b200lut_device_status(void) {
   const int c = b200lut::gemm_cluster_status_take();
   const int s = b200lut::kv_status_take();
   const int a = b200lut::attend_status_take();
-  return v != 0 ? v : c != 0 ? c : e != 0 ? e : g != 0 ? g : s != 0 ? s : a;
+  const int at = b200lut::attend_tiles_status_take();
+  return v != 0 ? v : c != 0 ? c : e != 0 ? e : g != 0 ? g : s != 0 ? s : at != 0 ? at : a;
 }
 
 namespace {

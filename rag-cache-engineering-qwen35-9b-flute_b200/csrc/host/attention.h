@@ -171,7 +171,7 @@ PyObject* attend(Guard&& guarded, Context&& context, PyObject* const* a, Py_ssiz
       const WithoutGil free;
       out = given ? *given : empty({T, Hq, D}, c->scalar, c->device);
       // a buffer of the current stream (of the capture's pool under capture): calls never share one
-      const size_t need = b200lut_attend_workspace_bytes(int(Hq), int(H), int(D));
+      const size_t need = b200lut_attend_workspace_bytes(int(Hq), int(H), int(D), !start);
       ws = empty({int64_t(need)}, at::kByte, c->device);
       b200lut_attend_args g = {};
       g.cache = &c->view;

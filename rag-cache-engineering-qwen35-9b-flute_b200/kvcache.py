@@ -227,7 +227,7 @@ class KVCache4:
         L = _lib.lib()
         with _lib._on_device(self.device):
             # a buffer of the current stream (of the capture's pool under capture): calls never share one
-            ws = torch.empty(L.b200lut_attend_workspace_bytes(Hq, self.n_kv_heads, D), dtype=torch.uint8, device=self.device)
+            ws = torch.empty(L.b200lut_attend_workspace_bytes(Hq, self.n_kv_heads, D, int(row_start is None)), dtype=torch.uint8, device=self.device)
             a = _lib.AttendArgs(ctypes.pointer(self._view), q.data_ptr(), _lib.ptr(gate), out.data_ptr(),
                                 block_table.data_ptr(), kv_len.data_ptr(), _lib.ptr(row_start), q.stride(0), q.stride(1),
                                 gate.stride(0) if gate is not None else 0, gate.stride(1) if gate is not None else 0,

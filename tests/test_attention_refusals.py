@@ -165,6 +165,6 @@ def test_c_attend():
     refused(call(args(), None, big, None), 4, "workspace")
     refused(call(args(), AT, 64, None), 4, "workspace")
     assert call(args(T=0), None, 0, None) == 0 and call(args(B=0), None, 0, None) == 0
-    assert L.b200lut_attend_workspace_bytes(16, 4, 256) > 0
+    assert L.b200lut_attend_workspace_bytes(16, 4, 256, 0) > L.b200lut_attend_workspace_bytes(16, 4, 256, 1) > 0
     for bad in ((0, 1, 64), (4, 3, 64), (4, 0, 64), (4, 2, 96)):
-        assert L.b200lut_attend_workspace_bytes(*bad) == 0
+        assert L.b200lut_attend_workspace_bytes(*bad, 1) == 0
