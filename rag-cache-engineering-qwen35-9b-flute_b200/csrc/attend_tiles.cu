@@ -101,16 +101,15 @@ __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint3
 __device__ __forceinline__ void sts64(uint32_t a, uint32_t x, uint32_t y) {
   asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(a), "r"(x), "r"(y) : "memory");
 }
-__device__ __forceinline__ void tmem_ld32(uint32_t t, float* v) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
-        "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]),
-        "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
-        "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
-      : "r"(t)
-      : "memory");
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ void tmem_st8(uint32_t t, const uint32_t (&v)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(t), "r"(v[0]), "r"(v[1]),
+               "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t t, const uint32_t (&v)[16]) {
   asm volatile(
@@ -374,14 +373,9 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
         wait(kSFull + int(m & 1), (m >> 1) & 1u, tc::kStatusWaitDone);
         tc::fence_after_sync();
         const uint32_t s_at = lane_base + 256 + 128 * (m & 1);
-        float s[64];
-        tmem_ld32(s_at + 64 * half, s);
-        tmem_ld32(s_at + 64 * half + 32, s + 32);
-        tc::wait_ld();
-        const uint32_t prm = sm + S::kParam + ps * S::kParamBytes + half * 512;
-        float2 top2[2] = {make_float2(-INFINITY, -INFINITY), make_float2(-INFINITY, -INFINITY)};
-        uint32_t mask[2] = {0xffffffffu, 0xffffffffu};
+        const uint32_t prm = sm + S::kParam + ps * S::kParamBytes + half * 512, mine = s_at + 64 * half;
         const bool whole = info[ps].whole != 0;
+        uint32_t mask[2] = {0xffffffffu, 0xffffffffu};
         if (!whole) {
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
@@ -391,23 +385,43 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
             if (p.window) mask[c] &= ~below(pos - p.window + 1 - f) | below(p.sinks - f);
           }
         }
+        // Two passes over 16 tokens at a time, the scores read from tensor memory in each: loops short enough for
+        // the instruction cache (unrolled over 64 tokens the kernel stalled on fetches more than on anything else).
+        auto score = [&](float4 k, uint32_t s0, uint32_t s1) {
+          return fma2(make_float2(k.x, k.y), make_float2(__uint_as_float(s0), __uint_as_float(s1)),
+                      mul2(make_float2(k.z, k.w), qs));
+        };
+        float top = -INFINITY;
+        if (whole) {
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t s[16];
+            tc::tmem_ld_32x32b_x16(mine + 16 * c, s);
+            float4 k[8];
 #pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          const float4 k = lds128f(prm + 16 * c);
-          const float2 y = fma2(make_float2(k.x, k.y), make_float2(s[2 * c], s[2 * c + 1]), mul2(make_float2(k.z, k.w), qs));
-          s[2 * c] = y.x, s[2 * c + 1] = y.y;
-        }
-        if (!whole) {
+            for (int e = 0; e < 8; ++e) k[e] = lds128f(prm + 128 * c + 16 * e);
+            tc::wait_ld();
 #pragma unroll
-          for (int c = 0; c < 64; ++c)
-            if (!((mask[c >> 5] >> (c & 31)) & 1u)) s[c] = -INFINITY;
-        }
+            for (int e = 0; e < 8; ++e) {
+              const float2 y = score(k[e], s[2 * e], s[2 * e + 1]);
+              top = max3(top, y.x, y.y);
+            }
+          }
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t s[16];
+            tc::tmem_ld_32x32b_x16(mine + 16 * c, s);
+            tc::wait_ld();
+            const uint32_t see = mask[c >> 1] >> (16 * (c & 1));
 #pragma unroll
-        for (int c = 0; c < 64; c += 4) {
-          top2[0].x = fmaxf(top2[0].x, s[c]), top2[0].y = fmaxf(top2[0].y, s[c + 1]);
-          top2[1].x = fmaxf(top2[1].x, s[c + 2]), top2[1].y = fmaxf(top2[1].y, s[c + 3]);
+            for (int e = 0; e < 8; ++e) {
+              const float2 y = score(lds128f(prm + 128 * c + 16 * e), s[2 * e], s[2 * e + 1]);
+              if ((see >> (2 * e)) & 1u) top = fmaxf(top, y.x);
+              if ((see >> (2 * e + 1)) & 1u) top = fmaxf(top, y.y);
+            }
+          }
         }
-        float top = fmaxf(fmaxf(top2[0].x, top2[0].y), fmaxf(top2[1].x, top2[1].y));
         half_top[m & 1][half][r] = top;
         pair_sync(1 + (warp & 3));
         top = fmaxf(top, half_top[m & 1][half ^ 1][r]) * qf.x;
@@ -422,7 +436,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
           if (t > 0) {         // each of the two threads rescales half of the row
             wait_pv(m - 1);
             tc::fence_after_sync();
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
               uint32_t o[16];
               const uint32_t at = lane_base + half * (D / 2) + 16 * c;
@@ -437,24 +451,44 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
         }
         const float off = m_run == -INFINITY ? 0.f : -m_run;
         const float2 off2 = make_float2(off, off);
+        // P of a half lies at the head of that half's scores: columns that this thread has read by then
+        if (whole) {
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t s[16], pk[8];
+            tc::tmem_ld_32x32b_x16(mine + 16 * c, s);
+            tc::wait_ld();
 #pragma unroll
-        for (int part = 0; part < 2; ++part) {
-          uint32_t pk[16];
-#pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            const int c = part * 16 + k;
-            float4 v = lds128f(prm + 1024 + 16 * c);
-            if (!whole) {        // a hidden token may be poisoned: 0 times NaN
-              if (!((mask[part] >> (2 * k)) & 1u)) v.x = v.z = 0.f;
-              if (!((mask[part] >> (2 * k + 1)) & 1u)) v.y = v.w = 0.f;
+            for (int e = 0; e < 8; ++e) {
+              const float2 x = fma2(score(lds128f(prm + 128 * c + 16 * e), s[2 * e], s[2 * e + 1]), qf, off2);
+              const float4 v = lds128f(prm + 1024 + 128 * c + 16 * e);
+              const float2 w2 = make_float2(ex2(x.x), ex2(x.y));
+              l2 = add2(l2, w2);
+              pm2 = fma2(w2, make_float2(v.z, v.w), pm2);
+              pk[e] = half2_of(mul2(w2, make_float2(v.x, v.y)));
             }
-            const float2 x = fma2(make_float2(s[2 * c], s[2 * c + 1]), qf, off2);
-            const float2 e = make_float2(ex2(x.x), ex2(x.y));
-            l2 = add2(l2, e);
-            pm2 = fma2(e, make_float2(v.z, v.w), pm2);
-            pk[k] = half2_of(mul2(e, make_float2(v.x, v.y)));
+            tmem_st8(mine + 8 * c, pk);
           }
-          tmem_st16(s_at + 32 * half + 16 * part, pk);
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t s[16], pk[8];
+            tc::tmem_ld_32x32b_x16(mine + 16 * c, s);
+            tc::wait_ld();
+            const uint32_t see = mask[c >> 1] >> (16 * (c & 1));
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float2 x = fma2(score(lds128f(prm + 128 * c + 16 * e), s[2 * e], s[2 * e + 1]), qf, off2);
+              float4 v = lds128f(prm + 1024 + 128 * c + 16 * e);
+              float2 w2 = make_float2(ex2(x.x), ex2(x.y));
+              if (!((see >> (2 * e)) & 1u)) w2.x = v.x = v.z = 0.f;        // what is hidden may be poisoned
+              if (!((see >> (2 * e + 1)) & 1u)) w2.y = v.y = v.w = 0.f;
+              l2 = add2(l2, w2);
+              pm2 = fma2(w2, make_float2(v.z, v.w), pm2);
+              pk[e] = half2_of(mul2(w2, make_float2(v.x, v.y)));
+            }
+            tmem_st8(mine + 8 * c, pk);
+          }
         }
         tc::wait_st();
         tc::fence_before_sync();
@@ -482,7 +516,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
       const long long slot = 2LL * blockIdx.x + (starts ? 1 : 0);
       const long long tok = w.rq.row0 + (it.r0 + r) / p.G;
       const int head = w.h * p.G + int((it.r0 + r) % p.G);
-#pragma unroll
+#pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         uint32_t o[16];
         const int d = half * (D / 2) + 16 * c;
@@ -526,52 +560,69 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
   } else if (warp < kKeyWarp) {
     // ================================================================ values: 32 tokens a warp
     const int q = warp - kValueWarp, tg = lane >> 3, g = lane & 7;
-    constexpr int kLoads = D / 32;               // 16-byte loads per lane and tile
+    constexpr int kLoads = D / 32, kBlocks = D / 64;       // 16-byte loads per lane and tile
     const int page_mask = (1 << p.c.page_log2) - 1;
+    // where the pair of element (n + g) % 8 goes: row, chunk of the swizzle, half of the chunk; a step of 16 tokens
+    // flips bit 1 of the chunk
+    uint32_t put[8];
+    {
+      const int tok = 32 * q + 4 * tg;
+#pragma unroll
+      for (int n = 0; n < 8; ++n) {
+        const uint32_t dim = uint32_t(n + g) & 7u;
+        put[n] = sm + S::kV + (tok >> 6) * (D * 128) + (8 * g + dim) * 128 + ((((tok & 63) >> 3) ^ dim) << 4) + (tg & 1) * 8;
+      }
+    }
     items([&](const Item& it) {
       uint4 vc[kLoads];
-      auto load = [&](int t) {
+      const uint4* from[2];
+      bool ok[2];
+      auto locate = [&](int t) {
         const uint32_t m = it.n0 + uint32_t(t);
         const int ps = int(m % kParamStages), first = it.span.id(w.i0 + t) * kTile + 32 * q;
         wait(kPrmFull + ps, (m / kParamStages) & 1u, tc::kStatusWaitFull);
 #pragma unroll
         for (int blk = 0; blk < 2; ++blk) {
           const int page = info[ps].page[2 * q + blk];
-          const bool ok = unsigned(page) < unsigned(p.c.n_pages);      // after a wait that gave up it may be anything
-          const uint4* at = reinterpret_cast<const uint4*>(p.c.v + cache_codes_at(page, w.h, p.c.heads, p.c.page_log2, D) +
-                                                           value_word_at((first + 16 * blk) & page_mask, 0, D)) + lane;
-#pragma unroll
-          for (int db = 0; db < D / 64; ++db) vc[blk * (D / 64) + db] = ok ? __ldg(at + 32 * db) : make_uint4(0, 0, 0, 0);
+          ok[blk] = unsigned(page) < unsigned(p.c.n_pages);      // after a wait that gave up it may be anything
+          from[blk] = reinterpret_cast<const uint4*>(p.c.v + cache_codes_at(ok[blk] ? page : 0, w.h, p.c.heads, p.c.page_log2, D) +
+                                                     value_word_at((first + 16 * blk) & page_mask, 0, D)) + lane;
         }
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(bar(kPrmEmpty + ps));
       };
-      load(0);
+      auto load = [&](int i) {
+        vc[i] = ok[i / kBlocks] ? __ldg(from[i / kBlocks] + 32 * (i % kBlocks)) : make_uint4(0, 0, 0, 0);
+      };
+      locate(0);
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) load(i);
       for (int t = 0; t < it.count; ++t) {
         const uint32_t m = it.n0 + uint32_t(t), use = m / S::kStages;
         const int st = int(m % S::kStages);
+        const bool more = t + 1 < it.count;
+        if (more) locate(t + 1);
         if (use > 0) wait(kVEmpty + st, (use - 1) & 1u, tc::kStatusWaitEmpty);
-        const uint32_t at = sm + S::kV + st * S::kOperand;
+        uint32_t to[8];
+#pragma unroll
+        for (int n = 0; n < 8; ++n) to[n] = put[n] + st * S::kOperand;
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-          const int blk = i / (D / 64), db = i % (D / 64);
-          const int tok = 32 * q + 16 * blk + 4 * tg;
+          const int blk = i / kBlocks, db = i % kBlocks;
           const uint32_t a0 = __funnelshift_r(vc[i].x, vc[i].x, 4 * g), a1 = __funnelshift_r(vc[i].y, vc[i].y, 4 * g);
           const uint32_t a2 = __funnelshift_r(vc[i].z, vc[i].z, 4 * g), a3 = __funnelshift_r(vc[i].w, vc[i].w, 4 * g);
-          const uint32_t row0 = at + (tok >> 6) * (D * 128) + (64 * db + 8 * g) * 128 + (tg & 1) * 8;
-          const uint32_t chunk = uint32_t(tok & 63) >> 3;
+          if (more) load(i);                     // the next tile's, into the registers just read
 #pragma unroll
           for (int hf = 0; hf < 2; ++hf) {
             uint32_t x = __byte_perm(a0, a1, hf ? 0x7632 : 0x5410), y = __byte_perm(a2, a3, hf ? 0x7632 : 0x5410);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const uint32_t dim = uint32_t(hf * 4 + e + g) & 7u;
-              const uint32_t to = row0 + dim * 128 + ((chunk ^ dim) << 4);
+              const uint32_t at = (blk ? to[hf * 4 + e] ^ 32u : to[hf * 4 + e]) + db * 8192;
               if (e & 1) {
-                sts64(to, hfma2(x & 0x00F000F0u, 0x2C002C00u, 0x80088008u), hfma2(y & 0x00F000F0u, 0x2C002C00u, 0x80088008u));
+                sts64(at, hfma2(x & 0x00F000F0u, 0x2C002C00u, 0x80088008u), hfma2(y & 0x00F000F0u, 0x2C002C00u, 0x80088008u));
                 x >>= 8, y >>= 8;
               } else {
-                sts64(to, hadd2(x & 0x000F000Fu, 0x80088008u), hadd2(y & 0x000F000Fu, 0x80088008u));
+                sts64(at, hadd2(x & 0x000F000Fu, 0x80088008u), hadd2(y & 0x000F000Fu, 0x80088008u));
               }
             }
           }
@@ -579,55 +630,68 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
         tc::fence_proxy_async();
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(bar(kVFull + st));
-        if (t + 1 < it.count) load(t + 1);
       }
     });
   } else if (warp < kParamWarp) {
     // ================================================================ keys: 64 tokens a warp
-    const int q = warp - kKeyWarp;
+    const int q = warp - kKeyWarp, l8 = lane >> 3, tk = lane & 7;
     constexpr int kLoads = D / 16;               // 16-byte loads per lane and tile
-    constexpr int kPieces = D / 32;              // 16-byte pieces of a row
     const int page_mask = (1 << p.c.page_log2) - 1;
+    // load i: piece e % (D / 32) of token 8 (e / (D / 32)) + lane % 8 of the warp's 64, e = 4 i + lane / 8
+    constexpr int kPer = D == 256 ? 2 : 1;       // loads that stay with the same tokens
+    const int tok0 = (D == 64 ? 8 * (l8 >> 1) : 0) + tk, piece0 = D == 64 ? (l8 & 1) : l8;
+    constexpr int kTokStep = D == 64 ? 16 : 8;   // tokens between the loads (between pairs of loads for 256)
+    uint32_t put[4];                             // word j of the piece
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int ch = piece0 * 4 + j;
+      put[j] = sm + S::kK + (ch >> 3) * (kTile * 128) + (64 * q + tok0) * 128 + (((ch & 7) ^ tk) << 4);
+    }
     items([&](const Item& it) {
       uint4 kc[kLoads];
-      // load i: piece e % kPieces of token 8 (e / kPieces) + lane % 8, e = 4 i + lane / 8
-      auto load = [&](int t) {
+      int page[4], first = 0;
+      auto locate = [&](int t) {
         const uint32_t m = it.n0 + uint32_t(t);
-        const int ps = int(m % kParamStages), first = it.span.id(w.i0 + t) * kTile + 64 * q;
+        const int ps = int(m % kParamStages);
+        first = it.span.id(w.i0 + t) * kTile + 64 * q;
         wait(kPrmFull + ps, (m / kParamStages) & 1u, tc::kStatusWaitFull);
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-          const int e = i * 4 + (lane >> 3), tok = (e / kPieces) * 8 + (lane & 7);
-          const int page = info[ps].page[4 * q + (tok >> 4)];
-          const uint4* at = reinterpret_cast<const uint4*>(p.c.k + cache_codes_at(page, w.h, p.c.heads, p.c.page_log2, D) +
-                                                           key_word_at((first + tok) & page_mask, (e % kPieces) * 4, D));
-          kc[i] = unsigned(page) < unsigned(p.c.n_pages) ? __ldg(at) : make_uint4(0, 0, 0, 0);
-        }
+        for (int j = 0; j < 4; ++j) page[j] = info[ps].page[4 * q + j];
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(bar(kPrmEmpty + ps));
       };
-      load(0);
+      auto load = [&](int i) {
+        const int step = (i / kPer) * kTokStep, pg = page[step >> 4];      // tok0 < 16: the same 16 tokens
+        const uint8_t* at = p.c.k + cache_codes_at(pg, w.h, p.c.heads, p.c.page_log2, D) +
+                            key_word_at((first + tok0 + step) & page_mask, (piece0 + (kPer == 2 ? 4 * (i & 1) : 0)) * 4, D);
+        kc[i] = unsigned(pg) < unsigned(p.c.n_pages) ? __ldg(reinterpret_cast<const uint4*>(at)) : make_uint4(0, 0, 0, 0);
+      };
+      locate(0);
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) load(i);
       for (int t = 0; t < it.count; ++t) {
         const uint32_t m = it.n0 + uint32_t(t), use = m / S::kStages;
         const int st = int(m % S::kStages);
+        const bool more = t + 1 < it.count;
+        if (more) locate(t + 1);
         if (use > 0) wait(kKEmpty + st, (use - 1) & 1u, tc::kStatusWaitEmpty);
-        const uint32_t at = sm + S::kK + st * S::kOperand;
+        uint32_t to[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) to[j] = put[j] + st * S::kOperand;
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-          const int e = i * 4 + (lane >> 3), tok = 64 * q + (e / kPieces) * 8 + (lane & 7);
           const uint32_t u[4] = {kc[i].x, kc[i].y, kc[i].z, kc[i].w};
+          if (more) load(i);                     // the next tile's, into the registers just read
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const int ch = (e % kPieces) * 4 + j;
             const uint32_t x = u[j], y = x >> 8;
-            sts128(at + (ch >> 3) * (kTile * 128) + tok * 128 + (((ch & 7) ^ (tok & 7)) << 4), x & 0x000F000Fu,
+            sts128(to[j] + (i / kPer) * (kTokStep * 128) + (kPer == 2 ? (i & 1) * (2 * kTile * 128) : 0), x & 0x000F000Fu,
                    x & 0x00F000F0u, y & 0x000F000Fu, y & 0x00F000F0u);
           }
         }
         tc::fence_proxy_async();
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(bar(kKFull + st));
-        if (t + 1 < it.count) load(t + 1);
       }
     });
   } else if (warp == kParamWarp) {
@@ -636,20 +700,38 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
     items([&](const Item& it) {
       const int* table = p.table + (long long)w.b * p.table_ld;
       float sig = 0.f;                           // running power of two of the item
-      int page[4];
-      auto pages = [&](int t) {
+      int page[4], page_next[4];                 // this tile's, the next one's
+      uint32_t kp[4], vp[4];                     // pairs of this tile
+      auto pages = [&](int t, int (&to)[4]) {
         const int first = it.span.id(w.i0 + t) * kTile;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int tok = first + 32 * j + lane;
-          page[j] = tok < w.rq.len ? table[tok >> p.c.page_log2] : -1;
-          if (tok < w.rq.len && (page[j] < 0 || page[j] >= p.c.n_pages)) {
+          to[j] = tok < w.rq.len ? table[tok >> p.c.page_log2] : -1;
+        }
+      };
+      auto seen = [&](int tok, int pg) {
+        return pg >= 0 && tok <= it.last_pos && (p.window == 0 || tok > it.first_pos - p.window || tok < p.sinks);
+      };
+      auto pairs = [&](int t) {                  // checks the pages too
+        const int first = it.span.id(w.i0 + t) * kTile;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int tok = first + 32 * j + lane;
+          if (tok < w.rq.len && unsigned(page[j]) >= unsigned(p.c.n_pages)) {
             atomicExch(&g_tiles_status, kBadPage);
             page[j] = -1;
           }
+          kp[j] = vp[j] = 0;
+          if (seen(tok, page[j])) {
+            const long long at = cache_pair_at(page[j], w.h, p.c.heads, p.c.page_log2, tok & page_mask);
+            kp[j] = __ldg(p.c.k_pair + at), vp[j] = __ldg(p.c.v_pair + at);
+          }
         }
       };
-      pages(0);
+      pages(0, page);
+      pairs(0);
+      if (it.count > 1) pages(1, page_next);
       for (int t = 0; t < it.count; ++t) {
         const uint32_t m = it.n0 + uint32_t(t);
         const int ps = int(m % kParamStages), first = it.span.id(w.i0 + t) * kTile;
@@ -659,19 +741,16 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
         bool all = true;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int tok = first + 32 * j + lane;
-          const bool see = page[j] >= 0 && tok <= it.last_pos &&
-                           (p.window == 0 || tok > it.first_pos - p.window || tok < p.sinks);
-          kk[j] = vv[j] = make_float2(0.f, 0.f);
-          if (see) {
-            const long long at = cache_pair_at(page[j], w.h, p.c.heads, p.c.page_log2, tok & page_mask);
-            kk[j] = lo_step<T>(__ldg(p.c.k_pair + at)), vv[j] = lo_step<T>(__ldg(p.c.v_pair + at));
-          }
-          valid[j] = __ballot_sync(0xffffffffu, see);
+          kk[j] = lo_step<T>(kp[j]), vv[j] = lo_step<T>(vp[j]);
+          valid[j] = __ballot_sync(0xffffffffu, seen(first + 32 * j + lane, page[j]));
           all = all && valid[j] == 0xffffffffu;
+          top = fmaxf(top, vv[j].y);
         }
+        int now[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) top = fmaxf(top, vv[j].y);
+        for (int j = 0; j < 4; ++j) now[j] = page[j], page[j] = page_next[j];
+        if (t + 1 < it.count) pairs(t + 1);      // under way while this tile's are written
+        if (t + 2 < it.count) pages(t + 2, page_next);
         for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         sig = fmaxf(sig, pow2_above(top));
         const float inv = 1.f / sig;
@@ -682,7 +761,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
           const int c = 32 * j + lane, at = (c >> 1) * 4 + (c & 1);
           prm[at] = kk[j].y, prm[at + 2] = kk[j].x;
           prm[256 + at] = vv[j].y * inv, prm[256 + at + 2] = fmaf(8.f, vv[j].y, vv[j].x);
-          if ((lane & 15) == 0) info[ps].page[2 * j + (lane >> 4)] = page[j];
+          if ((lane & 15) == 0) info[ps].page[2 * j + (lane >> 4)] = now[j];
         }
         if (lane == 0) {
           info[ps].sig = sig;
@@ -693,7 +772,6 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
         }
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(bar(kPrmFull + ps));
-        if (t + 1 < it.count) pages(t + 1);
       }
     });
   } else {
@@ -727,7 +805,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
           const uint64_t b = tmpl | ((sm + S::kV + st * S::kOperand) >> 4);
 #pragma unroll
           for (int k = 0; k < 2; ++k)
-            tc::mma_ts_kblock(tmem, tmem + 256 + 128 * (m & 1) + 32 * k, uint32_t(b) + k * (D * 8), uint32_t(b >> 32), idesc_o,
+            tc::mma_ts_kblock(tmem, tmem + 256 + 128 * (m & 1) + 64 * k, uint32_t(b) + k * (D * 8), uint32_t(b >> 32), idesc_o,
                               t > 0 || k > 0);
           tc::mma_commit(bar(kVEmpty + st));
           tc::mma_commit(bar(kPvDone + int(m & 1)));
