@@ -127,11 +127,6 @@ __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint3
       : "memory");
 }
 
-__device__ __forceinline__ float4 lds128f(uint32_t a) {
-  float4 r;
-  asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(r.x), "=f"(r.y), "=f"(r.z), "=f"(r.w) : "r"(a) : "memory");
-  return r;
-}
 __device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
 
 // ---- the line of tiles ---------------------------------------------------------------------------------------
@@ -177,7 +172,7 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_constant__ AttendParams p) {
   using S = Shape<D>;
   extern __shared__ uint8_t raw_sm[];
-  __shared__ __align__(8) uint64_t bars[24];
+  __shared__ __align__(8) uint64_t bars[32];
   __shared__ uint32_t tmem_base;
   __shared__ int abort_word;
   __shared__ float2 row_k[kRows];              // factor of the scores, sum of the scaled row
@@ -189,11 +184,15 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
   __shared__ int first_b;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t sm = (tc::smem_addr(raw_sm) + 1023u) & ~1023u;
+  const uint32_t base_off = sm - tc::smem_addr(raw_sm);
   volatile int* abort_flag = &abort_word;
   const uint32_t bar0 = tc::smem_addr(bars);
   auto bar = [&](int i) { return bar0 + 8u * uint32_t(i); };
-  constexpr int kKFull = 0, kKEmpty = 2, kVFull = 4, kVEmpty = 6, kSFull = 8, kPFull = 10, kPvDone = 12, kPrmFull = 14,
-                kPrmEmpty = 18;
+  // keys are handed over in blocks of 64 elements, values in blocks of 64 tokens: [stage][block]
+  constexpr int kKB = D / 64, kKBars = S::kStages * kKB, kVBars = S::kStages * 2;
+  constexpr int kKFull = 0, kKEmpty = 4, kVFull = 8, kVEmpty = 12, kSFull = 16, kPFull = 18, kPvDone = 20, kPrmFull = 22,
+                kPrmEmpty = 26;
+  static_assert(kKBars <= 4 && kVBars <= 4, "barriers");
 
   // ---- this block's share
   if (tid == 0) {
@@ -232,11 +231,10 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
   }
   if (warp == kProductWarp) tc::tmem_alloc(tc::smem_addr(&tmem_base), 512);
   if (tid == 0) {
-    for (int i = 0; i < 2; ++i) {
-      tc::mbar_init(bar(kKFull + i), 2), tc::mbar_init(bar(kKEmpty + i), 1);
-      tc::mbar_init(bar(kVFull + i), 4), tc::mbar_init(bar(kVEmpty + i), 1);
+    for (int i = 0; i < kKBars; ++i) tc::mbar_init(bar(kKFull + i), 2), tc::mbar_init(bar(kKEmpty + i), 1);
+    for (int i = 0; i < kVBars; ++i) tc::mbar_init(bar(kVFull + i), 2), tc::mbar_init(bar(kVEmpty + i), 1);
+    for (int i = 0; i < 2; ++i)
       tc::mbar_init(bar(kSFull + i), 1), tc::mbar_init(bar(kPFull + i), 8), tc::mbar_init(bar(kPvDone + i), 1);
-    }
     for (int i = 0; i < kParamStages; ++i) tc::mbar_init(bar(kPrmFull + i), 1), tc::mbar_init(bar(kPrmEmpty + i), 14);
     tc::mbar_init_fence();
   }
@@ -373,7 +371,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
         wait(kSFull + int(m & 1), (m >> 1) & 1u, tc::kStatusWaitDone);
         tc::fence_after_sync();
         const uint32_t s_at = lane_base + 256 + 128 * (m & 1);
-        const uint32_t prm = sm + S::kParam + ps * S::kParamBytes + half * 512, mine = s_at + 64 * half;
+        const float4* prm = reinterpret_cast<const float4*>(raw_sm + base_off + S::kParam + ps * S::kParamBytes) + 32 * half;
+        const uint32_t mine = s_at + 64 * half;
         const bool whole = info[ps].whole != 0;
         uint32_t mask[2] = {0xffffffffu, 0xffffffffu};
         if (!whole) {
@@ -385,29 +384,66 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
             if (p.window) mask[c] &= ~below(pos - p.window + 1 - f) | below(p.sinks - f);
           }
         }
-        // Two passes over 16 tokens at a time, the scores read from tensor memory in each: loops short enough for
-        // the instruction cache (unrolled over 64 tokens the kernel stalled on fetches more than on anything else).
         auto score = [&](float4 k, uint32_t s0, uint32_t s1) {
           return fma2(make_float2(k.x, k.y), make_float2(__uint_as_float(s0), __uint_as_float(s1)),
                       mul2(make_float2(k.z, k.w), qs));
         };
-        float top = -INFINITY;
-        if (whole) {
+        const float sig_new = info[ps].sig;
+        // O times `ab`, each of the two threads half of the row; the products in flight have to be through
+        auto rescale = [&](float ab) {
+          wait_pv(m - 1);
+          tc::fence_after_sync();
 #pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[16];
+            const uint32_t at = lane_base + half * (D / 2) + 16 * c;
+            tc::tmem_ld_32x32b_x16(at, o);
+            tc::wait_ld();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * ab);
+            tmem_st16(at, o);
+          }
+          tc::wait_st();
+        };
+        bool done = false;
+        if (whole && t > 0 && __all_sync(0xffffffffu, m_run > -INFINITY || r >= it.n_rows)) {
+          // One pass under the maximum so far, P kept in registers: it holds unless a score is more than 2^8 above.
+          const float2 off2 = make_float2(-m_run, -m_run);
+          const float2 l_old = l2, pm_old = pm2;
+          float top = -INFINITY;
+          uint32_t pk[32];
+#pragma unroll
           for (int c = 0; c < 4; ++c) {
             uint32_t s[16];
             tc::tmem_ld_32x32b_x16(mine + 16 * c, s);
-            float4 k[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) k[e] = lds128f(prm + 128 * c + 16 * e);
             tc::wait_ld();
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-              const float2 y = score(k[e], s[2 * e], s[2 * e + 1]);
-              top = max3(top, y.x, y.y);
+              const float2 x = fma2(score(prm[8 * c + e], s[2 * e], s[2 * e + 1]), qf, off2);
+              top = max3(top, x.x, x.y);
+              const float4 v = prm[64 + 8 * c + e];
+              const float2 w2 = make_float2(ex2(x.x), ex2(x.y));
+              l2 = add2(l2, w2);
+              pm2 = fma2(w2, make_float2(v.z, v.w), pm2);
+              pk[8 * c + e] = half2_of(mul2(w2, make_float2(v.x, v.y)));
             }
           }
-        } else {
+          half_top[m & 1][half][r] = top;
+          pair_sync(1 + (warp & 3));
+          top = fmaxf(top, half_top[m & 1][half ^ 1][r]);
+          done = !__any_sync(0xffffffffu, top > kLazy && r < it.n_rows);
+          if (done) {
+            if (sig_new != sig_run) rescale(sig_run / sig_new), sig_run = sig_new;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) tmem_st16(mine + 16 * c, reinterpret_cast<const uint32_t(&)[16]>(pk[16 * c]));
+          } else {
+            l2 = l_old, pm2 = pm_old;
+            pair_sync(1 + (warp & 3));           // half_top is written again
+          }
+        }
+        if (!done) {
+          // Two passes over 16 tokens at a time, the scores read from tensor memory in each.
+          float top = -INFINITY;
 #pragma unroll 1
           for (int c = 0; c < 4; ++c) {
             uint32_t s[16];
@@ -416,60 +452,26 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
             const uint32_t see = mask[c >> 1] >> (16 * (c & 1));
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-              const float2 y = score(lds128f(prm + 128 * c + 16 * e), s[2 * e], s[2 * e + 1]);
+              const float2 y = score(prm[8 * c + e], s[2 * e], s[2 * e + 1]);
               if ((see >> (2 * e)) & 1u) top = fmaxf(top, y.x);
               if ((see >> (2 * e + 1)) & 1u) top = fmaxf(top, y.y);
             }
           }
-        }
-        half_top[m & 1][half][r] = top;
-        pair_sync(1 + (warp & 3));
-        top = fmaxf(top, half_top[m & 1][half ^ 1][r]) * qf.x;
-        const float sig_new = info[ps].sig;
-        if (__any_sync(0xffffffffu, top > m_run + kLazy || sig_new != sig_run)) {
-          const float m_new = fmaxf(m_run, top);
-          const float alpha = m_new == -INFINITY ? 1.f : ex2(m_run - m_new);
-          const float ab = alpha * (sig_run / sig_new);
-          m_run = m_new, sig_run = sig_new;
-          l2 = mul2(l2, make_float2(alpha, alpha));
-          pm2 = mul2(pm2, make_float2(alpha, alpha));
-          if (t > 0) {         // each of the two threads rescales half of the row
-            wait_pv(m - 1);
-            tc::fence_after_sync();
-#pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-              uint32_t o[16];
-              const uint32_t at = lane_base + half * (D / 2) + 16 * c;
-              tc::tmem_ld_32x32b_x16(at, o);
-              tc::wait_ld();
-#pragma unroll
-              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * ab);
-              tmem_st16(at, o);
-            }
-            tc::wait_st();
+          half_top[m & 1][half][r] = top;
+          pair_sync(1 + (warp & 3));
+          top = fmaxf(top, half_top[m & 1][half ^ 1][r]) * qf.x;
+          if (__any_sync(0xffffffffu, top > m_run + kLazy || sig_new != sig_run)) {
+            const float m_new = fmaxf(m_run, top);
+            const float alpha = m_new == -INFINITY ? 1.f : ex2(m_run - m_new);
+            const float ab = alpha * (sig_run / sig_new);
+            m_run = m_new, sig_run = sig_new;
+            l2 = mul2(l2, make_float2(alpha, alpha));
+            pm2 = mul2(pm2, make_float2(alpha, alpha));
+            if (t > 0) rescale(ab);
           }
-        }
-        const float off = m_run == -INFINITY ? 0.f : -m_run;
-        const float2 off2 = make_float2(off, off);
-        // P of a half lies at the head of that half's scores: columns that this thread has read by then
-        if (whole) {
-#pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
-            uint32_t s[16], pk[8];
-            tc::tmem_ld_32x32b_x16(mine + 16 * c, s);
-            tc::wait_ld();
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float2 x = fma2(score(lds128f(prm + 128 * c + 16 * e), s[2 * e], s[2 * e + 1]), qf, off2);
-              const float4 v = lds128f(prm + 1024 + 128 * c + 16 * e);
-              const float2 w2 = make_float2(ex2(x.x), ex2(x.y));
-              l2 = add2(l2, w2);
-              pm2 = fma2(w2, make_float2(v.z, v.w), pm2);
-              pk[e] = half2_of(mul2(w2, make_float2(v.x, v.y)));
-            }
-            tmem_st8(mine + 8 * c, pk);
-          }
-        } else {
+          const float off = m_run == -INFINITY ? 0.f : -m_run;
+          const float2 off2 = make_float2(off, off);
+          // P of a half lies at the head of that half's scores: columns that this thread has read by then
 #pragma unroll 1
           for (int c = 0; c < 4; ++c) {
             uint32_t s[16], pk[8];
@@ -478,8 +480,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
             const uint32_t see = mask[c >> 1] >> (16 * (c & 1));
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-              const float2 x = fma2(score(lds128f(prm + 128 * c + 16 * e), s[2 * e], s[2 * e + 1]), qf, off2);
-              float4 v = lds128f(prm + 1024 + 128 * c + 16 * e);
+              const float2 x = fma2(score(prm[8 * c + e], s[2 * e], s[2 * e + 1]), qf, off2);
+              float4 v = prm[64 + 8 * c + e];
               float2 w2 = make_float2(ex2(x.x), ex2(x.y));
               if (!((see >> (2 * e)) & 1u)) w2.x = v.x = v.z = 0.f;        // what is hidden may be poisoned
               if (!((see >> (2 * e + 1)) & 1u)) w2.y = v.y = v.w = 0.f;
@@ -560,7 +562,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
   } else if (warp < kKeyWarp) {
     // ================================================================ values: 32 tokens a warp
     const int q = warp - kValueWarp, tg = lane >> 3, g = lane & 7;
-    constexpr int kLoads = D / 32, kBlocks = D / 64;       // 16-byte loads per lane and tile
+    constexpr int kBlocks = D / 64;              // 16-byte loads per lane and 16 tokens
     const int page_mask = (1 << p.c.page_log2) - 1;
     // where the pair of element (n + g) % 8 goes: row, chunk of the swizzle, half of the chunk; a step of 16 tokens
     // flips bit 1 of the chunk
@@ -574,9 +576,9 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
       }
     }
     items([&](const Item& it) {
-      uint4 vc[kLoads];
-      const uint4* from[2];
-      bool ok[2];
+      uint4 vc[kBlocks];                         // the next 16 tokens'
+      const uint4 *from[2], *next;
+      bool ok[2], next_ok;
       auto locate = [&](int t) {
         const uint32_t m = it.n0 + uint32_t(t);
         const int ps = int(m % kParamStages), first = it.span.id(w.i0 + t) * kTile + 32 * q;
@@ -591,107 +593,112 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(bar(kPrmEmpty + ps));
       };
-      auto load = [&](int i) {
-        vc[i] = ok[i / kBlocks] ? __ldg(from[i / kBlocks] + 32 * (i % kBlocks)) : make_uint4(0, 0, 0, 0);
-      };
+      auto load = [&](int i) { vc[i] = next_ok ? __ldg(next + 32 * i) : make_uint4(0, 0, 0, 0); };
       locate(0);
+      next = from[0], next_ok = ok[0];
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) load(i);
+      for (int i = 0; i < kBlocks; ++i) load(i);
       for (int t = 0; t < it.count; ++t) {
         const uint32_t m = it.n0 + uint32_t(t), use = m / S::kStages;
-        const int st = int(m % S::kStages);
-        const bool more = t + 1 < it.count;
-        if (more) locate(t + 1);
-        if (use > 0) wait(kVEmpty + st, (use - 1) & 1u, tc::kStatusWaitEmpty);
-        uint32_t to[8];
+        const int st = int(m % S::kStages), vb = 2 * st + (q >> 1);
+        if (use > 0) wait(kVEmpty + vb, (use - 1) & 1u, tc::kStatusWaitEmpty);
+#pragma unroll 1
+        for (int blk = 0; blk < 2; ++blk) {
+          if (blk == 0) {
+            next = from[1], next_ok = ok[1];
+          } else if (t + 1 < it.count) {
+            locate(t + 1);
+            next = from[0], next_ok = ok[0];
+          } else {
+            next_ok = false;
+          }
+          uint32_t to[8];
 #pragma unroll
-        for (int n = 0; n < 8; ++n) to[n] = put[n] + st * S::kOperand;
+          for (int n = 0; n < 8; ++n) to[n] = (put[n] ^ uint32_t(32 * blk)) + st * S::kOperand;
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-          const int blk = i / kBlocks, db = i % kBlocks;
-          const uint32_t a0 = __funnelshift_r(vc[i].x, vc[i].x, 4 * g), a1 = __funnelshift_r(vc[i].y, vc[i].y, 4 * g);
-          const uint32_t a2 = __funnelshift_r(vc[i].z, vc[i].z, 4 * g), a3 = __funnelshift_r(vc[i].w, vc[i].w, 4 * g);
-          if (more) load(i);                     // the next tile's, into the registers just read
+          for (int db = 0; db < kBlocks; ++db) {
+            const uint32_t a0 = __funnelshift_r(vc[db].x, vc[db].x, 4 * g), a1 = __funnelshift_r(vc[db].y, vc[db].y, 4 * g);
+            const uint32_t a2 = __funnelshift_r(vc[db].z, vc[db].z, 4 * g), a3 = __funnelshift_r(vc[db].w, vc[db].w, 4 * g);
+            load(db);                            // into the registers just read
 #pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            uint32_t x = __byte_perm(a0, a1, hf ? 0x7632 : 0x5410), y = __byte_perm(a2, a3, hf ? 0x7632 : 0x5410);
+            for (int hf = 0; hf < 2; ++hf) {
+              uint32_t x = __byte_perm(a0, a1, hf ? 0x7632 : 0x5410), y = __byte_perm(a2, a3, hf ? 0x7632 : 0x5410);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint32_t at = (blk ? to[hf * 4 + e] ^ 32u : to[hf * 4 + e]) + db * 8192;
-              if (e & 1) {
-                sts64(at, hfma2(x & 0x00F000F0u, 0x2C002C00u, 0x80088008u), hfma2(y & 0x00F000F0u, 0x2C002C00u, 0x80088008u));
-                x >>= 8, y >>= 8;
-              } else {
-                sts64(at, hadd2(x & 0x000F000Fu, 0x80088008u), hadd2(y & 0x000F000Fu, 0x80088008u));
+              for (int e = 0; e < 4; ++e) {
+                const uint32_t at = to[hf * 4 + e] + db * 8192;
+                if (e & 1) {
+                  sts64(at, hfma2(x & 0x00F000F0u, 0x2C002C00u, 0x80088008u), hfma2(y & 0x00F000F0u, 0x2C002C00u, 0x80088008u));
+                  x >>= 8, y >>= 8;
+                } else {
+                  sts64(at, hadd2(x & 0x000F000Fu, 0x80088008u), hadd2(y & 0x000F000Fu, 0x80088008u));
+                }
               }
             }
           }
         }
         tc::fence_proxy_async();
         __syncwarp();
-        if (lane == 0) tc::mbar_arrive(bar(kVFull + st));
+        if (lane == 0) tc::mbar_arrive(bar(kVFull + vb));
       }
     });
   } else if (warp < kParamWarp) {
     // ================================================================ keys: 64 tokens a warp
-    const int q = warp - kKeyWarp, l8 = lane >> 3, tk = lane & 7;
-    constexpr int kLoads = D / 16;               // 16-byte loads per lane and tile
+    // A block of 64 elements is two 16-byte pieces a token: load i holds piece l8 & 1 of token 16 i + tok0.
+    const int q = warp - kKeyWarp, l8 = lane >> 3, tk = lane & 7, tok0 = 8 * (l8 >> 1) + tk;
     const int page_mask = (1 << p.c.page_log2) - 1;
-    // load i: piece e % (D / 32) of token 8 (e / (D / 32)) + lane % 8 of the warp's 64, e = 4 i + lane / 8
-    constexpr int kPer = D == 256 ? 2 : 1;       // loads that stay with the same tokens
-    const int tok0 = (D == 64 ? 8 * (l8 >> 1) : 0) + tk, piece0 = D == 64 ? (l8 & 1) : l8;
-    constexpr int kTokStep = D == 64 ? 16 : 8;   // tokens between the loads (between pairs of loads for 256)
     uint32_t put[4];                             // word j of the piece
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int ch = piece0 * 4 + j;
-      put[j] = sm + S::kK + (ch >> 3) * (kTile * 128) + (64 * q + tok0) * 128 + (((ch & 7) ^ tk) << 4);
-    }
+    for (int j = 0; j < 4; ++j) put[j] = sm + S::kK + (64 * q + tok0) * 128 + ((((l8 & 1) * 4 + j) ^ tk) << 4);
     items([&](const Item& it) {
-      uint4 kc[kLoads];
-      int page[4], first = 0;
-      auto locate = [&](int t) {
-        const uint32_t m = it.n0 + uint32_t(t);
-        const int ps = int(m % kParamStages);
-        first = it.span.id(w.i0 + t) * kTile + 64 * q;
-        wait(kPrmFull + ps, (m / kParamStages) & 1u, tc::kStatusWaitFull);
+      const int units = it.count * kKB;          // blocks of the item's tiles
+      uint4 kc[2][4];                            // the next two blocks
+      const uint8_t* from[4];
+      bool ok[4];
+      auto load = [&](uint4 (&to)[4], int u) {
+        if (u % kKB == 0) {
+          const uint32_t m = it.n0 + uint32_t(u / kKB);
+          const int ps = int(m % kParamStages), first = it.span.id(w.i0 + u / kKB) * kTile + 64 * q + tok0;
+          wait(kPrmFull + ps, (m / kParamStages) & 1u, tc::kStatusWaitFull);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) page[j] = info[ps].page[4 * q + j];
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(bar(kPrmEmpty + ps));
+          for (int i = 0; i < 4; ++i) {
+            const int page = info[ps].page[4 * q + i];
+            ok[i] = unsigned(page) < unsigned(p.c.n_pages);      // after a wait that gave up it may be anything
+            from[i] = p.c.k + cache_codes_at(ok[i] ? page : 0, w.h, p.c.heads, p.c.page_log2, D) +
+                      key_word_at((first + 16 * i) & page_mask, 4 * (l8 & 1), D);
+          }
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(bar(kPrmEmpty + ps));
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          to[i] = ok[i] ? __ldg(reinterpret_cast<const uint4*>(from[i] + 32 * (u % kKB))) : make_uint4(0, 0, 0, 0);
       };
-      auto load = [&](int i) {
-        const int step = (i / kPer) * kTokStep, pg = page[step >> 4];      // tok0 < 16: the same 16 tokens
-        const uint8_t* at = p.c.k + cache_codes_at(pg, w.h, p.c.heads, p.c.page_log2, D) +
-                            key_word_at((first + tok0 + step) & page_mask, (piece0 + (kPer == 2 ? 4 * (i & 1) : 0)) * 4, D);
-        kc[i] = unsigned(pg) < unsigned(p.c.n_pages) ? __ldg(reinterpret_cast<const uint4*>(at)) : make_uint4(0, 0, 0, 0);
-      };
-      locate(0);
+      auto unpack = [&](const uint4 (&c)[4], int u) {
+        const uint32_t m = it.n0 + uint32_t(u / kKB), use = m / S::kStages;
+        const int st = int(m % S::kStages), kb = u % kKB, kbar = st * kKB + kb;
+        if (use > 0) wait(kKEmpty + kbar, (use - 1) & 1u, tc::kStatusWaitEmpty);
+        const uint32_t at = uint32_t(st * S::kOperand + kb * (kTile * 128));
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) load(i);
-      for (int t = 0; t < it.count; ++t) {
-        const uint32_t m = it.n0 + uint32_t(t), use = m / S::kStages;
-        const int st = int(m % S::kStages);
-        const bool more = t + 1 < it.count;
-        if (more) locate(t + 1);
-        if (use > 0) wait(kKEmpty + st, (use - 1) & 1u, tc::kStatusWaitEmpty);
-        uint32_t to[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) to[j] = put[j] + st * S::kOperand;
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-          const uint32_t u[4] = {kc[i].x, kc[i].y, kc[i].z, kc[i].w};
-          if (more) load(i);                     // the next tile's, into the registers just read
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t v[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const uint32_t x = u[j], y = x >> 8;
-            sts128(to[j] + (i / kPer) * (kTokStep * 128) + (kPer == 2 ? (i & 1) * (2 * kTile * 128) : 0), x & 0x000F000Fu,
-                   x & 0x00F000F0u, y & 0x000F000Fu, y & 0x00F000F0u);
+            const uint32_t x = v[j], y = x >> 8;
+            sts128(put[j] + at + i * 2048, x & 0x000F000Fu, x & 0x00F000F0u, y & 0x000F000Fu, y & 0x00F000F0u);
           }
         }
         tc::fence_proxy_async();
         __syncwarp();
-        if (lane == 0) tc::mbar_arrive(bar(kKFull + st));
+        if (lane == 0) tc::mbar_arrive(bar(kKFull + kbar));
+      };
+      load(kc[0], 0);
+      if (units > 1) load(kc[1], 1);
+#pragma unroll 1
+      for (int u = 0; u < units; u += 2) {
+        unpack(kc[0], u);
+        if (u + 2 < units) load(kc[0], u + 2);
+        if (u + 1 < units) unpack(kc[1], u + 1);
+        if (u + 3 < units) load(kc[1], u + 3);
       }
     });
   } else if (warp == kParamWarp) {
@@ -755,7 +762,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
         sig = fmaxf(sig, pow2_above(top));
         const float inv = 1.f / sig;
         if (m >= kParamStages) wait(kPrmEmpty + ps, (m / kParamStages - 1) & 1u, tc::kStatusWaitEmpty);
-        float* prm = reinterpret_cast<float*>(raw_sm + (sm - tc::smem_addr(raw_sm)) + S::kParam + ps * S::kParamBytes);
+        float* prm = reinterpret_cast<float*>(raw_sm + base_off + S::kParam + ps * S::kParamBytes);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int c = 32 * j + lane, at = (c >> 1) * 4 + (c & 1);
@@ -782,16 +789,18 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
         const uint32_t idesc_s = tc::instr_desc(0, 128, kTile), idesc_o = tc::instr_desc(0, 128, D);
         auto scores = [&](uint32_t m) {
           const int st = int(m % S::kStages);
-          wait(kKFull + st, (m / S::kStages) & 1u, tc::kStatusWaitFull);
           // S's buffer held P of the tile before last: its product has to be through
           if (m >= 2 + it.n0) wait_pv(m - 2);
-          tc::fence_after_sync();
           const uint64_t a = tmpl | ((sm + S::kQ) >> 4), b = tmpl | ((sm + S::kK + st * S::kOperand) >> 4);
+#pragma unroll 1
+          for (int kb = 0; kb < kKB; ++kb) {
+            wait(kKFull + st * kKB + kb, (m / S::kStages) & 1u, tc::kStatusWaitFull);
+            tc::fence_after_sync();
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k)
-            mma_ss(tmem + 256 + 128 * (m & 1), a + (k >> 2) * 1024 + (k & 3) * 2, b + (k >> 2) * 1024 + (k & 3) * 2, idesc_s,
-                   k > 0);
-          tc::mma_commit(bar(kKEmpty + st));
+            for (int k = 0; k < 4; ++k)
+              mma_ss(tmem + 256 + 128 * (m & 1), a + kb * 1024 + k * 2, b + kb * 1024 + k * 2, idesc_s, kb > 0 || k > 0);
+            tc::mma_commit(bar(kKEmpty + st * kKB + kb));
+          }
           tc::mma_commit(bar(kSFull + int(m & 1)));
         };
         scores(it.n0);
@@ -799,15 +808,16 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
           const uint32_t m = it.n0 + uint32_t(t);
           if (t + 1 < it.count) scores(m + 1);
           const int st = int(m % S::kStages);
-          wait(kVFull + st, (m / S::kStages) & 1u, tc::kStatusWaitFull);
           wait(kPFull + int(m & 1), (m >> 1) & 1u, tc::kStatusWaitFull);
-          tc::fence_after_sync();
           const uint64_t b = tmpl | ((sm + S::kV + st * S::kOperand) >> 4);
-#pragma unroll
-          for (int k = 0; k < 2; ++k)
+#pragma unroll 1
+          for (int k = 0; k < 2; ++k) {
+            wait(kVFull + 2 * st + k, (m / S::kStages) & 1u, tc::kStatusWaitFull);
+            tc::fence_after_sync();
             tc::mma_ts_kblock(tmem, tmem + 256 + 128 * (m & 1) + 64 * k, uint32_t(b) + k * (D * 8), uint32_t(b >> 32), idesc_o,
                               t > 0 || k > 0);
-          tc::mma_commit(bar(kVEmpty + st));
+            tc::mma_commit(bar(kVEmpty + 2 * st + k));
+          }
           tc::mma_commit(bar(kPvDone + int(m & 1)));
         }
       }
