@@ -59,6 +59,7 @@ __device__ __forceinline__ Request request_of(const AttendParams& p, int b) {
 template <int kTile>
 struct Span {
   int sink_tiles, main0, tiles;
+  __device__ Span() {}
   __device__ __forceinline__ Span(int first, int last, int len, int window, int sinks) {
     const int hi = min(len, last + 1);                       // tokens below hi
     const int lo = window ? max(0, first - window + 1) : 0;

@@ -4,14 +4,14 @@
 // tokens are cut into tiles of 128. All items' tiles form one line that is dealt to the blocks (one per SM) in
 // equal contiguous shares; items that span blocks are joined by a second kernel in the order of the blocks.
 // Per tile, in the roles of one block:
-//   warp 14     parameters: pages, and what the tokens' pairs say (one tile ahead of everybody else).
-//   warps 12-13 keys: codes from global memory (fetched one tile ahead) into fp16 operands in shared memory, 128-byte
+//   warp 20     parameters: pages, and what the tokens' pairs say (one tile ahead of everybody else).
+//   warps 16-19 keys: codes from global memory (fetched one tile ahead) into fp16 operands in shared memory, 128-byte
 //               swizzle, [token, dim] rows.
-//   warps 8-11  values: transposed, [dim, token] rows. A 16-byte piece holds four tokens' words side by side, two byte
+//   warps 8-15  values: transposed, [dim, token] rows. A 16-byte piece holds four tokens' words side by side, two byte
 //               permutes make pairs of tokens. The words are rotated by the lane's group first, so that the
 //               eight rows a store hits differ in their swizzle.
-//   warp 15     one thread issues S = Q K^T (128 x 128, fp32 in tensor memory, two buffers) and O += P V (128 x D).
-//   warps 0-7   softmax, two threads a row (64 tokens each): scores from tensor memory, the token's two parameters
+//   warp 21     one thread issues S = Q K^T (128 x 128, fp32 in tensor memory, two buffers) and O += P V (128 x D).
+//   warps 0-7   softmax, two warps for 32 rows (64 tokens each): scores from tensor memory, the token's two parameters
 //               applied as packed pairs, P back into the place of S as fp16 (the A operand of the second product).
 //               The running maximum may lag by 2^8 before O is rescaled, which then waits for the products in flight.
 // Tensor memory: O in columns 0 .. D - 1, S in 256 .. 383 and 384 .. 511.
@@ -23,8 +23,11 @@ namespace {
 
 __device__ int g_tiles_status = 0;
 constexpr int kRows = 128, kTile = 128;
-constexpr int kThreads = 512, kWarps = kThreads / 32;
-constexpr int kValueWarp = 8, kKeyWarp = 12, kParamWarp = 14, kProductWarp = 15;
+constexpr int kThreads = 768, kWarps = kThreads / 32;
+constexpr int kValueWarp = 8, kKeyWarp = 16, kParamWarp = 20, kProductWarp = 21;
+// Registers per thread of the softmax warpgroups (two) and of the others (four): together 6 x 80, the launch's. The
+// unpacking warps are many because one warp issues an instruction in six to seven cycles at best here.
+constexpr int kSoftmaxRegs = 128, kOtherRegs = 56;
 constexpr int kParamStages = 4;
 constexpr float kLazy = 8.f;
 constexpr float kMinStep = 7.888609e-31f;   // 2^-100
@@ -106,8 +109,30 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-__device__ __forceinline__ void tmem_st8(uint32_t t, const uint32_t (&v)[8]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(t), "r"(v[0]), "r"(v[1]),
+// 16 rows x 16 columns: register 4 i + 2 h + e of lane (g, t) is (row g + 8 h, column 8 i + 2 t + e).
+__device__ __forceinline__ void tmem_ld_rows16(uint32_t a, uint32_t (&v)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+               : "r"(a)
+               : "memory");
+}
+// The same over 32 columns.
+__device__ __forceinline__ void tmem_ld_rows16(uint32_t a, uint32_t (&v)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+                 "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+               : "r"(a)
+               : "memory");
+}
+// 16 rows x 8 columns: register 2 i + h is (row g + 8 h, column 4 i + t).
+__device__ __forceinline__ void tmem_st_rows16(uint32_t a, const uint32_t (&v)[4]) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x2.b32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3])
+               : "memory");
+}
+// The same over 16 columns.
+__device__ __forceinline__ void tmem_st_rows16(uint32_t a, const uint32_t (&v)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(a), "r"(v[0]), "r"(v[1]),
                "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
                : "memory");
 }
@@ -118,16 +143,47 @@ __device__ __forceinline__ void tmem_st16(uint32_t t, const uint32_t (&v)[16]) {
       "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
 }
-// D[d] (+)= A[desc a] B[desc b], one K = 16 step; one thread issues.
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// The four K = 16 steps of a block of 64: D[d] (+)= A[a + 32 j bytes] B[b + 32 j bytes], both in shared memory; a and b
+// are the low words of the descriptors. One thread issues.
+__device__ __forceinline__ void mma_ss_block(uint32_t d, uint32_t a, uint32_t b, uint32_t hi, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
-      "r"(accumulate), "r"(0u)
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 a0, a1, a2, a3, b0, b1, b2, b3;\n\t.reg .b32 x1, x2, x3, y1, y2, y3;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\tsetp.eq.b32 q, %6, %6;\n\t"
+      "add.u32 x1, %1, 2;\n\tadd.u32 x2, %1, 4;\n\tadd.u32 x3, %1, 6;\n\t"
+      "add.u32 y1, %2, 2;\n\tadd.u32 y2, %2, 4;\n\tadd.u32 y3, %2, 6;\n\t"
+      "mov.b64 a0, {%1, %3};\n\tmov.b64 a1, {x1, %3};\n\tmov.b64 a2, {x2, %3};\n\tmov.b64 a3, {x3, %3};\n\t"
+      "mov.b64 b0, {%2, %3};\n\tmov.b64 b1, {y1, %3};\n\tmov.b64 b2, {y2, %3};\n\tmov.b64 b3, {y3, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a0, b0, %4, {%6, %6, %6, %6}, p;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %4, {%6, %6, %6, %6}, q;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %4, {%6, %6, %6, %6}, q;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %4, {%6, %6, %6, %6}, q;\n\t}"
+      :
+      : "r"(d), "r"(a), "r"(b), "r"(hi), "r"(idesc), "r"(accumulate), "r"(0u)
       : "memory");
 }
 
 __device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
+__device__ __forceinline__ bool pair_any(int id, bool x) {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %2, 0;\n\tbar.red.or.pred q, %1, 64, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
+               : "=r"(r)
+               : "r"(id), "r"(x ? 1 : 0)
+               : "memory");
+  return r != 0;
+}
+// tc::mbar_wait without its call: a kernel that moves registers between its warps has none.
+__device__ __forceinline__ void bounded_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int why, long long limit) {
+  if (tc::mbar_test(bar, parity)) return;
+  const long long t0 = clock64();
+  while (!tc::mbar_try(bar, parity)) {
+    if (*abort_flag) return;
+    if (clock64() - t0 > limit) {
+      *abort_flag = 1;
+      atomicCAS(&g_tiles_status, 0, why);
+      return;
+    }
+  }
+}
 
 // ---- the line of tiles ---------------------------------------------------------------------------------------
 __device__ __forceinline__ Request tiles_request(const AttendParams& p, int b) {
@@ -150,23 +206,46 @@ __device__ __forceinline__ long long head_tiles(const AttendParams& p, const Req
   return sum;
 }
 
-// A part of an item: tiles [i0, i1) of row tile rt of head h of request b.
+// The block's present part of an item: tiles [i0, i1) of row tile rt of head h of request b. Kept in shared memory: in
+// registers it cost every role two dozen, and what spills goes past an L1 that shared memory has left little of.
 struct Work {
-  int b, h;
-  long long rt;
-  int i0, i1, tiles;
   Request rq;
-  long long item_at;           // tiles of the line before the item
-};
-
-// What the roles need of it.
-struct Item {
   Span<kTile> span;
-  long long r0;
+  long long rt, r0, item_at;   // item_at: tiles of the line before the item
+  int b, h, i0, i1;
   int n_rows, base, first_pos, last_pos;
-  uint32_t n0;                 // tiles of this block before the item's
-  int count;
+  uint32_t n0;                 // tiles of this block before this part's
+  int count, more;
+  __device__ Work() {}
 };
+// The part that starts at tile `cur` of the line; b, h, rt, rq and item_at say where that is.
+__device__ __forceinline__ void open_part(const AttendParams& p, Work* w, long long cur, long long stop) {
+  w->span = span_of(p, w->rq, w->rt * kRows);
+  w->i0 = int(cur - w->item_at), w->i1 = int(min((long long)w->span.tiles, stop - w->item_at));
+  w->count = w->i1 - w->i0;
+  w->r0 = w->rt * kRows;
+  const long long rows = (long long)w->rq.rows * p.G;
+  w->n_rows = int(min((long long)kRows, rows - w->r0));
+  w->base = w->rq.len - w->rq.rows;
+  w->first_pos = w->base + int(w->r0 / p.G), w->last_pos = w->base + int((w->r0 + w->n_rows - 1) / p.G);
+  w->more = w->item_at + w->i1 < stop;
+}
+__device__ __forceinline__ void next_part(const AttendParams& p, Work* w, long long stop) {
+  const long long cur = w->item_at + w->i1;
+  w->n0 += uint32_t(w->count);
+  w->item_at += w->span.tiles;
+  if ((w->rt + 1) * kRows < (long long)w->rq.rows * p.G) {
+    ++w->rt;
+  } else {
+    w->rt = 0;
+    if (++w->h == p.c.heads) {
+      w->h = 0;
+      do w->rq = tiles_request(p, ++w->b);
+      while (w->rq.rows == 0);
+    }
+  }
+  open_part(p, w, cur, stop);
+}
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_constant__ AttendParams p) {
@@ -177,9 +256,12 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
   __shared__ int abort_word;
   __shared__ float2 row_k[kRows];              // factor of the scores, sum of the scaled row
   __shared__ TileInfo info[kParamStages];
-  __shared__ float half_top[2][2][kRows];      // [tile & 1][half][row]
-  __shared__ float2 half_sum[kRows];
+  __shared__ float half_top[2][kRows];         // [half][row]
+  __shared__ float row_f[2][kRows];            // [half][row]: a factor on its way to another thread
+  __shared__ float2 half_sum[2][kRows];
+  __shared__ float row_m[kRows];
   __shared__ long long scan[kWarps];
+  __shared__ Work w;
   __shared__ long long first_at;
   __shared__ int first_b;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -231,11 +313,11 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
   }
   if (warp == kProductWarp) tc::tmem_alloc(tc::smem_addr(&tmem_base), 512);
   if (tid == 0) {
-    for (int i = 0; i < kKBars; ++i) tc::mbar_init(bar(kKFull + i), 2), tc::mbar_init(bar(kKEmpty + i), 1);
-    for (int i = 0; i < kVBars; ++i) tc::mbar_init(bar(kVFull + i), 2), tc::mbar_init(bar(kVEmpty + i), 1);
+    for (int i = 0; i < kKBars; ++i) tc::mbar_init(bar(kKFull + i), 4), tc::mbar_init(bar(kKEmpty + i), 1);
+    for (int i = 0; i < kVBars; ++i) tc::mbar_init(bar(kVFull + i), 4), tc::mbar_init(bar(kVEmpty + i), 1);
     for (int i = 0; i < 2; ++i)
       tc::mbar_init(bar(kSFull + i), 1), tc::mbar_init(bar(kPFull + i), 8), tc::mbar_init(bar(kPvDone + i), 1);
-    for (int i = 0; i < kParamStages; ++i) tc::mbar_init(bar(kPrmFull + i), 1), tc::mbar_init(bar(kPrmEmpty + i), 14);
+    for (int i = 0; i < kParamStages; ++i) tc::mbar_init(bar(kPrmFull + i), 1), tc::mbar_init(bar(kPrmEmpty + i), 20);
     tc::mbar_init_fence();
   }
   tc::fence_before_sync();
@@ -243,7 +325,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
   tc::fence_after_sync();
   const uint32_t tmem = tmem_base;
   auto wait = [&](int i, uint32_t parity, int why) {
-    tc::mbar_wait(bar(i), parity, abort_flag, &g_tiles_status, why, p.wait_cycles);
+    bounded_wait(bar(i), parity, abort_flag, why, p.wait_cycles);
   };
 
   // A wait names a phase by its parity alone: whoever waits must know that the phase before is complete and that
@@ -251,19 +333,18 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
   // there, tile m + 2 waits for P of m.
   auto wait_pv = [&](uint32_t m) { wait(kPvDone + int(m & 1), (m >> 1) & 1u, tc::kStatusWaitDone); };
 
-  // the first item (every warp finds it by itself)
-  Work w;
-  w.b = first_b;
-  {
-    w.rq = tiles_request(p, w.b);
-    const long long per_head = head_tiles(p, w.rq, lane);
+  // ---- the first part: warp 0 looks for the row tile
+  if (warp == 0) {
+    const int b = first_b;
+    const Request rq = tiles_request(p, b);
+    const long long per_head = head_tiles(p, rq, lane);
     long long off = begin - first_at;
-    w.h = int(off / per_head);
-    off -= w.h * per_head;
-    const long long n = ((long long)w.rq.rows * p.G + kRows - 1) / kRows;
-    w.rt = 0;
+    const int h = int(off / per_head);
+    off -= h * per_head;
+    const long long n = ((long long)rq.rows * p.G + kRows - 1) / kRows;
+    long long rt = 0;
     for (long long c0 = 0; c0 < n; c0 += 32) {
-      const long long tiles = c0 + lane < n ? span_of(p, w.rq, (c0 + lane) * kRows).tiles : 0;
+      const long long tiles = c0 + lane < n ? span_of(p, rq, (c0 + lane) * kRows).tiles : 0;
       long long inc = tiles;
       for (int o = 1; o < 32; o <<= 1) {
         const long long v = __shfl_up_sync(0xffffffffu, inc, o);
@@ -272,125 +353,121 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
       const unsigned hit = __ballot_sync(0xffffffffu, off < inc);
       if (hit) {
         const int l = __ffs(int(hit)) - 1;
-        w.rt = c0 + l;
+        rt = c0 + l;
         off -= __shfl_sync(0xffffffffu, inc - tiles, l);
         break;
       }
       off -= __shfl_sync(0xffffffffu, inc, 31);
     }
-    w.item_at = begin - off;
+    if (lane == 0) {
+      w.b = b, w.h = h, w.rt = rt, w.rq = rq, w.item_at = begin - off, w.n0 = 0;
+      open_part(p, &w, begin, stop);
+    }
   }
+  __syncthreads();
 
-  uint32_t n = 0;                              // tiles of this block so far
-  // Every role walks the block's items: the rows' operand is made by all warps, then `body` does the role's
-  // part of the item's tiles.
+  // Every role walks the block's parts: the rows' operand is made by all warps, then `body` does the role's part of
+  // the tiles.
   auto items = [&](auto&& body) {
-    long long cur = begin;
-    while (cur < stop) {
-      const Span<kTile> span = span_of(p, w.rq, w.rt * kRows);
-      w.tiles = span.tiles;
-      w.i0 = int(cur - w.item_at), w.i1 = int(min((long long)w.tiles, stop - w.item_at));
-      const long long r0 = w.rt * kRows, rows = (long long)w.rq.rows * p.G;
-      const int n_rows = int(min((long long)kRows, rows - r0)), base = w.rq.len - w.rq.rows;
-      const int first_pos = base + int(r0 / p.G), last_pos = base + int((r0 + n_rows - 1) / p.G);
-
-      // ---- the item's rows: fp16, scaled, in the order of the codes' pairs
-      for (int r = warp; r < kRows; r += kWarps) {
-        constexpr int kChunks = D / 8;           // 16-byte chunks of eight elements
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (r < n_rows && lane < kChunks) {
-          const long long tok = w.rq.row0 + (r0 + r) / p.G;
-          x = __ldg(reinterpret_cast<const uint4*>(p.q + tok * p.q_token +
-                                                   (long long)(w.h * p.G + int((r0 + r) % p.G)) * p.q_head) + lane);
-        }
-        const uint32_t u[4] = {x.x, x.y, x.z, x.w};
-        float v[8], top = 0.f, sum = 0.f;
+    while (true) {
+      // the rows: fp16, scaled, in the order of the codes' pairs; a warp's rows are all under way at once
+      {
+        constexpr int kChunks = D / 8, kMine = (kRows + kWarps - 1) / kWarps;       // 16-byte chunks of eight elements; rows of a warp
+        uint4 x[kMine];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          v[e] = DType<T>::to_float(uint16_t(u[e >> 1] >> (16 * (e & 1))));
-          top = fmaxf(top, fabsf(v[e])), sum += v[e];
-        }
-        for (int o = 16; o; o >>= 1) {
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-          sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        }
-        const int ex = int(__float_as_uint(top) >> 23);
-        const int fe = ex == 255 || top == 0.f ? 127 : max(24, min(254, 127 + 13 + 127 - ex));   // 2^24 / f stays finite
-        const float f = __uint_as_float(uint32_t(fe) << 23), fs = p.scale < 0.f ? -f : f;
-        if (lane < kChunks) {
-          uint32_t o[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float g = e & 1 ? fs * 0.0625f : fs;
-            o[e] = half2_of(make_float2(v[e] * g, v[e + 4] * g));
+        for (int i = 0; i < kMine; ++i) {
+          const int r = warp + i * kWarps;
+          x[i] = make_uint4(0, 0, 0, 0);
+          if (r < w.n_rows && lane < kChunks) {
+            const long long tok = w.rq.row0 + (w.r0 + r) / p.G;
+            x[i] = __ldg(reinterpret_cast<const uint4*>(p.q + tok * p.q_token +
+                                                        (long long)(w.h * p.G + int((w.r0 + r) % p.G)) * p.q_head) + lane);
           }
-          sts128(sm + S::kQ + (lane >> 3) * (kRows * 128) + r * 128 + (((lane & 7) ^ (r & 7)) << 4), o[0], o[1], o[2], o[3]);
         }
-        if (lane == 0) row_k[r] = make_float2(fmaxf(fabsf(p.scale) * (16777216.f / f), 1.17549435e-38f), sum * fs * 5.9604645e-8f);
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+          const int r = warp + i * kWarps;
+          if (r >= kRows) break;
+          const uint32_t u[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+          float v[8], top = 0.f, sum = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            v[e] = DType<T>::to_float(uint16_t(u[e >> 1] >> (16 * (e & 1))));
+            top = fmaxf(top, fabsf(v[e])), sum += v[e];
+          }
+          for (int o = 16; o; o >>= 1) {
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            sum += __shfl_xor_sync(0xffffffffu, sum, o);
+          }
+          const int ex = int(__float_as_uint(top) >> 23);
+          const int fe = ex == 255 || top == 0.f ? 127 : max(24, min(254, 127 + 13 + 127 - ex));   // 2^24 / f stays finite
+          const float f = __uint_as_float(uint32_t(fe) << 23), fs = p.scale < 0.f ? -f : f;
+          if (lane < kChunks) {
+            uint32_t o[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float g = e & 1 ? fs * 0.0625f : fs;
+              o[e] = half2_of(make_float2(v[e] * g, v[e + 4] * g));
+            }
+            sts128(sm + S::kQ + (lane >> 3) * (kRows * 128) + r * 128 + (((lane & 7) ^ (r & 7)) << 4), o[0], o[1], o[2], o[3]);
+          }
+          if (lane == 0)
+            row_k[r] = make_float2(fmaxf(fabsf(p.scale) * (16777216.f / f), 1.17549435e-38f), sum * fs * 5.9604645e-8f);
+        }
       }
       tc::fence_proxy_async();
       __syncthreads();
-
-      const Item item{span, r0, n_rows, base, first_pos, last_pos, n, w.i1 - w.i0};
-      body(item);
-      n += uint32_t(item.count);
-      cur = w.item_at + w.i1;
-      // ---- on to the next item: the rows' operand and O are free once every role is through
-      if (cur < stop) {
-        w.item_at += w.tiles;
-        if ((w.rt + 1) * kRows < rows) {
-          ++w.rt;
-        } else {
-          w.rt = 0;
-          if (++w.h == p.c.heads) {
-            w.h = 0;
-            do w.rq = tiles_request(p, ++w.b);
-            while (w.rq.rows == 0);
-          }
-        }
-      }
+      body();
+      const bool more = w.more != 0;
+      // on to the next part: the rows' operand and O are free once every role is through
+      __syncthreads();
+      if (!more) break;
+      if (tid == 0) next_part(p, &w, stop);
       __syncthreads();
       tc::fence_after_sync();
     }
   };
 
   if (warp < kValueWarp) {
-    // ================================================================ softmax: two threads a row
-    const int r = tid & 127, half = warp >> 2;
-    const uint32_t lane_base = tmem + (uint32_t((warp & 3) * 32) << 16);
-    items([&](const Item& it) {
-      const float2 rk = row_k[r];
-      const float2 qf = make_float2(rk.x, rk.x), qs = make_float2(rk.y, rk.y);
-      const int pos = r < it.n_rows ? it.base + int((it.r0 + r) / p.G) : -1;
-      float m_run = -INFINITY, sig_run = 0.f;
-      float2 l2 = make_float2(0.f, 0.f), pm2 = make_float2(0.f, 0.f);
-      for (int t = 0; t < it.count; ++t) {
-        const uint32_t m = it.n0 + uint32_t(t);
-        const int ps = int(m % kParamStages), first = it.span.id(w.i0 + t) * kTile + 64 * half;
+    // ================================================================ softmax
+    // A warp takes 64 of the tile's tokens for 32 rows. A lane (g, t) has the columns 8 i + 2 t, + 1 of the rows g + 8 k,
+    // k = 0 .. 3: a token's parameters, fetched once, serve four rows.
+    const int half = warp >> 2, row0 = 32 * (warp & 3), g = lane >> 2, t4 = lane & 3, pair_bar = 1 + (warp & 3);
+    const uint32_t lane_base = tmem + (uint32_t(row0) << 16);
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    constexpr uint32_t kLower = 16u << 16;       // rows 16 .. 31 of the warp
+    items([&]() {
+      float qf[4], qs[4], m_run[4];
+      float2 l2[4], pm2[4];
+      int pos[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int r = row0 + g + 8 * k;
+        qf[k] = row_k[r].x, qs[k] = row_k[r].y;
+        pos[k] = r < w.n_rows ? w.base + int((w.r0 + r) / p.G) : -1;
+        m_run[k] = -INFINITY;
+        l2[k] = pm2[k] = make_float2(0.f, 0.f);
+      }
+      float sig_run = 0.f;
+      for (int t = 0; t < w.count; ++t) {
+        const uint32_t m = w.n0 + uint32_t(t);
+        const int ps = int(m % kParamStages), first = w.span.id(w.i0 + t) * kTile + 64 * half;
         wait(kPrmFull + ps, (m / kParamStages) & 1u, tc::kStatusWaitFull);
         wait(kSFull + int(m & 1), (m >> 1) & 1u, tc::kStatusWaitDone);
         tc::fence_after_sync();
-        const uint32_t s_at = lane_base + 256 + 128 * (m & 1);
-        const float4* prm = reinterpret_cast<const float4*>(raw_sm + base_off + S::kParam + ps * S::kParamBytes) + 32 * half;
-        const uint32_t mine = s_at + 64 * half;
+        const uint32_t mine = lane_base + 256 + 128 * (m & 1) + 64 * half;
+        const float4* prm = reinterpret_cast<const float4*>(raw_sm + base_off + S::kParam + ps * S::kParamBytes) + 32 * half + t4;
         const bool whole = info[ps].whole != 0;
-        uint32_t mask[2] = {0xffffffffu, 0xffffffffu};
-        if (!whole) {
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            auto below = [](int k) { return k <= 0 ? 0u : k >= 32 ? 0xffffffffu : (1u << k) - 1u; };
-            const int f = first + 32 * c;
-            mask[c] = below(pos + 1 - f) & info[ps].valid[2 * half + c];
-            if (p.window) mask[c] &= ~below(pos - p.window + 1 - f) | below(p.sinks - f);
-          }
-        }
-        auto score = [&](float4 k, uint32_t s0, uint32_t s1) {
-          return fma2(make_float2(k.x, k.y), make_float2(__uint_as_float(s0), __uint_as_float(s1)),
-                      mul2(make_float2(k.z, k.w), qs));
-        };
         const float sig_new = info[ps].sig;
-        // O times `ab`, each of the two threads half of the row; the products in flight have to be through
-        auto rescale = [&](float ab) {
+        auto pair = [](float x) { return make_float2(x, x); };
+        // O's rows times ab: the two warps of a row do half of its columns each; the products in flight have to be through
+        auto rescale = [&](const float (&ab)[4]) {
+          if (t4 == 0) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) row_f[half][row0 + g + 8 * k] = ab[k];
+          }
+          __syncwarp();
+          const float f = row_f[half][row0 + lane];
           wait_pv(m - 1);
           tc::fence_after_sync();
 #pragma unroll 1
@@ -400,96 +477,140 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
             tc::tmem_ld_32x32b_x16(at, o);
             tc::wait_ld();
 #pragma unroll
-            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * ab);
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
             tmem_st16(at, o);
           }
           tc::wait_st();
         };
-        bool done = false;
-        if (whole && t > 0 && __all_sync(0xffffffffu, m_run > -INFINITY || r >= it.n_rows)) {
-          // One pass under the maximum so far, P kept in registers: it holds unless a score is more than 2^8 above.
-          const float2 off2 = make_float2(-m_run, -m_run);
-          const float2 l_old = l2, pm_old = pm2;
-          float top = -INFINITY;
-          uint32_t pk[32];
+        // Two passes over 16 tokens at a time, the scores fetched from tensor memory in each: short loops. The
+        // scheduler's instruction cache holds about 600 instructions; beyond it a warp gets one in three to six cycles.
+        uint32_t s[2][8];
+        auto fetch = [&](int c) {
+          tmem_ld_rows16(mine + 16 * c, s[0]);
+          tmem_ld_rows16(mine + kLower + 16 * c, s[1]);
+          tc::wait_ld();
+        };
+        auto score_of = [&](float4 kk, uint32_t s0, uint32_t s1, int k) {      // up to the row's factor
+          return fma2(make_float2(kk.x, kk.y), make_float2(__uint_as_float(s0), __uint_as_float(s1)),
+                      mul2(make_float2(kk.z, kk.w), pair(qs[k])));
+        };
+        auto score = [&](float4 kk, int i, int k) {
+          return score_of(kk, s[k >> 1][4 * i + 2 * (k & 1)], s[k >> 1][4 * i + 2 * (k & 1) + 1], k);
+        };
+        auto seen = [&](int c, int i, int k, int e) {
+          const int col = 16 * c + 8 * i + 2 * t4 + e, j = first + col;
+          return ((info[ps].valid[2 * half + (col >> 5)] >> (col & 31)) & 1u) && j <= pos[k] &&
+                 (p.window == 0 || j > pos[k] - p.window || j < p.sinks);
+        };
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        if (whole) {
+#pragma unroll 1
+          for (int c = 0; c < 2; ++c) {
+            uint32_t z[2][16];
+            tmem_ld_rows16(mine + 32 * c, z[0]);
+            tmem_ld_rows16(mine + kLower + 32 * c, z[1]);
+            float4 kk[4];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t s[16];
-            tc::tmem_ld_32x32b_x16(mine + 16 * c, s);
+            for (int i = 0; i < 4; ++i) kk[i] = prm[16 * c + 4 * i];
             tc::wait_ld();
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float2 x = fma2(score(prm[8 * c + e], s[2 * e], s[2 * e + 1]), qf, off2);
-              top = max3(top, x.x, x.y);
-              const float4 v = prm[64 + 8 * c + e];
-              const float2 w2 = make_float2(ex2(x.x), ex2(x.y));
-              l2 = add2(l2, w2);
-              pm2 = fma2(w2, make_float2(v.z, v.w), pm2);
-              pk[8 * c + e] = half2_of(mul2(w2, make_float2(v.x, v.y)));
-            }
-          }
-          half_top[m & 1][half][r] = top;
-          pair_sync(1 + (warp & 3));
-          top = fmaxf(top, half_top[m & 1][half ^ 1][r]);
-          done = !__any_sync(0xffffffffu, top > kLazy && r < it.n_rows);
-          if (done) {
-            if (sig_new != sig_run) rescale(sig_run / sig_new), sig_run = sig_new;
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int c = 0; c < 2; ++c) tmem_st16(mine + 16 * c, reinterpret_cast<const uint32_t(&)[16]>(pk[16 * c]));
-          } else {
-            l2 = l_old, pm2 = pm_old;
-            pair_sync(1 + (warp & 3));           // half_top is written again
+              for (int k = 0; k < 4; ++k) {
+                const float2 y = score_of(kk[i], z[k >> 1][4 * i + 2 * (k & 1)], z[k >> 1][4 * i + 2 * (k & 1) + 1], k);
+                top[k] = max3(top[k], y.x, y.y);
+              }
+          }
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            fetch(c);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float4 kk = prm[8 * c + 4 * i];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const float2 y = score(kk, i, k);
+                if (seen(c, i, k, 0)) top[k] = fmaxf(top[k], y.x);
+                if (seen(c, i, k, 1)) top[k] = fmaxf(top[k], y.y);
+              }
+            }
           }
         }
-        if (!done) {
-          // Two passes over 16 tokens at a time, the scores read from tensor memory in each.
-          float top = -INFINITY;
+        // ---- the maximum so far serves unless a score of the tile is more than 2^8 above it
+        bool grow = sig_new != sig_run;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) grow = grow || top[k] * qf[k] > m_run[k] + kLazy;
+        if (pair_any(pair_bar, grow)) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 1));
+            top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 2));
+            if (t4 == 0) half_top[half][row0 + g + 8 * k] = top[k];
+          }
+          pair_sync(pair_bar);
+          float ab[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float m_new = fmaxf(m_run[k], fmaxf(top[k], half_top[half ^ 1][row0 + g + 8 * k]) * qf[k]);
+            const float alpha = m_new == -INFINITY ? 1.f : ex2(m_run[k] - m_new);
+            ab[k] = alpha * (sig_run / sig_new);
+            m_run[k] = m_new;
+            l2[k] = mul2(l2[k], pair(alpha));
+            pm2[k] = mul2(pm2[k], pair(alpha));
+          }
+          sig_run = sig_new;
+          if (t > 0) rescale(ab);
+        }
+        // ---- P, at the head of this half's scores: columns that this warp has read by then
+        float off[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) off[k] = m_run[k] == -INFINITY ? 0.f : -m_run[k];
+        if (whole) {
+#pragma unroll 1
+          for (int c = 0; c < 2; ++c) {
+            uint32_t z[2][16], pk[2][8];
+            tmem_ld_rows16(mine + 32 * c, z[0]);
+            tmem_ld_rows16(mine + kLower + 32 * c, z[1]);
+            tc::wait_ld();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float4 kk = prm[16 * c + 4 * i], vv = prm[64 + 16 * c + 4 * i];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const float2 x = fma2(score_of(kk, z[k >> 1][4 * i + 2 * (k & 1)], z[k >> 1][4 * i + 2 * (k & 1) + 1], k),
+                                      pair(qf[k]), pair(off[k]));
+                const float2 w2 = make_float2(ex2(x.x), ex2(x.y));
+                l2[k] = add2(l2[k], w2);
+                pm2[k] = fma2(w2, make_float2(vv.z, vv.w), pm2[k]);
+                pk[k >> 1][2 * i + (k & 1)] = half2_of(mul2(w2, make_float2(vv.x, vv.y)));
+              }
+            }
+            tmem_st_rows16(mine + 16 * c, pk[0]);
+            tmem_st_rows16(mine + kLower + 16 * c, pk[1]);
+          }
+        } else {
 #pragma unroll 1
           for (int c = 0; c < 4; ++c) {
-            uint32_t s[16];
-            tc::tmem_ld_32x32b_x16(mine + 16 * c, s);
-            tc::wait_ld();
-            const uint32_t see = mask[c >> 1] >> (16 * (c & 1));
+            uint32_t pk[2][4];
+            fetch(c);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float2 y = score(prm[8 * c + e], s[2 * e], s[2 * e + 1]);
-              if ((see >> (2 * e)) & 1u) top = fmaxf(top, y.x);
-              if ((see >> (2 * e + 1)) & 1u) top = fmaxf(top, y.y);
-            }
-          }
-          half_top[m & 1][half][r] = top;
-          pair_sync(1 + (warp & 3));
-          top = fmaxf(top, half_top[m & 1][half ^ 1][r]) * qf.x;
-          if (__any_sync(0xffffffffu, top > m_run + kLazy || sig_new != sig_run)) {
-            const float m_new = fmaxf(m_run, top);
-            const float alpha = m_new == -INFINITY ? 1.f : ex2(m_run - m_new);
-            const float ab = alpha * (sig_run / sig_new);
-            m_run = m_new, sig_run = sig_new;
-            l2 = mul2(l2, make_float2(alpha, alpha));
-            pm2 = mul2(pm2, make_float2(alpha, alpha));
-            if (t > 0) rescale(ab);
-          }
-          const float off = m_run == -INFINITY ? 0.f : -m_run;
-          const float2 off2 = make_float2(off, off);
-          // P of a half lies at the head of that half's scores: columns that this thread has read by then
-#pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
-            uint32_t s[16], pk[8];
-            tc::tmem_ld_32x32b_x16(mine + 16 * c, s);
-            tc::wait_ld();
-            const uint32_t see = mask[c >> 1] >> (16 * (c & 1));
+            for (int i = 0; i < 2; ++i) {
+              const float4 kk = prm[8 * c + 4 * i], vv = prm[64 + 8 * c + 4 * i];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float2 x = fma2(score(prm[8 * c + e], s[2 * e], s[2 * e + 1]), qf, off2);
-              float4 v = prm[64 + 8 * c + e];
-              float2 w2 = make_float2(ex2(x.x), ex2(x.y));
-              if (!((see >> (2 * e)) & 1u)) w2.x = v.x = v.z = 0.f;        // what is hidden may be poisoned
-              if (!((see >> (2 * e + 1)) & 1u)) w2.y = v.y = v.w = 0.f;
-              l2 = add2(l2, w2);
-              pm2 = fma2(w2, make_float2(v.z, v.w), pm2);
-              pk[e] = half2_of(mul2(w2, make_float2(v.x, v.y)));
+              for (int k = 0; k < 4; ++k) {
+                const float2 x = fma2(score(kk, i, k), pair(qf[k]), pair(off[k]));
+                float2 w2 = make_float2(ex2(x.x), ex2(x.y));
+                float4 v = vv;
+                if (!seen(c, i, k, 0)) w2.x = v.x = v.z = 0.f;             // what is hidden may be poisoned: 0 times NaN
+                if (!seen(c, i, k, 1)) w2.y = v.y = v.w = 0.f;
+                l2[k] = add2(l2[k], w2);
+                pm2[k] = fma2(w2, make_float2(v.z, v.w), pm2[k]);
+                pk[k >> 1][2 * i + (k & 1)] = half2_of(mul2(w2, make_float2(v.x, v.y)));
+              }
             }
-            tmem_st8(mine + 8 * c, pk);
+            tmem_st_rows16(mine + 8 * c, pk[0]);
+            tmem_st_rows16(mine + kLower + 8 * c, pk[1]);
           }
         }
         tc::wait_st();
@@ -500,138 +621,134 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
           tc::mbar_arrive(bar(kPrmEmpty + ps));
         }
       }
-      // ---- the item's result; each of the two threads writes half of the row
-      const uint32_t last = it.n0 + uint32_t(it.count) - 1;
-      wait_pv(last);
-      tc::fence_after_sync();
-      float l = l2.x + l2.y, pm = pm2.x + pm2.y;
-      if (half) half_sum[r] = make_float2(l, pm);
-      pair_sync(1 + (warp & 3));
-      if (!half) {
-        l += half_sum[r].x, pm += half_sum[r].y;
-        half_sum[r] = make_float2(l, pm);
-      }
-      pair_sync(1 + (warp & 3));
-      l = half_sum[r].x, pm = half_sum[r].y;
-      const float back = 16777216.f * sig_run, inv = l == 0.f ? 0.f : 1.f / l;
-      const bool starts = w.i0 == 0, ends = w.i1 == w.tiles;
-      const long long slot = 2LL * blockIdx.x + (starts ? 1 : 0);
-      const long long tok = w.rq.row0 + (it.r0 + r) / p.G;
-      const int head = w.h * p.G + int((it.r0 + r) % p.G);
-#pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t o[16];
-        const int d = half * (D / 2) + 16 * c;
-        tc::tmem_ld_32x32b_x16(lane_base + d, o);
-        tc::wait_ld();
-        if (r < it.n_rows) {
-          float x[16];
+      // ---- the item's result: a thread per row and half of its columns
 #pragma unroll
-          for (int e = 0; e < 16; ++e) x[e] = fmaf(__uint_as_float(o[e]), back, pm);
-          if (starts && ends) {
-            uint4* to = reinterpret_cast<uint4*>(p.out + tok * p.out_token + (long long)head * p.out_head + d);
-            const uint4* gt = reinterpret_cast<const uint4*>(p.gate + tok * p.gate_token + (long long)head * p.gate_head + d);
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const uint4 gv = p.gate ? __ldg(gt + e) : make_uint4(0, 0, 0, 0);
-              const uint32_t gw[4] = {gv.x, gv.y, gv.z, gv.w};
-              uint32_t out[4];
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                float a = x[8 * e + 2 * k] * inv, b = x[8 * e + 2 * k + 1] * inv;
-                if (p.gate) {
-                  a /= 1.f + __expf(-DType<T>::to_float(uint16_t(gw[k] & 0xFFFFu)));
-                  b /= 1.f + __expf(-DType<T>::to_float(uint16_t(gw[k] >> 16)));
-                }
-                out[k] = uint32_t(DType<T>::from_float(a)) | (uint32_t(DType<T>::from_float(b)) << 16);
-              }
-              to[e] = make_uint4(out[0], out[1], out[2], out[3]);
-            }
-          } else {
-            float4* to = reinterpret_cast<float4*>(p.part_o + (slot * kRows + r) * D + d);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) to[e] = make_float4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
-          }
+      for (int k = 0; k < 4; ++k) {
+        float l = l2[k].x + l2[k].y, pm = pm2[k].x + pm2[k].y;
+        l += __shfl_xor_sync(0xffffffffu, l, 1), pm += __shfl_xor_sync(0xffffffffu, pm, 1);
+        l += __shfl_xor_sync(0xffffffffu, l, 2), pm += __shfl_xor_sync(0xffffffffu, pm, 2);
+        if (t4 == 0) {
+          half_sum[half][row0 + g + 8 * k] = make_float2(l, pm);
+          if (!half) row_m[row0 + g + 8 * k] = m_run[k];
         }
       }
-      if (!(starts && ends) && !half) p.part_ml[slot * kRows + r] = make_float2(m_run, l);
+      pair_sync(pair_bar);
+      const int r = row0 + lane;
+      const uint32_t last = w.n0 + uint32_t(w.count) - 1;
+      wait_pv(last);
+      tc::fence_after_sync();
+      const float l = half_sum[0][r].x + half_sum[1][r].x, pm = half_sum[0][r].y + half_sum[1][r].y;
+      const float back = 16777216.f * sig_run, inv = l == 0.f ? 0.f : 1.f / l;
+      const bool starts = w.i0 == 0, ends = w.i1 == w.span.tiles;
+      const long long slot = 2LL * blockIdx.x + (starts ? 1 : 0);
+      const long long tok = w.rq.row0 + (w.r0 + r) / p.G;
+      const int head = w.h * p.G + int((w.r0 + r) % p.G);
+#pragma unroll 1
+      for (int c = 0; c < D / 64; ++c) {
+        const int d = half * (D / 2) + 32 * c;
+        const bool write = starts && ends && r < w.n_rows;
+        uint4 gv[4];
+        if (write && p.gate) {
+          const uint4* gt = reinterpret_cast<const uint4*>(p.gate + tok * p.gate_token + (long long)head * p.gate_head + d);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) gv[e] = __ldg(gt + e);
+        }
+        uint32_t o[2][16];
+        tc::tmem_ld_32x32b_x16(lane_base + d, o[0]);
+        tc::tmem_ld_32x32b_x16(lane_base + d + 16, o[1]);
+        tc::wait_ld();
+        if (write) {
+          uint4* to = reinterpret_cast<uint4*>(p.out + tok * p.out_token + (long long)head * p.out_head + d);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t gw[4] = {gv[e].x, gv[e].y, gv[e].z, gv[e].w};
+            uint32_t out[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              float a = fmaf(__uint_as_float(o[e >> 1][8 * (e & 1) + 2 * k]), back, pm) * inv;
+              float b = fmaf(__uint_as_float(o[e >> 1][8 * (e & 1) + 2 * k + 1]), back, pm) * inv;
+              if (p.gate) {
+                a /= 1.f + __expf(-DType<T>::to_float(uint16_t(gw[k] & 0xFFFFu)));
+                b /= 1.f + __expf(-DType<T>::to_float(uint16_t(gw[k] >> 16)));
+              }
+              out[k] = uint32_t(DType<T>::from_float(a)) | (uint32_t(DType<T>::from_float(b)) << 16);
+            }
+            to[e] = make_uint4(out[0], out[1], out[2], out[3]);
+          }
+        } else if (r < w.n_rows) {
+          float4* to = reinterpret_cast<float4*>(p.part_o + (slot * kRows + r) * D + d);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            to[e] = make_float4(fmaf(__uint_as_float(o[e >> 2][4 * (e & 3)]), back, pm),
+                                fmaf(__uint_as_float(o[e >> 2][4 * (e & 3) + 1]), back, pm),
+                                fmaf(__uint_as_float(o[e >> 2][4 * (e & 3) + 2]), back, pm),
+                                fmaf(__uint_as_float(o[e >> 2][4 * (e & 3) + 3]), back, pm));
+        }
+      }
+      if (!(starts && ends) && !half) p.part_ml[slot * kRows + r] = make_float2(row_m[r], l);
       if (starts && !ends && tid == 0)
-        p.meta[blockIdx.x] = make_int4(int((w.item_at + w.tiles - 1) / share), w.b, w.h, int(w.rt));
+        p.meta[blockIdx.x] = make_int4(int((w.item_at + w.span.tiles - 1) / share), w.b, w.h, int(w.rt));
       tc::fence_before_sync();
     });
   } else if (warp < kKeyWarp) {
-    // ================================================================ values: 32 tokens a warp
+    // ================================================================ values: 16 tokens a warp
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     const int q = warp - kValueWarp, tg = lane >> 3, g = lane & 7;
-    constexpr int kBlocks = D / 64;              // 16-byte loads per lane and 16 tokens
+    constexpr int kBlocks = D / 64;              // 16-byte loads per lane and tile
     const int page_mask = (1 << p.c.page_log2) - 1;
-    // where the pair of element (n + g) % 8 goes: row, chunk of the swizzle, half of the chunk; a step of 16 tokens
-    // flips bit 1 of the chunk
+    // where the pair of element (n + g) % 8 goes: row, chunk of the swizzle, half of the chunk
     uint32_t put[8];
     {
-      const int tok = 32 * q + 4 * tg;
+      const int tok = 16 * q + 4 * tg;
 #pragma unroll
       for (int n = 0; n < 8; ++n) {
         const uint32_t dim = uint32_t(n + g) & 7u;
         put[n] = sm + S::kV + (tok >> 6) * (D * 128) + (8 * g + dim) * 128 + ((((tok & 63) >> 3) ^ dim) << 4) + (tg & 1) * 8;
       }
     }
-    items([&](const Item& it) {
-      uint4 vc[kBlocks];                         // the next 16 tokens'
-      const uint4 *from[2], *next;
-      bool ok[2], next_ok;
+    items([&]() {
+      uint4 vc[kBlocks];
+      const uint4* from = nullptr;
+      bool ok = false;
       auto locate = [&](int t) {
-        const uint32_t m = it.n0 + uint32_t(t);
-        const int ps = int(m % kParamStages), first = it.span.id(w.i0 + t) * kTile + 32 * q;
+        const uint32_t m = w.n0 + uint32_t(t);
+        const int ps = int(m % kParamStages), first = w.span.id(w.i0 + t) * kTile + 16 * q;
         wait(kPrmFull + ps, (m / kParamStages) & 1u, tc::kStatusWaitFull);
-#pragma unroll
-        for (int blk = 0; blk < 2; ++blk) {
-          const int page = info[ps].page[2 * q + blk];
-          ok[blk] = unsigned(page) < unsigned(p.c.n_pages);      // after a wait that gave up it may be anything
-          from[blk] = reinterpret_cast<const uint4*>(p.c.v + cache_codes_at(ok[blk] ? page : 0, w.h, p.c.heads, p.c.page_log2, D) +
-                                                     value_word_at((first + 16 * blk) & page_mask, 0, D)) + lane;
-        }
+        const int page = info[ps].page[q];
+        ok = unsigned(page) < unsigned(p.c.n_pages);             // after a wait that gave up it may be anything
+        from = reinterpret_cast<const uint4*>(p.c.v + cache_codes_at(ok ? page : 0, w.h, p.c.heads, p.c.page_log2, D) +
+                                              value_word_at(first & page_mask, 0, D)) + lane;
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(bar(kPrmEmpty + ps));
       };
-      auto load = [&](int i) { vc[i] = next_ok ? __ldg(next + 32 * i) : make_uint4(0, 0, 0, 0); };
+      auto load = [&](int i) { vc[i] = ok ? __ldg(from + 32 * i) : make_uint4(0, 0, 0, 0); };
       locate(0);
-      next = from[0], next_ok = ok[0];
 #pragma unroll
       for (int i = 0; i < kBlocks; ++i) load(i);
-      for (int t = 0; t < it.count; ++t) {
-        const uint32_t m = it.n0 + uint32_t(t), use = m / S::kStages;
-        const int st = int(m % S::kStages), vb = 2 * st + (q >> 1);
-        if (use > 0) wait(kVEmpty + vb, (use - 1) & 1u, tc::kStatusWaitEmpty);
 #pragma unroll 1
-        for (int blk = 0; blk < 2; ++blk) {
-          if (blk == 0) {
-            next = from[1], next_ok = ok[1];
-          } else if (t + 1 < it.count) {
-            locate(t + 1);
-            next = from[0], next_ok = ok[0];
-          } else {
-            next_ok = false;
-          }
-          uint32_t to[8];
+      for (int t = 0; t < w.count; ++t) {
+        const uint32_t m = w.n0 + uint32_t(t), use = m / S::kStages;
+        const int st = int(m % S::kStages), vb = 2 * st + (q >> 2);
+        if (t + 1 < w.count) locate(t + 1);
+        else ok = false;
+        if (use > 0) wait(kVEmpty + vb, (use - 1) & 1u, tc::kStatusWaitEmpty);
+        const uint32_t at = uint32_t(st * S::kOperand);
 #pragma unroll
-          for (int n = 0; n < 8; ++n) to[n] = (put[n] ^ uint32_t(32 * blk)) + st * S::kOperand;
+        for (int db = 0; db < kBlocks; ++db) {
+          const uint32_t a0 = __funnelshift_r(vc[db].x, vc[db].x, 4 * g), a1 = __funnelshift_r(vc[db].y, vc[db].y, 4 * g);
+          const uint32_t a2 = __funnelshift_r(vc[db].z, vc[db].z, 4 * g), a3 = __funnelshift_r(vc[db].w, vc[db].w, 4 * g);
+          load(db);                              // the next tile's, into the registers just read
 #pragma unroll
-          for (int db = 0; db < kBlocks; ++db) {
-            const uint32_t a0 = __funnelshift_r(vc[db].x, vc[db].x, 4 * g), a1 = __funnelshift_r(vc[db].y, vc[db].y, 4 * g);
-            const uint32_t a2 = __funnelshift_r(vc[db].z, vc[db].z, 4 * g), a3 = __funnelshift_r(vc[db].w, vc[db].w, 4 * g);
-            load(db);                            // into the registers just read
+          for (int hf = 0; hf < 2; ++hf) {
+            uint32_t x = __byte_perm(a0, a1, hf ? 0x7632 : 0x5410), y = __byte_perm(a2, a3, hf ? 0x7632 : 0x5410);
 #pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-              uint32_t x = __byte_perm(a0, a1, hf ? 0x7632 : 0x5410), y = __byte_perm(a2, a3, hf ? 0x7632 : 0x5410);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const uint32_t at = to[hf * 4 + e] + db * 8192;
-                if (e & 1) {
-                  sts64(at, hfma2(x & 0x00F000F0u, 0x2C002C00u, 0x80088008u), hfma2(y & 0x00F000F0u, 0x2C002C00u, 0x80088008u));
-                  x >>= 8, y >>= 8;
-                } else {
-                  sts64(at, hadd2(x & 0x000F000Fu, 0x80088008u), hadd2(y & 0x000F000Fu, 0x80088008u));
-                }
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t to = put[hf * 4 + e] + at + db * 8192;
+              if (e & 1) {
+                sts64(to, hfma2(x & 0x00F000F0u, 0x2C002C00u, 0x80088008u), hfma2(y & 0x00F000F0u, 0x2C002C00u, 0x80088008u));
+                x >>= 8, y >>= 8;
+              } else {
+                sts64(to, hadd2(x & 0x000F000Fu, 0x80088008u), hadd2(y & 0x000F000Fu, 0x80088008u));
               }
             }
           }
@@ -642,26 +759,28 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
       }
     });
   } else if (warp < kParamWarp) {
-    // ================================================================ keys: 64 tokens a warp
+    // ================================================================ keys: 32 tokens a warp
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     // A block of 64 elements is two 16-byte pieces a token: load i holds piece l8 & 1 of token 16 i + tok0.
     const int q = warp - kKeyWarp, l8 = lane >> 3, tk = lane & 7, tok0 = 8 * (l8 >> 1) + tk;
     const int page_mask = (1 << p.c.page_log2) - 1;
     uint32_t put[4];                             // word j of the piece
 #pragma unroll
-    for (int j = 0; j < 4; ++j) put[j] = sm + S::kK + (64 * q + tok0) * 128 + ((((l8 & 1) * 4 + j) ^ tk) << 4);
-    items([&](const Item& it) {
-      const int units = it.count * kKB;          // blocks of the item's tiles
-      uint4 kc[2][4];                            // the next two blocks
-      const uint8_t* from[4];
-      bool ok[4];
-      auto load = [&](uint4 (&to)[4], int u) {
+    for (int j = 0; j < 4; ++j) put[j] = sm + S::kK + (32 * q + tok0) * 128 + ((((l8 & 1) * 4 + j) ^ tk) << 4);
+    items([&]() {
+      const int units = w.count * kKB;           // blocks of the part's tiles
+      uint4 kc[2][2];                            // the next two blocks
+      const uint8_t* from[2];
+      bool ok[2];
+      auto load = [&](uint4 (&to)[2], int u) {
+        if (u >= units) return;
         if (u % kKB == 0) {
-          const uint32_t m = it.n0 + uint32_t(u / kKB);
-          const int ps = int(m % kParamStages), first = it.span.id(w.i0 + u / kKB) * kTile + 64 * q + tok0;
+          const uint32_t m = w.n0 + uint32_t(u / kKB);
+          const int ps = int(m % kParamStages), first = w.span.id(w.i0 + u / kKB) * kTile + 32 * q + tok0;
           wait(kPrmFull + ps, (m / kParamStages) & 1u, tc::kStatusWaitFull);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int page = info[ps].page[4 * q + i];
+          for (int i = 0; i < 2; ++i) {
+            const int page = info[ps].page[2 * q + i];
             ok[i] = unsigned(page) < unsigned(p.c.n_pages);      // after a wait that gave up it may be anything
             from[i] = p.c.k + cache_codes_at(ok[i] ? page : 0, w.h, p.c.heads, p.c.page_log2, D) +
                       key_word_at((first + 16 * i) & page_mask, 4 * (l8 & 1), D);
@@ -670,16 +789,17 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
           if (lane == 0) tc::mbar_arrive(bar(kPrmEmpty + ps));
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 2; ++i)
           to[i] = ok[i] ? __ldg(reinterpret_cast<const uint4*>(from[i] + 32 * (u % kKB))) : make_uint4(0, 0, 0, 0);
       };
-      auto unpack = [&](const uint4 (&c)[4], int u) {
-        const uint32_t m = it.n0 + uint32_t(u / kKB), use = m / S::kStages;
+      auto unpack = [&](const uint4 (&c)[2], int u) {
+        if (u >= units) return;
+        const uint32_t m = w.n0 + uint32_t(u / kKB), use = m / S::kStages;
         const int st = int(m % S::kStages), kb = u % kKB, kbar = st * kKB + kb;
         if (use > 0) wait(kKEmpty + kbar, (use - 1) & 1u, tc::kStatusWaitEmpty);
         const uint32_t at = uint32_t(st * S::kOperand + kb * (kTile * 128));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 2; ++i) {
           const uint32_t v[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -692,25 +812,26 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
         if (lane == 0) tc::mbar_arrive(bar(kKFull + kbar));
       };
       load(kc[0], 0);
-      if (units > 1) load(kc[1], 1);
+      load(kc[1], 1);
 #pragma unroll 1
       for (int u = 0; u < units; u += 2) {
         unpack(kc[0], u);
-        if (u + 2 < units) load(kc[0], u + 2);
-        if (u + 1 < units) unpack(kc[1], u + 1);
-        if (u + 3 < units) load(kc[1], u + 3);
+        load(kc[0], u + 2);
+        unpack(kc[1], u + 1);
+        load(kc[1], u + 3);
       }
     });
   } else if (warp == kParamWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     // ================================================================ parameters: tokens 32 j + lane
     const int page_mask = (1 << p.c.page_log2) - 1;
-    items([&](const Item& it) {
+    items([&]() {
       const int* table = p.table + (long long)w.b * p.table_ld;
       float sig = 0.f;                           // running power of two of the item
       int page[4], page_next[4];                 // this tile's, the next one's
       uint32_t kp[4], vp[4];                     // pairs of this tile
       auto pages = [&](int t, int (&to)[4]) {
-        const int first = it.span.id(w.i0 + t) * kTile;
+        const int first = w.span.id(w.i0 + t) * kTile;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int tok = first + 32 * j + lane;
@@ -718,10 +839,10 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
         }
       };
       auto seen = [&](int tok, int pg) {
-        return pg >= 0 && tok <= it.last_pos && (p.window == 0 || tok > it.first_pos - p.window || tok < p.sinks);
+        return pg >= 0 && tok <= w.last_pos && (p.window == 0 || tok > w.first_pos - p.window || tok < p.sinks);
       };
       auto pairs = [&](int t) {                  // checks the pages too
-        const int first = it.span.id(w.i0 + t) * kTile;
+        const int first = w.span.id(w.i0 + t) * kTile;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int tok = first + 32 * j + lane;
@@ -738,10 +859,10 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
       };
       pages(0, page);
       pairs(0);
-      if (it.count > 1) pages(1, page_next);
-      for (int t = 0; t < it.count; ++t) {
-        const uint32_t m = it.n0 + uint32_t(t);
-        const int ps = int(m % kParamStages), first = it.span.id(w.i0 + t) * kTile;
+      if (w.count > 1) pages(1, page_next);
+      for (int t = 0; t < w.count; ++t) {
+        const uint32_t m = w.n0 + uint32_t(t);
+        const int ps = int(m % kParamStages), first = w.span.id(w.i0 + t) * kTile;
         float2 kk[4], vv[4];
         float top = kMinStep;
         uint32_t valid[4];
@@ -756,8 +877,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
         int now[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) now[j] = page[j], page[j] = page_next[j];
-        if (t + 1 < it.count) pairs(t + 1);      // under way while this tile's are written
-        if (t + 2 < it.count) pages(t + 2, page_next);
+        if (t + 1 < w.count) pairs(t + 1);      // under way while this tile's are written
+        if (t + 2 < w.count) pages(t + 2, page_next);
         for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         sig = fmaxf(sig, pow2_above(top));
         const float inv = 1.f / sig;
@@ -774,47 +895,47 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
           info[ps].sig = sig;
 #pragma unroll
           for (int j = 0; j < 4; ++j) info[ps].valid[j] = valid[j];
-          info[ps].whole = all && first + kTile <= it.first_pos + 1 &&
-                           (p.window == 0 || first > it.last_pos - p.window || first + kTile <= p.sinks);
+          info[ps].whole = all && first + kTile <= w.first_pos + 1 &&
+                           (p.window == 0 || first > w.last_pos - p.window || first + kTile <= p.sinks);
         }
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(bar(kPrmFull + ps));
       }
     });
   } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     // ================================================================ products
-    items([&](const Item& it) {
-      if (tc::elect_one()) {
+    items([&]() {
+      if (warp == kProductWarp && tc::elect_one()) {
         const uint64_t tmpl = tc::smem_desc(0u, 16u, 1024u, 2u);
+        const uint32_t lo = uint32_t(tmpl), hi = uint32_t(tmpl >> 32);
         const uint32_t idesc_s = tc::instr_desc(0, 128, kTile), idesc_o = tc::instr_desc(0, 128, D);
         auto scores = [&](uint32_t m) {
           const int st = int(m % S::kStages);
           // S's buffer held P of the tile before last: its product has to be through
-          if (m >= 2 + it.n0) wait_pv(m - 2);
-          const uint64_t a = tmpl | ((sm + S::kQ) >> 4), b = tmpl | ((sm + S::kK + st * S::kOperand) >> 4);
+          if (m >= 2 + w.n0) wait_pv(m - 2);
+          const uint32_t a = lo | ((sm + S::kQ) >> 4), b = lo | ((sm + S::kK + st * S::kOperand) >> 4);
 #pragma unroll 1
           for (int kb = 0; kb < kKB; ++kb) {
             wait(kKFull + st * kKB + kb, (m / S::kStages) & 1u, tc::kStatusWaitFull);
             tc::fence_after_sync();
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              mma_ss(tmem + 256 + 128 * (m & 1), a + kb * 1024 + k * 2, b + kb * 1024 + k * 2, idesc_s, kb > 0 || k > 0);
+            mma_ss_block(tmem + 256 + 128 * (m & 1), a + kb * 1024, b + kb * 1024, hi, idesc_s, kb > 0);
             tc::mma_commit(bar(kKEmpty + st * kKB + kb));
           }
           tc::mma_commit(bar(kSFull + int(m & 1)));
         };
-        scores(it.n0);
-        for (int t = 0; t < it.count; ++t) {
-          const uint32_t m = it.n0 + uint32_t(t);
-          if (t + 1 < it.count) scores(m + 1);
+        scores(w.n0);
+        for (int t = 0; t < w.count; ++t) {
+          const uint32_t m = w.n0 + uint32_t(t);
+          if (t + 1 < w.count) scores(m + 1);
           const int st = int(m % S::kStages);
           wait(kPFull + int(m & 1), (m >> 1) & 1u, tc::kStatusWaitFull);
-          const uint64_t b = tmpl | ((sm + S::kV + st * S::kOperand) >> 4);
+          const uint32_t b = lo | ((sm + S::kV + st * S::kOperand) >> 4);
 #pragma unroll 1
           for (int k = 0; k < 2; ++k) {
             wait(kVFull + 2 * st + k, (m / S::kStages) & 1u, tc::kStatusWaitFull);
             tc::fence_after_sync();
-            tc::mma_ts_kblock(tmem, tmem + 256 + 128 * (m & 1) + 64 * k, uint32_t(b) + k * (D * 8), uint32_t(b >> 32), idesc_o,
+            tc::mma_ts_kblock(tmem, tmem + 256 + 128 * (m & 1) + 64 * k, b + k * (D * 8), hi, idesc_o,
                               t > 0 || k > 0);
             tc::mma_commit(bar(kVEmpty + 2 * st + k));
           }
