@@ -88,18 +88,16 @@ __device__ __forceinline__ float pow2_above(float x) {
 // Tiles of all items of request b (its row tiles are equal but for what they see).
 __device__ __forceinline__ Request rows_request(const AttendParams& p, int b) {
   Request r = request_of(p, b);
-  if ((long long)r.rows * p.G > p.rows_limit) r.rows = 0;        // the tile kernel's
+  if (r.rows * p.G > p.rows_limit) r.rows = 0;        // the tile kernel's
   return r;
 }
 template <int kRows>
 __device__ __forceinline__ long long request_tiles(const AttendParams& p, int b) {
   const Request r = rows_request(p, b);
   long long sum = 0;
-  const long long rows = (long long)r.rows * p.G;
-  for (long long r0 = 0; r0 < rows; r0 += kRows) {
-    const int last = int((min(r0 + kRows, rows) - 1) / p.G), base = r.len - r.rows;
-    sum += Span<kTile>(base + int(r0 / p.G), base + last, r.len, p.window, p.sinks).tiles;
-  }
+  const int rows = r.rows * p.G, base = r.len - r.rows;
+  for (int r0 = 0; r0 < rows; r0 += kRows)
+    sum += Span<kTile>(base + token_of(p, r0), base + token_of(p, min(r0 + kRows, rows) - 1), r.len, p.window, p.sinks).tiles;
   return sum * p.c.heads;
 }
 
@@ -165,12 +163,12 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) attend_rows_kern
   long long cur = begin, req_at = first_tile;
   for (int b = first_b; cur < stop && b < p.B; ++b) {
     const Request rq = rows_request(p, b);
-    const long long rows = (long long)rq.rows * p.G;
+    const int rows = rq.rows * p.G;
     const int base = rq.len - rq.rows;
     for (int h = 0; h < p.c.heads && cur < stop; ++h) {
-      for (long long r0 = 0; r0 < rows && cur < stop; r0 += kRows) {
-        const int n_rows = int(min((long long)kRows, rows - r0));
-        const int first_pos = base + int(r0 / p.G), last_pos = base + int((r0 + n_rows - 1) / p.G);
+      for (int r0 = 0; r0 < rows && cur < stop; r0 += kRows) {
+        const int n_rows = min(kRows, rows - r0);
+        const int first_pos = base + token_of(p, r0), last_pos = base + token_of(p, r0 + n_rows - 1);
         const Span<kTile> span(first_pos, last_pos, rq.len, p.window, p.sinks);
         if (req_at + span.tiles <= cur) {
           req_at += span.tiles;
@@ -185,8 +183,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) attend_rows_kern
 #pragma unroll
           for (int i = 0; i < D / 32; ++i) v[i] = 0.f;
           if (r < n_rows) {
-            const long long tok = rq.row0 + (r0 + r) / p.G;
-            const uint16_t* x = p.q + tok * p.q_token + (long long)(h * p.G + int((r0 + r) % p.G)) * p.q_head;
+            const int tok = token_of(p, r0 + r);
+            const uint16_t* x = p.q + (rq.row0 + tok) * p.q_token + (long long)(h * p.G + r0 + r - tok * p.G) * p.q_head;
 #pragma unroll
             for (int i = 0; i < D / 32; ++i) v[i] = DType<T>::to_float(x[lane * (D / 32) + i]);
           }
@@ -222,7 +220,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) attend_rows_kern
             const float2 k = row_k[r];
             qf[n][e] = k.x, qs[n][e] = k.y;
             m[n][e] = -INFINITY, l[n][e] = 0.f, pm[n][e] = 0.f;
-            pos[n][e] = r < n_rows ? base + int((r0 + r) / p.G) : -1;
+            pos[n][e] = r < n_rows ? base + token_of(p, r0 + r) : -1;
           }
         float o[NT][D / 16][4];
 #pragma unroll
@@ -473,8 +471,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) attend_rows_kern
             c = fmaf(part[1], f, c);
           }
           if (starts && ends) {
-            const long long tok = rq.row0 + (r0 + r) / p.G;
-            const int head = h * p.G + int((r0 + r) % p.G);
+            const int at = token_of(p, r0 + r), head = h * p.G + r0 + r - at * p.G;
+            const long long tok = rq.row0 + at;
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
             const uint32_t lo = DType<T>::from_float(gated<T>(a * inv, p, tok, head, d));
             const uint32_t hi = DType<T>::from_float(gated<T>(c * inv, p, tok, head, d + 1));
@@ -486,7 +484,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) attend_rows_kern
         }
         if (starts && !ends && tid == 0) {
           const long long last = (req_at + span.tiles - 1) / share;
-          p.meta[blockIdx.x] = make_int4(int(last), b, h, int(r0 / kRows));
+          p.meta[blockIdx.x] = make_int4(int(last), b, h, r0 / kRows);
         }
         req_at += span.tiles;
         cur = min(req_at, stop);
@@ -508,9 +506,9 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const __gr
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, way = warp % Ways;
   const int c0 = blockIdx.x, c1 = meta.x, b = meta.y, h = meta.z, r = blockIdx.y * (kJoinWarps / Ways) + warp / Ways;
   const Request rq = request_of(p, b);
-  const long long row = (long long)meta.w * kRows + r;
-  if (row - r + blockIdx.y * (kJoinWarps / Ways) >= (long long)rq.rows * p.G) return;      // none of the block's rows
-  const bool live = row < (long long)rq.rows * p.G;
+  const int row = meta.w * kRows + r;
+  if (row - r + int(blockIdx.y) * (kJoinWarps / Ways) >= rq.rows * p.G) return;      // none of the block's rows
+  const bool live = row < rq.rows * p.G;
   auto slot = [&](int c) { return (c == c0 ? 2LL * c + 1 : 2LL * c) * kRows + r; };
   float top = -INFINITY, sum = 0.f, x[kPer];
 #pragma unroll
@@ -547,8 +545,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const __gr
     }
   }
   if (!live) return;
-  const long long tok = rq.row0 + row / p.G;
-  const int head = h * p.G + int(row % p.G), d = lane * kPer;
+  const int at = token_of(p, row), head = h * p.G + row - at * p.G, d = lane * kPer;
+  const long long tok = rq.row0 + at;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   uint32_t* to = reinterpret_cast<uint32_t*>(p.out + tok * p.out_token + (long long)head * p.out_head + d);
 #pragma unroll
@@ -674,6 +672,10 @@ extern "C" int b200lut_attend(const b200lut_attend_args* a, void* workspace, siz
   p.table = a->block_table, p.table_ld = a->table_stride, p.kv_len = a->kv_len, p.row_start = a->row_start;
   p.T = a->T, p.B = a->B, p.Hq = a->n_heads, p.G = a->n_heads / p.c.heads, p.width = a->width;
   p.window = a->window, p.sinks = a->sinks;
+  B200LUT_REQUIRE((long long)a->T * p.G <= INT_MAX - 256, B200LUT_ERR_UNSUPPORTED, "attend: too many rows (T %d)", a->T);
+  int up = 0;                  // 2^up is the power of two >= G
+  while ((1 << up) < p.G) ++up;
+  p.g_mul = uint32_t(((1ull << (31 + up)) + p.G - 1) / p.G), p.g_shift = up - 1;
   p.scale = a->scale * 1.4426950408889634f;
   p.wait_cycles = gemm_wait_cycles();
   const cudaStream_t st = cudaStream_t(stream);

@@ -28,7 +28,9 @@ struct AttendParams {
   const int* kv_len;
   const int* row_start;        // or null: one row per request
   long long table_ld;
-  int T, B, Hq, G, width, window, sinks;
+  int T, B, Hq, G, width, window, sinks;     // T * G < 2^31
+  uint32_t g_mul;              // x / G = umulhi(x, g_mul) >> g_shift for x < 2^31 (G = 1: x)
+  int g_shift;
   float scale;                 // scale * log2(e)
   // a request of at most so many rows (times query heads per key/value head) is the single-row kernel's, the
   // others are the tile kernel's; INT_MAX: no tile kernel runs
@@ -39,6 +41,11 @@ struct AttendParams {
   float2* part_ml;
   float* part_o;
 };
+
+// Row r of a request's head is its token r / G and the head's query head r % G.
+__device__ __forceinline__ int token_of(const AttendParams& p, int r) {
+  return p.G == 1 ? r : int(__umulhi(uint32_t(r), p.g_mul) >> p.g_shift);
+}
 
 // The requests' rows and lengths as the kernels read them (device data: clamped, never trusted).
 struct Request {

@@ -188,20 +188,18 @@ __device__ __forceinline__ void bounded_wait(uint32_t bar, uint32_t parity, vola
 // ---- the line of tiles ---------------------------------------------------------------------------------------
 __device__ __forceinline__ Request tiles_request(const AttendParams& p, int b) {
   Request r = request_of(p, b);
-  if ((long long)r.rows * p.G <= p.rows_limit) r.rows = 0;       // the other kernel's
+  if (r.rows * p.G <= p.rows_limit) r.rows = 0;       // the other kernel's
   return r;
 }
-__device__ __forceinline__ Span<kTile> span_of(const AttendParams& p, const Request& r, long long r0) {
-  const long long rows = (long long)r.rows * p.G;
+__device__ __forceinline__ Span<kTile> span_of(const AttendParams& p, const Request& r, int r0) {
   const int base = r.len - r.rows;
-  const long long last = min(r0 + kRows, rows) - 1;
-  return Span<kTile>(base + int(r0 / p.G), base + int(last / p.G), r.len, p.window, p.sinks);
+  return Span<kTile>(base + token_of(p, r0), base + token_of(p, min(r0 + kRows, r.rows * p.G) - 1), r.len, p.window, p.sinks);
 }
 // Tiles of one head of request b, summed over its row tiles by a whole warp (all lanes get the sum).
 __device__ __forceinline__ long long head_tiles(const AttendParams& p, const Request& r, int lane) {
-  const long long n = ((long long)r.rows * p.G + kRows - 1) / kRows;
+  const int n = (r.rows * p.G + kRows - 1) / kRows;
   long long sum = 0;
-  for (long long i = lane; i < n; i += 32) sum += span_of(p, r, i * kRows).tiles;
+  for (int i = lane; i < n; i += 32) sum += span_of(p, r, i * kRows).tiles;
   for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   return sum;
 }
@@ -211,8 +209,8 @@ __device__ __forceinline__ long long head_tiles(const AttendParams& p, const Req
 struct Work {
   Request rq;
   Span<kTile> span;
-  long long rt, r0, item_at;   // item_at: tiles of the line before the item
-  int b, h, i0, i1;
+  long long item_at;           // tiles of the line before the item
+  int b, h, rt, r0, i0, i1;
   int n_rows, base, first_pos, last_pos;
   uint32_t n0;                 // tiles of this block before this part's
   int count, more;
@@ -224,17 +222,16 @@ __device__ __forceinline__ void open_part(const AttendParams& p, Work* w, long l
   w->i0 = int(cur - w->item_at), w->i1 = int(min((long long)w->span.tiles, stop - w->item_at));
   w->count = w->i1 - w->i0;
   w->r0 = w->rt * kRows;
-  const long long rows = (long long)w->rq.rows * p.G;
-  w->n_rows = int(min((long long)kRows, rows - w->r0));
+  w->n_rows = min(kRows, w->rq.rows * p.G - w->r0);
   w->base = w->rq.len - w->rq.rows;
-  w->first_pos = w->base + int(w->r0 / p.G), w->last_pos = w->base + int((w->r0 + w->n_rows - 1) / p.G);
+  w->first_pos = w->base + token_of(p, w->r0), w->last_pos = w->base + token_of(p, w->r0 + w->n_rows - 1);
   w->more = w->item_at + w->i1 < stop;
 }
 __device__ __forceinline__ void next_part(const AttendParams& p, Work* w, long long stop) {
   const long long cur = w->item_at + w->i1;
   w->n0 += uint32_t(w->count);
   w->item_at += w->span.tiles;
-  if ((w->rt + 1) * kRows < (long long)w->rq.rows * p.G) {
+  if ((w->rt + 1) * kRows < w->rq.rows * p.G) {
     ++w->rt;
   } else {
     w->rt = 0;
@@ -341,9 +338,9 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
     long long off = begin - first_at;
     const int h = int(off / per_head);
     off -= h * per_head;
-    const long long n = ((long long)rq.rows * p.G + kRows - 1) / kRows;
-    long long rt = 0;
-    for (long long c0 = 0; c0 < n; c0 += 32) {
+    const int n = (rq.rows * p.G + kRows - 1) / kRows;
+    int rt = 0;
+    for (int c0 = 0; c0 < n; c0 += 32) {
       const long long tiles = c0 + lane < n ? span_of(p, rq, (c0 + lane) * kRows).tiles : 0;
       long long inc = tiles;
       for (int o = 1; o < 32; o <<= 1) {
@@ -379,9 +376,9 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
           const int r = warp + i * kWarps;
           x[i] = make_uint4(0, 0, 0, 0);
           if (r < w.n_rows && lane < kChunks) {
-            const long long tok = w.rq.row0 + (w.r0 + r) / p.G;
-            x[i] = __ldg(reinterpret_cast<const uint4*>(p.q + tok * p.q_token +
-                                                        (long long)(w.h * p.G + int((w.r0 + r) % p.G)) * p.q_head) + lane);
+            const int tok = token_of(p, w.r0 + r);
+            x[i] = __ldg(reinterpret_cast<const uint4*>(p.q + (w.rq.row0 + tok) * p.q_token +
+                                                        (long long)(w.h * p.G + w.r0 + r - tok * p.G) * p.q_head) + lane);
           }
         }
 #pragma unroll
@@ -444,7 +441,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
       for (int k = 0; k < 4; ++k) {
         const int r = row0 + g + 8 * k;
         qf[k] = row_k[r].x, qs[k] = row_k[r].y;
-        pos[k] = r < w.n_rows ? w.base + int((w.r0 + r) / p.G) : -1;
+        pos[k] = r < w.n_rows ? w.base + token_of(p, w.r0 + r) : -1;
         m_run[k] = -INFINITY;
         l2[k] = pm2[k] = make_float2(0.f, 0.f);
       }
@@ -641,8 +638,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
       const float back = 16777216.f * sig_run, inv = l == 0.f ? 0.f : 1.f / l;
       const bool starts = w.i0 == 0, ends = w.i1 == w.span.tiles;
       const long long slot = 2LL * blockIdx.x + (starts ? 1 : 0);
-      const long long tok = w.rq.row0 + (w.r0 + r) / p.G;
-      const int head = w.h * p.G + int((w.r0 + r) % p.G);
+      const int at = token_of(p, w.r0 + r), head = w.h * p.G + w.r0 + r - at * p.G;
+      const long long tok = w.rq.row0 + at;
 #pragma unroll 1
       for (int c = 0; c < D / 64; ++c) {
         const int d = half * (D / 2) + 32 * c;
@@ -687,7 +684,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
       }
       if (!(starts && ends) && !half) p.part_ml[slot * kRows + r] = make_float2(row_m[r], l);
       if (starts && !ends && tid == 0)
-        p.meta[blockIdx.x] = make_int4(int((w.item_at + w.span.tiles - 1) / share), w.b, w.h, int(w.rt));
+        p.meta[blockIdx.x] = make_int4(int((w.item_at + w.span.tiles - 1) / share), w.b, w.h, w.rt);
       tc::fence_before_sync();
     });
   } else if (warp < kKeyWarp) {
