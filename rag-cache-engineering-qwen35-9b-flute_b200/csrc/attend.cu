@@ -23,8 +23,9 @@ namespace {
 
 __device__ int g_attend_status = 0;
 constexpr int kBadPage = 0x6200;
-constexpr int kWarps = 8;
-constexpr int kTile = 16;
+// What an item costs a block besides its tiles, in tiles: reading the rows, filling the ring, joining the warps. Counted
+// in the shares: blocks with six short items took twice as long as blocks with one long one.
+constexpr int kItemCost = 24;
 constexpr float kLazy = 8.f;           // the running maximum may lag by this many powers of two
 constexpr uint32_t kOnes = 0x3C003C00u;     // two halves of 1
 constexpr float kMinStep = 7.888609e-31f;   // 2^-100
@@ -32,9 +33,16 @@ constexpr float kMinStep = 7.888609e-31f;   // 2^-100
 template <int D, int NT>
 struct Shape {
   static constexpr int kRows = 8 * NT;
+  // 16-token pieces of a warp's step. One: with two the loop has 1100 instructions at 256 elements, more than the
+  // scheduler's instruction cache holds, and takes 134 us where it takes 111 (64 sequences of up to 8192 tokens).
+  static constexpr int kSub = 1;
+  static constexpr int kTile = 16 * kSub;
+  static constexpr int kWarps = 8;
+  static constexpr int kBlocks = NT == 1 ? 2 : 1;              // per SM
   static constexpr int kWords = D / 32;                        // 32-bit words of a key row per lane
   static constexpr int kPieces = D >= 128 ? D / 64 : 1;        // 16-byte key pieces per lane and tile
-  static constexpr int kStage = 16 * D + 512;                  // bytes of a tile: keys, values, pairs
+  static constexpr int kPart = 16 * D + 512;                   // bytes of 16 tokens: keys, values, pairs
+  static constexpr int kStage = kSub * kPart;
   static constexpr int kStages = D == 256 ? 2 : D == 128 ? 4 : 6;
   static constexpr int kFold = kRows * (D + 4) * 4;            // a warp's partial result, in its ring's place
   static constexpr int kRing = kStages * kStage > kFold ? kStages * kStage : kFold;
@@ -91,20 +99,21 @@ __device__ __forceinline__ Request rows_request(const AttendParams& p, int b) {
   if (r.rows * p.G > p.rows_limit) r.rows = 0;        // the tile kernel's
   return r;
 }
-template <int kRows>
+template <int kRows, int kTile>
 __device__ __forceinline__ long long request_tiles(const AttendParams& p, int b) {
   const Request r = rows_request(p, b);
   long long sum = 0;
   const int rows = r.rows * p.G, base = r.len - r.rows;
   for (int r0 = 0; r0 < rows; r0 += kRows)
-    sum += Span<kTile>(base + token_of(p, r0), base + token_of(p, min(r0 + kRows, rows) - 1), r.len, p.window, p.sinks).tiles;
+    sum += Span<kTile>(base + token_of(p, r0), base + token_of(p, min(r0 + kRows, rows) - 1), r.len, p.window, p.sinks).tiles + kItemCost;
   return sum * p.c.heads;
 }
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) attend_rows_kernel(const __grid_constant__ AttendParams p) {
+__global__ void __launch_bounds__(Shape<D, NT>::kWarps * 32, Shape<D, NT>::kBlocks)
+attend_rows_kernel(const __grid_constant__ AttendParams p) {
   using S = Shape<D, NT>;
-  constexpr int kRows = S::kRows;
+  constexpr int kRows = S::kRows, kWarps = S::kWarps, kTile = S::kTile, kSub = S::kSub;
   extern __shared__ __align__(128) uint8_t sm[];
   uint16_t* sq = reinterpret_cast<uint16_t*>(sm);
   uint8_t* ring = sm + S::kQ;
@@ -121,7 +130,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) attend_rows_kern
   long long mine = 0;
   for (int i = 0; i < per; ++i) {
     const int b = tid * per + i;
-    if (b < p.B) mine += request_tiles<kRows>(p, b);
+    if (b < p.B) mine += request_tiles<kRows, kTile>(p, b);
   }
   long long inc = mine;
   for (int o = 1; o < 32; o <<= 1) {
@@ -144,7 +153,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) attend_rows_kern
     for (int i = 0; i < per; ++i) {
       const int b = tid * per + i;
       if (b >= p.B) break;
-      const long long n = request_tiles<kRows>(p, b);
+      const long long n = request_tiles<kRows, kTile>(p, b);
       if (begin < at + n) {
         first_b = b;
         first_tile = at;
@@ -170,26 +179,93 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) attend_rows_kern
         const int n_rows = min(kRows, rows - r0);
         const int first_pos = base + token_of(p, r0), last_pos = base + token_of(p, r0 + n_rows - 1);
         const Span<kTile> span(first_pos, last_pos, rq.len, p.window, p.sinks);
-        if (req_at + span.tiles <= cur) {
-          req_at += span.tiles;
+        // the item's units: its cost, then its tiles
+        const int units = span.tiles + kItemCost;
+        const int i0 = max(0, int(min((long long)units, cur - req_at)) - kItemCost);
+        const int i1 = max(0, int(min((long long)units, stop - req_at)) - kItemCost);
+        if (i0 >= i1) {
+          req_at += units;
+          cur = max(cur, min(req_at, stop));
           continue;
         }
-        const int i0 = int(cur - req_at), i1 = int(min((long long)span.tiles, stop - req_at));
+
+        // ---- the ring (first, so that its copies are under way while the rows are read)
+        __syncthreads();
+        const int iters = i1 - i0 > warp ? (i1 - i0 - warp + kWarps - 1) / kWarps : 0;
+        const int* table = p.table + (long long)b * p.table_ld;
+        // this lane's places in the first page's codes and pairs of the head; a page further is `stride` bytes of codes
+        const long long head_at = (long long)h << p.c.page_log2;
+        const uint8_t* k_at = p.c.k + head_at * (D / 2) + (D == 64 ? tok0 * 32 + t4 * 8 : tok0 * (D / 2) + t4 * 16);
+        const uint8_t* v_at = p.c.v + head_at * (D / 2) + (t4 * 8 + g) * 16;
+        const uint32_t* kp_at = p.c.k_pair + head_at + tok0;
+        const uint32_t* vp_at = p.c.v_pair + head_at + tok0;
+        const uint32_t stride = uint32_t(p.c.heads << p.c.page_log2) * (D / 2);      // at most 4096 * 256 * 128
+        int pages = -1;              // lane x: the page of 16 tokens x of the next 32 / kSub steps
+        uint32_t bad = 0;            // bit of 16 tokens of a stage: their page is not one of the cache
+        auto load = [&](int k) {
+          if (k < iters) {
+            if (k % (32 / kSub) == 0) {
+              const int kk = k + lane / kSub;
+              pages = -1;
+              if (kk < iters) {
+                const int first = span.id(i0 + warp + kk * kWarps) * kTile + 16 * (lane % kSub);
+                if (first < rq.len) pages = table[first >> p.c.page_log2];
+              }
+            }
+            const int stage = k % S::kStages;
+#pragma unroll
+            for (int s = 0; s < kSub; ++s) {
+              const int page = __shfl_sync(0xffffffffu, pages, (k % (32 / kSub)) * kSub + s);
+              const int first = span.id(i0 + warp + k * kWarps) * kTile + 16 * s;
+              const uint32_t bit = 1u << (stage * kSub + s);
+              if (unsigned(page) < unsigned(p.c.n_pages)) {
+                bad &= ~bit;
+                const uint64_t codes = uint64_t(uint32_t(page)) * stride + uint32_t(first & ((1 << p.c.page_log2) - 1)) * (D / 2);
+                const uint32_t dst = ring_at + stage * S::kStage + s * S::kPart + lane * 16;
+                const uint8_t* kp = k_at + codes;
+                if constexpr (D == 64) {
+                  cp8(dst, kp);
+                  cp8(dst + 8, kp + 64);
+                } else {
+#pragma unroll
+                  for (int i = 0; i < S::kPieces; ++i) cp16(dst + i * 512, kp + (i & 1) * D + (i >> 1) * 64);
+                }
+                const uint8_t* vp = v_at + codes;
+#pragma unroll
+                for (int i = 0; i < D / 64; ++i) cp16(dst + S::kPieces * 512 + i * 512, vp + i * 512);
+                const uint64_t pair = codes / (D / 2);
+                const uint32_t pd = dst + 16 * D;
+                cp4(pd, kp_at + pair);
+                cp4(pd + 4, kp_at + pair + 2);
+                cp4(pd + 8, vp_at + pair);
+                cp4(pd + 12, vp_at + pair + 2);
+              } else {
+                bad |= bit;
+                if (first < rq.len && lane == 0) atomicExch(&g_attend_status, kBadPage);
+              }
+            }
+          }
+          cp_commit();
+        };
+#pragma unroll
+        for (int k = 0; k < S::kStages - 1; ++k) load(k);
 
         // ---- the item's rows as fp16 fragments
-        __syncthreads();
         for (int r = warp; r < kRows; r += kWarps) {
-          float v[D / 32], top = 0.f, sum = 0.f;
-#pragma unroll
-          for (int i = 0; i < D / 32; ++i) v[i] = 0.f;
-          if (r < n_rows) {
+          constexpr int kChunks = D / 8;         // 16-byte chunks: the eight elements of one word of codes
+          uint4 x = make_uint4(0, 0, 0, 0);
+          if (r < n_rows && lane < kChunks) {
             const int tok = token_of(p, r0 + r);
-            const uint16_t* x = p.q + (rq.row0 + tok) * p.q_token + (long long)(h * p.G + r0 + r - tok * p.G) * p.q_head;
-#pragma unroll
-            for (int i = 0; i < D / 32; ++i) v[i] = DType<T>::to_float(x[lane * (D / 32) + i]);
+            x = __ldg(reinterpret_cast<const uint4*>(p.q + (rq.row0 + tok) * p.q_token +
+                                                     (long long)(h * p.G + r0 + r - tok * p.G) * p.q_head) + lane);
           }
+          const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+          float v[8], top = 0.f, sum = 0.f;
 #pragma unroll
-          for (int i = 0; i < D / 32; ++i) top = fmaxf(top, fabsf(v[i])), sum += v[i];
+          for (int e = 0; e < 8; ++e) {
+            v[e] = DType<T>::to_float(uint16_t(u[e >> 1] >> (16 * (e & 1))));
+            top = fmaxf(top, fabsf(v[e])), sum += v[e];
+          }
           for (int o = 16; o; o >>= 1) {
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
             sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -197,21 +273,18 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) attend_rows_kern
           const int ex = int(__float_as_uint(top) >> 23);                // exponent of the largest element
           const int fe = ex == 255 || top == 0.f ? 127 : min(254, 127 + 13 + 127 - ex);
           const float f = __uint_as_float(uint32_t(fe) << 23);
-#pragma unroll
-          for (int i = 0; i < D / 32; ++i) {
-            const int d = lane * (D / 32) + i;
-            const int tig = D == 64 ? d / 16 : (d % 128) / 32, nib = d % 8;
-            const int w = D == 64 ? (d % 16) / 8 : (d / 128) * 4 + (d % 32) / 8;
-            const float x = v[i] * f * (nib & 1 ? 0.0625f : 1.f);
-            sq[((((r >> 3) * S::kWords + w) * 32 + (r & 7) * 4 + tig) * 4 + (nib & 3)) * 2 + (nib >> 2)] =
-                __half_as_ushort(__float2half_rn(x));
+          if (lane < kChunks) {
+            const int tig = D == 64 ? lane / 2 : (lane % 16) / 4, w = D == 64 ? lane % 2 : (lane / 16) * 4 + lane % 4;
+            uint4 o;
+            o.x = half2_of(v[0] * f, v[4] * f), o.y = half2_of(v[1] * f * 0.0625f, v[5] * f * 0.0625f);
+            o.z = half2_of(v[2] * f, v[6] * f), o.w = half2_of(v[3] * f * 0.0625f, v[7] * f * 0.0625f);
+            reinterpret_cast<uint4*>(sq)[((r >> 3) * S::kWords + w) * 32 + (r & 7) * 4 + tig] = o;
           }
           if (lane == 0) row_k[r] = make_float2(p.scale * 16777216.f / f, p.scale * sum);
         }
         __syncthreads();
 
         float qf[NT][2], qs[NT][2], m[NT][2], l[NT][2], pm[NT][2];
-        int pos[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -220,7 +293,6 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) attend_rows_kern
             const float2 k = row_k[r];
             qf[n][e] = k.x, qs[n][e] = k.y;
             m[n][e] = -INFINITY, l[n][e] = 0.f, pm[n][e] = 0.f;
-            pos[n][e] = r < n_rows ? base + token_of(p, r0 + r) : -1;
           }
         float o[NT][D / 16][4];
 #pragma unroll
@@ -236,135 +308,115 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) attend_rows_kern
           for (int e = 0; e < 4; ++e) ws[n][e] = 0.f;
         float sig = 0.f, inv_sig = 0.f;
 
-        // ---- the ring
-        const int iters = i1 - i0 > warp ? (i1 - i0 - warp + kWarps - 1) / kWarps : 0;
-        const int* table = p.table + (long long)b * p.table_ld;
-        int pages = -1;              // lane x: the page of iteration 32 * (k / 32) + x
-        uint32_t bad = 0;            // bit of a stage: its page is not one of the cache
-        auto load = [&](int k) {
-          if (k < iters) {
-            if ((k & 31) == 0) {
-              const int kk = k + lane;
-              pages = -1;
-              if (kk < iters) {
-                const int first = span.id(i0 + warp + kk * kWarps) * kTile;
-                if (first < rq.len) pages = table[first >> p.c.page_log2];
-              }
-            }
-            const int page = __shfl_sync(0xffffffffu, pages, k & 31);
-            const int first = span.id(i0 + warp + k * kWarps) * kTile;
-            const int stage = k % S::kStages;
-            const bool ok = page >= 0 && page < p.c.n_pages;
-            if (ok) {
-              bad &= ~(1u << stage);
-              const int off = first & ((1 << p.c.page_log2) - 1);
-              const long long codes = cache_codes_at(page, h, p.c.heads, p.c.page_log2, D) + (long long)off * (D / 2);
-              const uint32_t dst = ring_at + stage * S::kStage + lane * 16;
-              const uint8_t* kp = p.c.k + codes;
-              if constexpr (D == 64) {
-                cp8(dst, kp + tok0 * 32 + t4 * 8);
-                cp8(dst + 8, kp + (tok0 + 2) * 32 + t4 * 8);
-              } else {
-#pragma unroll
-                for (int i = 0; i < S::kPieces; ++i)
-                  cp16(dst + i * 512, kp + (tok0 + 2 * (i & 1)) * (D / 2) + (i >> 1) * 64 + t4 * 16);
-              }
-              const uint8_t* vp = p.c.v + codes + (t4 * 8 + g) * 16;
-#pragma unroll
-              for (int i = 0; i < D / 64; ++i) cp16(dst + S::kPieces * 512 + i * 512, vp + i * 512);
-              const long long pair = cache_pair_at(page, h, p.c.heads, p.c.page_log2, off) + tok0;
-              const uint32_t pd = dst + 16 * D;
-              cp4(pd, p.c.k_pair + pair);
-              cp4(pd + 4, p.c.k_pair + pair + 2);
-              cp4(pd + 8, p.c.v_pair + pair);
-              cp4(pd + 12, p.c.v_pair + pair + 2);
-            } else {
-              bad |= 1u << stage;
-              if (first < rq.len && lane == 0) atomicExch(&g_attend_status, kBadPage);
-            }
-          }
-          cp_commit();
-        };
-#pragma unroll
-        for (int k = 0; k < S::kStages - 1; ++k) load(k);
-
         for (int k = 0; k < iters; ++k) {
           cp_wait<S::kStages - 2>();
           const int stage = k % S::kStages;
-          const bool missing = (bad >> stage) & 1u;
+          const uint32_t missing = bad >> (stage * kSub);
           load(k + S::kStages - 1);
           const uint32_t at = ring_at + stage * S::kStage + lane * 16;
 
           // ---- scores
-          float acc[NT][2][4];
+          float acc[kSub][NT][2][4];
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
+          for (int s = 0; s < kSub; ++s)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) acc[n][i >> 2][i & 3] = 0.f;
-          const uint4 pr = lds128(at + 16 * D);
-          auto qk = [&](uint32_t x, uint32_t y, int w) {
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int i = 0; i < 8; ++i) acc[s][n][i >> 2][i & 3] = 0.f;
+          // word w of the rows: x and y are those of the lane's two tokens
+          auto qk = [&](int s, uint32_t x, uint32_t y, const uint4 (&q)[NT]) {
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-              const uint4 q = lds128(q_at + (n * S::kWords + w) * 512);
-              mma16(acc[n][0], x & 0x000F000Fu, y & 0x000F000Fu, x & 0x00F000F0u, y & 0x00F000F0u, q.x, q.y);
-              mma16(acc[n][1], (x >> 8) & 0x000F000Fu, (y >> 8) & 0x000F000Fu, (x >> 8) & 0x00F000F0u,
-                    (y >> 8) & 0x00F000F0u, q.z, q.w);
+              mma16(acc[s][n][0], x & 0x000F000Fu, y & 0x000F000Fu, x & 0x00F000F0u, y & 0x00F000F0u, q[n].x, q[n].y);
+              mma16(acc[s][n][1], (x >> 8) & 0x000F000Fu, (y >> 8) & 0x000F000Fu, (x >> 8) & 0x00F000F0u,
+                    (y >> 8) & 0x00F000F0u, q[n].z, q[n].w);
             }
           };
+          auto q_of = [&](uint4 (&q)[NT], int w) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) q[n] = lds128(q_at + (n * S::kWords + w) * 512);
+          };
           if constexpr (D == 64) {
-            const uint4 a = lds128(at);
-            qk(a.x, a.z, 0);
-            qk(a.y, a.w, 1);
+            uint4 a[kSub], q[NT];
+#pragma unroll
+            for (int s = 0; s < kSub; ++s) a[s] = lds128(at + s * S::kPart);
+            q_of(q, 0);
+#pragma unroll
+            for (int s = 0; s < kSub; ++s) qk(s, a[s].x, a[s].z, q);
+            q_of(q, 1);
+#pragma unroll
+            for (int s = 0; s < kSub; ++s) qk(s, a[s].y, a[s].w, q);
           } else {
 #pragma unroll
             for (int i = 0; i < S::kPieces; i += 2) {
-              const uint4 a = lds128(at + i * 512), c = lds128(at + (i + 1) * 512);
-              qk(a.x, c.x, i * 2);
-              qk(a.y, c.y, i * 2 + 1);
-              qk(a.z, c.z, i * 2 + 2);
-              qk(a.w, c.w, i * 2 + 3);
+              uint4 a[kSub], c[kSub], q[NT];
+#pragma unroll
+              for (int s = 0; s < kSub; ++s) a[s] = lds128(at + s * S::kPart + i * 512), c[s] = lds128(at + s * S::kPart + (i + 1) * 512);
+              q_of(q, i * 2);
+#pragma unroll
+              for (int s = 0; s < kSub; ++s) qk(s, a[s].x, c[s].x, q);
+              q_of(q, i * 2 + 1);
+#pragma unroll
+              for (int s = 0; s < kSub; ++s) qk(s, a[s].y, c[s].y, q);
+              q_of(q, i * 2 + 2);
+#pragma unroll
+              for (int s = 0; s < kSub; ++s) qk(s, a[s].z, c[s].z, q);
+              q_of(q, i * 2 + 3);
+#pragma unroll
+              for (int s = 0; s < kSub; ++s) qk(s, a[s].w, c[s].w, q);
             }
           }
 
           // ---- probabilities
           const int first = span.id(i0 + warp + k * kWarps) * kTile;
-          const float2 k0 = lo_step<T>(pr.x), k1 = lo_step<T>(pr.y);
-          float2 v0 = lo_step<T>(pr.z), v1 = lo_step<T>(pr.w);
-          float x[NT][4];
+          float2 v[kSub][2];                     // lo, step of the lane's two tokens
+          float x[kSub][NT][4];
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float2 kk = e < 2 ? k0 : k1;
-              x[n][e] = fmaf(kk.y, (acc[n][0][e] + acc[n][1][e]) * qf[n][e & 1], kk.x * qs[n][e & 1]);
-            }
-          const bool whole = !missing && first + kTile <= first_pos + 1 && first + kTile <= rq.len &&
-                             (p.window == 0 || first > last_pos - p.window || first + kTile <= p.sinks);
-          bool seen0 = true, seen1 = true;       // some row of this lane sees the token
-          uint32_t hidden = 0;
-          if (!whole) {
-            seen0 = seen1 = false;
+          for (int s = 0; s < kSub; ++s) {
+            const uint4 pr = lds128(at + s * S::kPart + 16 * D);
+            const float2 k0 = lo_step<T>(pr.x), k1 = lo_step<T>(pr.y);
+            v[s][0] = lo_step<T>(pr.z), v[s][1] = lo_step<T>(pr.w);
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                const int j = first + tok0 + (e < 2 ? 0 : 2);
-                const bool see = !missing && token_seen(j, pos[n][e & 1], rq.len, p.window, p.sinks);
-                if (!see) x[n][e] = -INFINITY, hidden |= 1u << (4 * n + e);
-                else if (e < 2) seen0 = true;
-                else seen1 = true;
+                const float2 kk = e < 2 ? k0 : k1;
+                x[s][n][e] = fmaf(kk.y, (acc[s][n][0][e] + acc[s][n][1][e]) * qf[n][e & 1], kk.x * qs[n][e & 1]);
               }
-            // what lies in hidden places may be anything, NaN too
-            if (!seen0) v0 = make_float2(0.f, 0.f);
-            if (!seen1) v1 = make_float2(0.f, 0.f);
           }
-          bool grow = fmaxf(v0.y, v1.y) > sig || sig == 0.f;
+          const bool whole = (missing & ((1u << kSub) - 1u)) == 0 && first + kTile <= first_pos + 1 && first + kTile <= rq.len &&
+                             (p.window == 0 || first > last_pos - p.window || first + kTile <= p.sinks);
+          uint32_t hidden = 0;
+          if (!whole) {
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
+            for (int s = 0; s < kSub; ++s) {
+              bool seen[2] = {false, false};     // some row of this lane sees the token
 #pragma unroll
-            for (int e = 0; e < 4; ++e) grow |= x[n][e] > m[n][e & 1] + kLazy;
+              for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const int j = first + 16 * s + tok0 + (e < 2 ? 0 : 2), r = n * 8 + 2 * t4 + (e & 1);
+                  const int pos = r < n_rows ? base + token_of(p, r0 + r) : -1;
+                  if (!((missing >> s) & 1u) && token_seen(j, pos, rq.len, p.window, p.sinks)) seen[e >> 1] = true;
+                  else x[s][n][e] = -INFINITY, hidden |= 1u << ((s * NT + n) * 4 + e);
+                }
+              // what lies in hidden places may be anything, NaN too
+              if (!seen[0]) v[s][0] = make_float2(0.f, 0.f);
+              if (!seen[1]) v[s][1] = make_float2(0.f, 0.f);
+            }
+          }
+          float big = v[0][0].y;                 // largest step
+#pragma unroll
+          for (int s = 0; s < kSub; ++s) big = fmaxf(big, fmaxf(v[s][0].y, v[s][1].y));
+          bool grow = big > sig || sig == 0.f;
+#pragma unroll
+          for (int s = 0; s < kSub; ++s)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) grow |= x[s][n][e] > m[n][e & 1] + kLazy;
           if (__any_sync(0xffffffffu, grow)) {
-            float vs = fmaxf(fmaxf(v0.y, v1.y), kMinStep);
+            float vs = fmaxf(big, kMinStep);
 #pragma unroll
             for (int s = 16; s; s >>= 1) vs = fmaxf(vs, __shfl_xor_sync(0xffffffffu, vs, s));
             const float sig_new = fmaxf(sig, pow2_above(vs));
@@ -375,7 +427,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) attend_rows_kern
             for (int n = 0; n < NT; ++n)
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
-                float top = fmaxf(x[n][e], x[n][e + 2]);
+                float top = fmaxf(x[0][n][e], x[0][n][e + 2]);
+                if constexpr (kSub == 2) top = fmaxf(top, fmaxf(x[kSub - 1][n][e], x[kSub - 1][n][e + 2]));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
@@ -390,43 +443,47 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) attend_rows_kern
                 ws[n][e] *= ab;
               }
           }
-          uint32_t bf[NT][2];
+          uint32_t bf[kSub][NT][2];
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            float w[4];
+          for (int s = 0; s < kSub; ++s)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float2 vv = e < 2 ? v0 : v1;
-              const float mm = m[n][e & 1];
-              const float pr_ = ex2(x[n][e] - (mm == -INFINITY ? 0.f : mm));
-              const bool none = (hidden >> (4 * n + e)) & 1u;
-              l[n][e & 1] += pr_;
-              pm[n][e & 1] += none ? 0.f : pr_ * fmaf(7.5f, vv.y, vv.x);
-              w[e] = none ? 0.f : pr_ * (vv.y * inv_sig);
+            for (int n = 0; n < NT; ++n) {
+              float w[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float2 vv = v[s][e >> 1];
+                const float mm = m[n][e & 1];
+                const float pr = ex2(x[s][n][e] - (mm == -INFINITY ? 0.f : mm));
+                const bool none = (hidden >> ((s * NT + n) * 4 + e)) & 1u;
+                l[n][e & 1] += pr;
+                pm[n][e & 1] += none ? 0.f : pr * fmaf(7.5f, vv.y, vv.x);
+                w[e] = none ? 0.f : pr * (vv.y * inv_sig);
+              }
+              bf[s][n][0] = transpose8x8(half2_of(w[0], w[1]));
+              bf[s][n][1] = transpose8x8(half2_of(w[2], w[3]));
+              mma16(ws[n], kOnes, kOnes, kOnes, kOnes, bf[s][n][0], bf[s][n][1]);
             }
-            bf[n][0] = transpose8x8(half2_of(w[0], w[1]));
-            bf[n][1] = transpose8x8(half2_of(w[2], w[3]));
-            mma16(ws[n], kOnes, kOnes, kOnes, kOnes, bf[n][0], bf[n][1]);
-          }
 
           // ---- values
 #pragma unroll
-          for (int i = 0; i < D / 64; ++i) {
-            const uint4 v = lds128(at + S::kPieces * 512 + i * 512);
-            uint32_t x01 = __byte_perm(v.x, v.y, 0x5410), y01 = __byte_perm(v.x, v.y, 0x7632);
-            uint32_t x23 = __byte_perm(v.z, v.w, 0x5410), y23 = __byte_perm(v.z, v.w, 0x7632);
+          for (int i = 0; i < D / 64; ++i)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
+            for (int s = 0; s < kSub; ++s) {
+              const uint4 c = lds128(at + s * S::kPart + S::kPieces * 512 + i * 512);
+              uint32_t x01 = __byte_perm(c.x, c.y, 0x5410), y01 = __byte_perm(c.x, c.y, 0x7632);
+              uint32_t x23 = __byte_perm(c.z, c.w, 0x5410), y23 = __byte_perm(c.z, c.w, 0x7632);
 #pragma unroll
-              for (int n = 0; n < NT; ++n) {
-                mma16(o[n][i * 4 + 2 * j], x01 & 0x000F000Fu, y01 & 0x000F000Fu, x23 & 0x000F000Fu, y23 & 0x000F000Fu,
-                      bf[n][0], bf[n][1]);
-                mma16(o[n][i * 4 + 2 * j + 1], x01 & 0x00F000F0u, y01 & 0x00F000F0u, x23 & 0x00F000F0u,
-                      y23 & 0x00F000F0u, bf[n][0], bf[n][1]);
+              for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                  mma16(o[n][i * 4 + 2 * j], x01 & 0x000F000Fu, y01 & 0x000F000Fu, x23 & 0x000F000Fu, y23 & 0x000F000Fu,
+                        bf[s][n][0], bf[s][n][1]);
+                  mma16(o[n][i * 4 + 2 * j + 1], x01 & 0x00F000F0u, y01 & 0x00F000F0u, x23 & 0x00F000F0u,
+                        y23 & 0x00F000F0u, bf[s][n][0], bf[s][n][1]);
+                }
+                x01 >>= 8, y01 >>= 8, x23 >>= 8, y23 >>= 8;
               }
-              x01 >>= 8, y01 >>= 8, x23 >>= 8, y23 >>= 8;
             }
-          }
         }
         cp_wait<0>();
 
@@ -483,89 +540,93 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) attend_rows_kern
           }
         }
         if (starts && !ends && tid == 0) {
-          const long long last = (req_at + span.tiles - 1) / share;
-          p.meta[blockIdx.x] = make_int4(int(last), b, h, r0 / kRows);
+          const long long last = (req_at + units - 1) / share;
+          p.meta[blockIdx.x] = joined_item(p, int(last), rq, h, r0, n_rows);
         }
-        req_at += span.tiles;
+        req_at += units;
         cur = min(req_at, stop);
       }
     }
   }
 }
 
-// Joins the parts of the item that block blockIdx.x began and others went on with. `Ways` warps share a row: each
-// adds every Ways-th part, then the first adds the warps' sums in their order.
+// Joins the parts of the item that block blockIdx.x began and others went on with (at most kRows rows). With many
+// parts all warps of the block share a row: each adds every eighth part, then the first adds the warps' sums in their
+// order; with few a warp has a row to itself.
 constexpr int kJoinWarps = 8;
-template <typename T, int D, int kRows, int Ways>
+template <typename T, int D, int kRows>
 __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const __grid_constant__ AttendParams p) {
   constexpr int kPer = D / 32;
   __shared__ float part[kJoinWarps][D + 2];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int4 meta = p.meta[blockIdx.x];
   if (meta.x == 0) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, way = warp % Ways;
-  const int c0 = blockIdx.x, c1 = meta.x, b = meta.y, h = meta.z, r = blockIdx.y * (kJoinWarps / Ways) + warp / Ways;
-  const Request rq = request_of(p, b);
-  const int row = meta.w * kRows + r;
-  if (row - r + int(blockIdx.y) * (kJoinWarps / Ways) >= rq.rows * p.G) return;      // none of the block's rows
-  const bool live = row < rq.rows * p.G;
-  auto slot = [&](int c) { return (c == c0 ? 2LL * c + 1 : 2LL * c) * kRows + r; };
-  float top = -INFINITY, sum = 0.f, x[kPer];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n_rows = (meta.w & 127) + 1;
+  const int c0 = blockIdx.x, c1 = meta.x, ways = c1 - c0 >= 16 ? kJoinWarps : 1, step = kJoinWarps / ways, way = warp / step;
+  const int h = meta.w >> 13, rem = (meta.w >> 7) & 63;
+  for (int first = blockIdx.y * step; first < n_rows; first += gridDim.y * step) {
+    const int r = first + warp % step;
+    const bool live = r < n_rows;
+    auto slot = [&](int c) { return (c == c0 ? 2LL * c + 1 : 2LL * c) * kRows + r; };
+    float top = -INFINITY, sum = 0.f, x[kPer];
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) x[i] = 0.f;
-  if (live) {
-    for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, p.part_ml[slot(c)].x);
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    for (int i = 0; i < kPer; ++i) x[i] = 0.f;
+    if (live) {
+      for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, p.part_ml[slot(c)].x);
+      for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
 #pragma unroll 4
-    for (int c = c0 + way; c <= c1; c += Ways) {
-      const float2 ml = p.part_ml[slot(c)];
-      const float* o = p.part_o + slot(c) * D + lane * kPer;
-      float v[kPer];
+      for (int c = c0 + way; c <= c1; c += ways) {
+        const float2 ml = p.part_ml[slot(c)];
+        const float* o = p.part_o + slot(c) * D + lane * kPer;
+        float v[kPer];
 #pragma unroll
-      for (int i = 0; i < kPer; i += 2) {
-        const float2 y = *reinterpret_cast<const float2*>(o + i);
-        v[i] = y.x, v[i + 1] = y.y;
+        for (int i = 0; i < kPer; i += 2) {
+          const float2 y = *reinterpret_cast<const float2*>(o + i);
+          v[i] = y.x, v[i + 1] = y.y;
+        }
+        const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : ex2(ml.x - top);
+        sum = fmaf(ml.y, f, sum);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) x[i] = fmaf(v[i], f, x[i]);
       }
-      const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : ex2(ml.x - top);
-      sum = fmaf(ml.y, f, sum);
+    }
+    if (ways > 1) {
+      __syncthreads();
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) x[i] = fmaf(v[i], f, x[i]);
+      for (int i = 0; i < kPer; ++i) part[warp][lane * kPer + i] = x[i];
+      if (lane == 0) part[warp][D] = sum;
+      __syncthreads();
+      if (way == 0)
+        for (int w = 1; w < ways; ++w) {
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) x[i] += part[warp + w * step][lane * kPer + i];
+          sum += part[warp + w * step][D];
+        }
+    }
+    if (live && way == 0) {
+      const int at = token_of(p, rem + r), head = h * p.G + rem + r - at * p.G, d = lane * kPer;
+      const long long tok = meta.y + at;
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      uint32_t* to = reinterpret_cast<uint32_t*>(p.out + tok * p.out_token + (long long)head * p.out_head + d);
+#pragma unroll
+      for (int i = 0; i < kPer; i += 2)
+        to[i / 2] = uint32_t(DType<T>::from_float(gated<T>(x[i] * inv, p, tok, head, d + i))) |
+                    (uint32_t(DType<T>::from_float(gated<T>(x[i + 1] * inv, p, tok, head, d + i + 1))) << 16);
     }
   }
-  if constexpr (Ways > 1) {
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) part[warp][lane * kPer + i] = x[i];
-    if (lane == 0) part[warp][D] = sum;
-    __syncthreads();
-    if (way != 0) return;
-    for (int w = 1; w < Ways; ++w) {
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) x[i] += part[warp + w][lane * kPer + i];
-      sum += part[warp + w][D];
-    }
-  }
-  if (!live) return;
-  const int at = token_of(p, row), head = h * p.G + row - at * p.G, d = lane * kPer;
-  const long long tok = rq.row0 + at;
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  uint32_t* to = reinterpret_cast<uint32_t*>(p.out + tok * p.out_token + (long long)head * p.out_head + d);
-#pragma unroll
-  for (int i = 0; i < kPer; i += 2)
-    to[i / 2] = uint32_t(DType<T>::from_float(gated<T>(x[i] * inv, p, tok, head, d + i))) |
-                (uint32_t(DType<T>::from_float(gated<T>(x[i + 1] * inv, p, tok, head, d + i + 1))) << 16);
 }
 
-template <typename T, int D, int kRows, int Ways>
-int join(const AttendParams& p, int blocks, cudaStream_t st) {
+template <typename T, int D, int kRows>
+int join(const AttendParams& p, int blocks, int blocks_a_item, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(blocks), kRows * Ways / kJoinWarps);
+  cfg.gridDim = dim3(unsigned(blocks), unsigned(blocks_a_item));
   cfg.blockDim = dim3(kJoinWarps * 32);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr, cfg.numAttrs = 1;
-  B200LUT_CUDA_OK(cudaLaunchKernelEx(&cfg, attend_join_kernel<T, D, kRows, Ways>, p));
+  B200LUT_CUDA_OK(cudaLaunchKernelEx(&cfg, attend_join_kernel<T, D, kRows>, p));
   return B200LUT_OK;
 }
 
@@ -579,14 +640,13 @@ int launch(AttendParams p, int blocks, cudaStream_t st) {
     B200LUT_CUDA_OK(cudaFuncSetAttribute(attend_rows_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
     if (dev < 64) configured[dev] = true;
   }
-  attend_rows_kernel<T, D, NT><<<unsigned(blocks), kWarps * 32, S::kSmem, st>>>(p);
+  attend_rows_kernel<T, D, NT><<<unsigned(blocks), S::kWarps * 32, S::kSmem, st>>>(p);
   B200LUT_CUDA_OK(cudaGetLastError());
-  return join<T, D, S::kRows, 8>(p, blocks, st);
+  return join<T, D, S::kRows>(p, blocks, 4, st);
 }
 
-// Blocks: two per SM with eight rows (fewer rows than that leave SMs without enough loads in flight), one with 16.
-int row_blocks(int sms, int G) { return G <= 8 ? 2 * sms : sms; }
 int rows_of(int G) { return G <= 8 ? 8 : 16; }
+int row_blocks(int sms, int G) { return G <= 8 ? 2 * sms : sms; }      // Shape::kBlocks
 
 // Workspace of a launch over `blocks` blocks of `rows` rows: what attend_*_kernel leave to the join.
 size_t workspace_of(int blocks, int rows, int D) { return size_t(blocks) * (16 + 2 * size_t(rows) * (8 + size_t(D) * 4)); }
@@ -606,7 +666,7 @@ int run(AttendParams p, int sms, void* ws, cudaStream_t st) {
     AttendParams t = p;
     lay_out(&t, static_cast<char*>(ws) + workspace_of(blocks, rows, D), sms, 128);
     int rc = attend_tiles(t, DType<T>::id, sms, st);
-    if (rc == B200LUT_OK) rc = join<T, D, 128, 1>(t, sms, st);
+    if (rc == B200LUT_OK) rc = join<T, D, 128>(t, sms, 16, st);
     if (rc != B200LUT_OK) return rc;
   }
   lay_out(&p, ws, blocks, rows);

@@ -61,6 +61,13 @@ __device__ __forceinline__ Request request_of(const AttendParams& p, int b) {
   return r;
 }
 
+// What the join has to know of an item that a block began: the last block of it, the row of q of the item's first row's
+// token, and packed: rows - 1, how far the first row is into its token's query heads, key/value head.
+__device__ __forceinline__ int4 joined_item(const AttendParams& p, int last, const Request& rq, int h, int r0, int n_rows) {
+  const int tok = token_of(p, r0);
+  return make_int4(last, rq.row0 + tok, 0, (n_rows - 1) | ((r0 - tok * p.G) << 7) | (h << 13));
+}
+
 // Tiles of kTile tokens that rows at positions [first, last] of a request see: ids 0 .. sink_tiles - 1, then from
 // main0 on. At least one, so that a row that sees nothing is written.
 template <int kTile>

@@ -29,6 +29,9 @@ constexpr int kValueWarp = 8, kKeyWarp = 16, kParamWarp = 20, kProductWarp = 21;
 // unpacking warps are many because one warp issues an instruction in six to seven cycles at best here.
 constexpr int kSoftmaxRegs = 128, kOtherRegs = 56;
 constexpr int kParamStages = 4;
+// What an item costs a block besides its tiles, in tiles (its rows, filling the pipeline, its result), counted in the
+// shares: an item's units are its cost, then its tiles.
+constexpr int kItemCost = 4;
 constexpr float kLazy = 8.f;
 constexpr float kMinStep = 7.888609e-31f;   // 2^-100
 constexpr int kBadPage = 0x6200;
@@ -199,7 +202,7 @@ __device__ __forceinline__ Span<kTile> span_of(const AttendParams& p, const Requ
 __device__ __forceinline__ long long head_tiles(const AttendParams& p, const Request& r, int lane) {
   const int n = (r.rows * p.G + kRows - 1) / kRows;
   long long sum = 0;
-  for (int i = lane; i < n; i += 32) sum += span_of(p, r, i * kRows).tiles;
+  for (int i = lane; i < n; i += 32) sum += span_of(p, r, i * kRows).tiles + kItemCost;
   for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   return sum;
 }
@@ -219,18 +222,18 @@ struct Work {
 // The part that starts at tile `cur` of the line; b, h, rt, rq and item_at say where that is.
 __device__ __forceinline__ void open_part(const AttendParams& p, Work* w, long long cur, long long stop) {
   w->span = span_of(p, w->rq, w->rt * kRows);
-  w->i0 = int(cur - w->item_at), w->i1 = int(min((long long)w->span.tiles, stop - w->item_at));
+  const int units = w->span.tiles + kItemCost;
+  w->i0 = max(0, int(cur - w->item_at) - kItemCost), w->i1 = int(min((long long)units, stop - w->item_at)) - kItemCost;
   w->count = w->i1 - w->i0;
   w->r0 = w->rt * kRows;
   w->n_rows = min(kRows, w->rq.rows * p.G - w->r0);
   w->base = w->rq.len - w->rq.rows;
   w->first_pos = w->base + token_of(p, w->r0), w->last_pos = w->base + token_of(p, w->r0 + w->n_rows - 1);
-  w->more = w->item_at + w->i1 < stop;
+  w->more = w->item_at + units + kItemCost < stop;             // a tile of the next item
 }
 __device__ __forceinline__ void next_part(const AttendParams& p, Work* w, long long stop) {
-  const long long cur = w->item_at + w->i1;
   w->n0 += uint32_t(w->count);
-  w->item_at += w->span.tiles;
+  w->item_at += w->span.tiles + kItemCost;
   if ((w->rt + 1) * kRows < w->rq.rows * p.G) {
     ++w->rt;
   } else {
@@ -241,7 +244,7 @@ __device__ __forceinline__ void next_part(const AttendParams& p, Work* w, long l
       while (w->rq.rows == 0);
     }
   }
-  open_part(p, w, cur, stop);
+  open_part(p, w, w->item_at, stop);
 }
 
 template <typename T, int D>
@@ -292,7 +295,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
     if (w < warp) before += scan[w];
     total += scan[w];
   }
-  const long long share = max(1LL, (total + gridDim.x - 1) / gridDim.x);
+  const long long share = max((long long)kItemCost + 1, (total + gridDim.x - 1) / gridDim.x);      // a tile at least
   const long long begin = share * blockIdx.x, stop = min(total, begin + share);
   if (begin >= stop) return;
   if (begin >= before && begin < before + mine) {
@@ -341,7 +344,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
     const int n = (rq.rows * p.G + kRows - 1) / kRows;
     int rt = 0;
     for (int c0 = 0; c0 < n; c0 += 32) {
-      const long long tiles = c0 + lane < n ? span_of(p, rq, (c0 + lane) * kRows).tiles : 0;
+      const long long tiles = c0 + lane < n ? span_of(p, rq, (c0 + lane) * kRows).tiles + kItemCost : 0;
       long long inc = tiles;
       for (int o = 1; o < 32; o <<= 1) {
         const long long v = __shfl_up_sync(0xffffffffu, inc, o);
@@ -684,7 +687,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
       }
       if (!(starts && ends) && !half) p.part_ml[slot * kRows + r] = make_float2(row_m[r], l);
       if (starts && !ends && tid == 0)
-        p.meta[blockIdx.x] = make_int4(int((w.item_at + w.span.tiles - 1) / share), w.b, w.h, w.rt);
+        p.meta[blockIdx.x] = joined_item(p, int((w.item_at + w.span.tiles + kItemCost - 1) / share), w.rq, w.h, w.r0, w.n_rows);
       tc::fence_before_sync();
     });
   } else if (warp < kKeyWarp) {
