@@ -164,7 +164,11 @@ attend_rows_kernel(const __grid_constant__ AttendParams p) {
   }
   __syncthreads();
   if (tid == 0) p.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
-  if (begin >= stop) return;
+  // A launch behind the tile kernel's may run beside its end; the join, which waits for this kernel, needs both complete.
+  if (begin >= stop) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    return;
+  }
 
   const uint32_t ring_at = uint32_t(__cvta_generic_to_shared(ring + warp * S::kRing));
   const uint32_t q_at = uint32_t(__cvta_generic_to_shared(sq)) + lane * 16;
@@ -548,41 +552,55 @@ attend_rows_kernel(const __grid_constant__ AttendParams p) {
       }
     }
   }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
-// Joins the parts of the item that block blockIdx.x began and others went on with (at most kRows rows). With many
-// parts all warps of the block share a row: each adds every eighth part, then the first adds the warps' sums in their
-// order; with few a warp has a row to itself.
+// What a kernel left to be joined: `blocks` blocks with items of at most `rows` rows, `per` blocks of the join each.
+struct JoinSide {
+  const int4* meta;
+  const float2* ml;
+  const float* o;
+  int blocks, rows, per;
+};
+
+// Joins the parts of the items that a block began and others went on with. With many parts all warps of a block share a
+// row: each adds every eighth part, then the first adds the warps' sums in their order; with few a warp has a row to
+// itself.
 constexpr int kJoinWarps = 8;
-template <typename T, int D, int kRows>
-__global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const __grid_constant__ AttendParams p) {
+template <typename T, int D>
+__global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const __grid_constant__ AttendParams p,
+                                                                      const JoinSide first_side, const JoinSide second_side) {
   constexpr int kPer = D / 32;
   __shared__ float part[kJoinWarps][D + 2];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int4 meta = p.meta[blockIdx.x];
+  const int cut = first_side.blocks * first_side.per;
+  const bool second = int(blockIdx.x) >= cut;
+  const JoinSide& side = second ? second_side : first_side;
+  const int id = int(blockIdx.x) - (second ? cut : 0), c0 = id / side.per, y = id % side.per;
+  const int4 meta = side.meta[c0];
   if (meta.x == 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n_rows = (meta.w & 127) + 1;
-  const int c0 = blockIdx.x, c1 = meta.x, ways = c1 - c0 >= 16 ? kJoinWarps : 1, step = kJoinWarps / ways, way = warp / step;
+  const int c1 = meta.x, ways = c1 - c0 >= 16 ? kJoinWarps : 1, step = kJoinWarps / ways, way = warp / step;
   const int h = meta.w >> 13, rem = (meta.w >> 7) & 63;
-  for (int first = blockIdx.y * step; first < n_rows; first += gridDim.y * step) {
+  for (int first = y * step; first < n_rows; first += side.per * step) {
     const int r = first + warp % step;
     const bool live = r < n_rows;
-    auto slot = [&](int c) { return (c == c0 ? 2LL * c + 1 : 2LL * c) * kRows + r; };
+    auto slot = [&](int c) { return (c == c0 ? 2LL * c + 1 : 2LL * c) * side.rows + r; };
     float top = -INFINITY, sum = 0.f, x[kPer];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) x[i] = 0.f;
     if (live) {
-      for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, p.part_ml[slot(c)].x);
+      for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, side.ml[slot(c)].x);
       for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
 #pragma unroll 4
       for (int c = c0 + way; c <= c1; c += ways) {
-        const float2 ml = p.part_ml[slot(c)];
-        const float* o = p.part_o + slot(c) * D + lane * kPer;
+        const float2 ml = side.ml[slot(c)];
+        const float* o = side.o + slot(c) * D + lane * kPer;
         float v[kPer];
 #pragma unroll
         for (int i = 0; i < kPer; i += 2) {
-          const float2 y = *reinterpret_cast<const float2*>(o + i);
-          v[i] = y.x, v[i + 1] = y.y;
+          const float2 z = *reinterpret_cast<const float2*>(o + i);
+          v[i] = z.x, v[i + 1] = z.y;
         }
         const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : ex2(ml.x - top);
         sum = fmaf(ml.y, f, sum);
@@ -616,22 +634,21 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const __gr
   }
 }
 
-template <typename T, int D, int kRows>
-int join(const AttendParams& p, int blocks, int blocks_a_item, cudaStream_t st) {
+// A launch that may begin before the one in front of it has ended.
+template <typename... P>
+int launch_behind(void (*kernel)(P...), unsigned grid, unsigned threads, size_t smem, cudaStream_t st, const P&... args) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(blocks), unsigned(blocks_a_item));
-  cfg.blockDim = dim3(kJoinWarps * 32);
-  cfg.stream = st;
+  cfg.gridDim = dim3(grid), cfg.blockDim = dim3(threads), cfg.dynamicSmemBytes = smem, cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr, cfg.numAttrs = 1;
-  B200LUT_CUDA_OK(cudaLaunchKernelEx(&cfg, attend_join_kernel<T, D, kRows>, p));
+  B200LUT_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, args...));
   return B200LUT_OK;
 }
 
 template <typename T, int D, int NT>
-int launch(AttendParams p, int blocks, cudaStream_t st) {
+int launch(const AttendParams& p, int blocks, bool behind, cudaStream_t st) {
   using S = Shape<D, NT>;
   static bool configured[64] = {false};
   int dev = 0;
@@ -640,9 +657,10 @@ int launch(AttendParams p, int blocks, cudaStream_t st) {
     B200LUT_CUDA_OK(cudaFuncSetAttribute(attend_rows_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
     if (dev < 64) configured[dev] = true;
   }
+  if (behind) return launch_behind(attend_rows_kernel<T, D, NT>, unsigned(blocks), S::kWarps * 32, S::kSmem, st, p);
   attend_rows_kernel<T, D, NT><<<unsigned(blocks), S::kWarps * 32, S::kSmem, st>>>(p);
   B200LUT_CUDA_OK(cudaGetLastError());
-  return join<T, D, S::kRows>(p, blocks, 4, st);
+  return B200LUT_OK;
 }
 
 int rows_of(int G) { return G <= 8 ? 8 : 16; }
@@ -659,18 +677,24 @@ void lay_out(AttendParams* p, void* ws, int blocks, int rows) {
 template <typename T, int D>
 int run(AttendParams p, int sms, void* ws, cudaStream_t st) {
   const int blocks = row_blocks(sms, p.G), rows = rows_of(p.G);
+  JoinSide tiles = {nullptr, nullptr, nullptr, 0, 128, 16};
   p.rows_limit = INT_MAX;
   if (p.row_start) {
-    // requests of many rows first, on the tensor cores; the others' launch follows
+    // requests of many rows first, on the tensor cores; the others' launch follows on their heels
     p.rows_limit = rows;
     AttendParams t = p;
     lay_out(&t, static_cast<char*>(ws) + workspace_of(blocks, rows, D), sms, 128);
-    int rc = attend_tiles(t, DType<T>::id, sms, st);
-    if (rc == B200LUT_OK) rc = join<T, D, 128>(t, sms, 16, st);
+    const int rc = attend_tiles(t, DType<T>::id, sms, st);
     if (rc != B200LUT_OK) return rc;
+    tiles.meta = t.meta, tiles.ml = t.part_ml, tiles.o = t.part_o, tiles.blocks = sms;
   }
   lay_out(&p, ws, blocks, rows);
-  return rows == 8 ? launch<T, D, 1>(p, blocks, st) : launch<T, D, 2>(p, blocks, st);
+  const bool behind = p.row_start != nullptr;
+  const int rc = rows == 8 ? launch<T, D, 1>(p, blocks, behind, st) : launch<T, D, 2>(p, blocks, behind, st);
+  if (rc != B200LUT_OK) return rc;
+  const JoinSide side = {p.meta, p.part_ml, p.part_o, blocks, rows, 4};
+  return launch_behind(attend_join_kernel<T, D>, unsigned(side.blocks * side.per + tiles.blocks * tiles.per), kJoinWarps * 32, 0,
+                       st, p, side, tiles);
 }
 
 template <typename T>

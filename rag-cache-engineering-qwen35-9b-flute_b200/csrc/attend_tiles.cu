@@ -31,7 +31,7 @@ constexpr int kSoftmaxRegs = 128, kOtherRegs = 56;
 constexpr int kParamStages = 4;
 // What an item costs a block besides its tiles, in tiles (its rows, filling the pipeline, its result), counted in the
 // shares: an item's units are its cost, then its tiles.
-constexpr int kItemCost = 4;
+constexpr int kItemCost = 7;
 constexpr float kLazy = 8.f;
 constexpr float kMinStep = 7.888609e-31f;   // 2^-100
 constexpr int kBadPage = 0x6200;
