@@ -40,6 +40,16 @@ inline bool ints(const at::Tensor& t, int device, int64_t n) {
 
 inline const int32_t* i32(const at::Tensor& t) { return static_cast<const int32_t*>(t.const_data_ptr()); }
 
+// n elements of `st` of base's memory, from byte `at` on (a dispatched view costs several times as much).
+inline at::Tensor piece(const at::Tensor& base, at::ScalarType st, int64_t at, int64_t n) {
+  const auto type = c10::scalarTypeToTypeMeta(st);
+  at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(base.storage()), base.key_set(), type);
+  c10::TensorImpl* impl = t.unsafeGetTensorImpl();
+  impl->set_storage_offset(at / int64_t(type.itemsize()));
+  impl->set_sizes_contiguous({n});
+  return t;
+}
+
 template <size_t N>
 PyObject* tuple_of(at::Tensor (&ts)[N]) {
   PyObject* r = PyTuple_New(N);
@@ -218,8 +228,12 @@ PyObject* kv_plan(Guard&& guarded, Context&& context, PyObject* const* a, Py_ssi
     at::Tensor out[6];
     {
       const WithoutGil free;
-      const int64_t sizes[6] = {B + 1, B, room, room, 1, B};
-      for (int i = 0; i < 6; ++i) out[i] = empty({sizes[i]}, i == 5 ? at::kBool : at::kInt, device);
+      // row_start, kv_len, positions, slots, taken, served: pieces of one allocation, 16-byte aligned
+      const int64_t sizes[6] = {4 * (B + 1), 4 * B, 4 * room, 4 * room, 4, B};
+      int64_t at[7] = {0};
+      for (int i = 0; i < 6; ++i) at[i + 1] = (at[i] + sizes[i] + 15) / 16 * 16;
+      const at::Tensor base = empty({at[6]}, at::kByte, device);
+      for (int i = 0; i < 6; ++i) out[i] = piece(base, i == 5 ? at::kBool : at::kInt, at[i], i == 5 ? B : sizes[i] / 4);
       auto p = [&](int i) { return static_cast<int32_t*>(out[i].mutable_data_ptr()); };
       b200lut_kv_plan_args g = {i32(*t[0]), i32(*t[1]), static_cast<int32_t*>(t[2]->mutable_data_ptr()), i32(*t[3]), i32(*t[4]),
                                 p(0), p(1), p(2), p(3), p(4), static_cast<uint8_t*>(out[5].mutable_data_ptr()), int(B),

@@ -117,85 +117,146 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Plan
 
 // ---- rows in ------------------------------------------------------------------------------------------
 // A row is D/8 lanes of eight elements: two shuffle reductions give lo and hi, then each lane writes the one
-// 32-bit word of codes its elements make. 15 (x - lo) / (hi - lo) is an IEEE division: codes on a border
-// (frequent with 8-bit significands) are decided as the definition does, half to even. Bound by memory: the
-// rows are read once.
-constexpr int kRowWarps = 8;
+// 32-bit word of codes its elements make. A warp takes the rows of U consecutive tokens, all loaded before the first is
+// worked on; four tokens whose slots are neighbours (a prompt's) make 16-byte stores of the values. Bound by memory:
+// rows are read once, codes written once.
+constexpr int kRowWarps = 4;
 constexpr float kRangeLimit = 1.329227996e36f;     // 2^120: 15 times a range below it is finite
 
-template <typename T>
-__global__ void __launch_bounds__(kRowWarps * 32) kv_write_kernel(const uint16_t* k, const uint16_t* v, long long kt,
-                                                                  long long kh, long long vt, long long vh,
-                                                                  const int* slots, int tokens, CacheView c) {
+// rint(a / w) for 0 <= a <= 15 w, half to even: c is at most one off, the remainder a - c w is exact (c w and a
+// are multiples of one unit that is at least 2^-24 of it), so codes on a border, frequent with eight-bit
+// significands, are decided as the definition does. Adding 1.5 * 2^23 rounds and leaves the integer in the low bits;
+// rintf, the conversion and the IEEE division are the slow instructions of the obvious form (62 us instead of 27 for
+// 16384 tokens x 4 heads of 256, keys and values).
+__device__ __forceinline__ uint32_t code_of(float a, float w, float inv) {
+  const float m = fmaf(a, inv, 12582912.f), rem = fmaf(12582912.f - m, w, a), twice = 2.f * fabsf(rem);
+  const uint32_t n = __float_as_uint(m);
+  return (twice > w || (twice == w && (n & 1u)) ? (rem > 0.f ? n + 1u : n - 1u) : n) & 15u;
+}
+
+template <typename T, int U>
+__global__ void __launch_bounds__(kRowWarps * 32) kv_write_kernel(const uint16_t* __restrict__ k, const uint16_t* __restrict__ v,
+                                                                  long long kt, long long kh, long long vt, long long vh,
+                                                                  const int* __restrict__ slots, int tokens, CacheView c) {
   const int lane = threadIdx.x & 31, lanes = c.D >> 3, per = 32 / lanes, at = lane % lanes;
+  const int groups = (tokens + U - 1) / U;
   const long long row = ((long long)blockIdx.x * kRowWarps + (threadIdx.x >> 5)) * per + lane / lanes;
-  const long long rows = (long long)tokens * c.heads * 2;
-  const bool in = row < rows;
-  const bool value = row >= rows / 2;
-  const long long r = in ? (value ? row - rows / 2 : row) : 0;
-  const long long t = r / c.heads;
-  const int h = int(r - t * c.heads);
-  const int slot = in ? slots[t] : -1;
-  uint4 raw = make_uint4(0, 0, 0, 0);
-  if (slot >= 0) raw = __ldg(reinterpret_cast<const uint4*>(value ? v + t * vt + h * vh : k + t * kt + h * kh) + at);
-  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-  float x[8];
+  const long long half = (long long)groups * c.heads;
+  const bool in = row < 2 * half, value = row >= half;
+  const long long r = in ? (value ? row - half : row) : 0;
+  const int group = int(r / c.heads), h = int(r - (long long)group * c.heads), t0 = group * U;
+  int slot[U];
+  uint4 raw[U];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = DType<T>::to_float(uint16_t(w[e >> 1] >> (16 * (e & 1))));
-  float lo = x[0], hi = x[0], bad = x[0] - x[0];         // 0, or NaN where an element is not finite
+  for (int u = 0; u < U; ++u) {
+    const int t = t0 + u;
+    slot[u] = -1;
+    raw[u] = make_uint4(0, 0, 0, 0);
+    if (in && t < tokens) {
+      slot[u] = slots[t];
+      const uint16_t* x = value ? v + t * vt + h * vh : k + t * kt + h * kh;
+      raw[u] = __ldg(reinterpret_cast<const uint4*>(x) + at);
+    }
+  }
+  uint32_t word[U], pair[U];
 #pragma unroll
-  for (int e = 1; e < 8; ++e) lo = fminf(lo, x[e]), hi = fmaxf(hi, x[e]), bad += x[e] - x[e];
-  for (int o = lanes >> 1; o; o >>= 1) {
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    bad += __shfl_xor_sync(0xffffffffu, bad, o);
-  }
-  const float range = hi - lo;
-  const bool finite = bad == 0.f && range < kRangeLimit;
-  uint32_t word = 0;
-  if (finite && range > 0.f) {
+  for (int u = 0; u < U; ++u) {
+    const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+    float x[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) word |= uint32_t(rintf(__fdiv_rn(15.f * (x[e] - lo), range))) << (4 * e);
+    for (int e = 0; e < 8; ++e) x[e] = DType<T>::to_float(uint16_t(w[e >> 1] >> (16 * (e & 1))));
+    float lo = x[0], hi = x[0], bad = x[0] - x[0];         // 0, or NaN where an element is not finite
+#pragma unroll
+    for (int e = 1; e < 8; ++e) lo = fminf(lo, x[e]), hi = fmaxf(hi, x[e]), bad += x[e] - x[e];
+    for (int o = lanes >> 1; o; o >>= 1) {
+      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    }
+    // the lanes of this row that hold one
+    const uint32_t odd = __ballot_sync(0xffffffffu, bad != 0.f) & ((lanes == 32 ? ~0u : (1u << lanes) - 1u) << (lane - at));
+    const float range = hi - lo;
+    const bool finite = odd == 0 && range < kRangeLimit;
+    word[u] = 0;
+    if (finite && range > 0.f) {
+      // scaled by a power of two that keeps 1 / range and the products normal
+      const float up = range < 1e-30f ? 1.329227996e36f : 1.f, width = range * up, inv = 1.f / width;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) word[u] |= code_of(15.f * (x[e] - lo) * up, width, inv) << (4 * e);
+    }
+    pair[u] = finite ? uint32_t(DType<T>::from_float(lo)) | (uint32_t(DType<T>::from_float(hi)) << 16) : 0x7FFF7FFFu;
   }
-  if (slot < 0) return;
-  if (slot >= (c.n_pages << c.page_log2)) {
-    if (at == 0) atomicExch(&g_kv_status, kBadSlot);
-    return;
+  const int limit = c.n_pages << c.page_log2;
+  if constexpr (U == 4) {
+    // four neighbours at a boundary of four (they share a page and a 16-token block)
+    if (value && slot[0] >= 0 && slot[0] < limit && (slot[0] & 3) == 0 && slot[1] == slot[0] + 1 && slot[2] == slot[0] + 2 &&
+        slot[3] == slot[0] + 3) {
+      const int page = slot[0] >> c.page_log2, offset = slot[0] & ((1 << c.page_log2) - 1);
+      *reinterpret_cast<uint4*>(c.v + cache_codes_at(page, h, c.heads, c.page_log2, c.D) + value_word_at(offset, at, c.D)) =
+          make_uint4(word[0], word[1], word[2], word[3]);
+      if (at == 0)
+        *reinterpret_cast<uint4*>(c.v_pair + cache_pair_at(page, h, c.heads, c.page_log2, offset)) =
+            make_uint4(pair[0], pair[1], pair[2], pair[3]);
+      return;
+    }
   }
-  const int page = slot >> c.page_log2, offset = slot & ((1 << c.page_log2) - 1);
-  uint8_t* codes = (value ? c.v : c.k) + cache_codes_at(page, h, c.heads, c.page_log2, c.D);
-  *reinterpret_cast<uint32_t*>(codes + (value ? value_word_at(offset, at, c.D) : key_word_at(offset, at, c.D))) = word;
-  if (at == 0)
-    (value ? c.v_pair : c.k_pair)[cache_pair_at(page, h, c.heads, c.page_log2, offset)] =
-        finite ? uint32_t(DType<T>::from_float(lo)) | (uint32_t(DType<T>::from_float(hi)) << 16) : 0x7FFF7FFFu;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (slot[u] < 0) continue;
+    if (slot[u] >= limit) {
+      if (at == 0) atomicExch(&g_kv_status, kBadSlot);
+      continue;
+    }
+    const int page = slot[u] >> c.page_log2, offset = slot[u] & ((1 << c.page_log2) - 1);
+    uint8_t* codes = (value ? c.v : c.k) + cache_codes_at(page, h, c.heads, c.page_log2, c.D);
+    *reinterpret_cast<uint32_t*>(codes + (value ? value_word_at(offset, at, c.D) : key_word_at(offset, at, c.D))) = word[u];
+    if (at == 0) (value ? c.v_pair : c.k_pair)[cache_pair_at(page, h, c.heads, c.page_log2, offset)] = pair[u];
+  }
 }
 
 // ---- rows out -----------------------------------------------------------------------------------------
-template <typename T>
-__global__ void __launch_bounds__(kRowWarps * 32) kv_read_kernel(uint16_t* k, uint16_t* v, const int* slots, int tokens,
-                                                                 CacheView c) {
+// The same shape: U tokens of a row's lane, all words under way before the first is unpacked.
+template <typename T, int U>
+__global__ void __launch_bounds__(kRowWarps * 32) kv_read_kernel(uint16_t* __restrict__ k, uint16_t* __restrict__ v,
+                                                                 const int* __restrict__ slots, int tokens, CacheView c) {
   const int lane = threadIdx.x & 31, lanes = c.D >> 3, per = 32 / lanes, at = lane % lanes;
+  const int groups = (tokens + U - 1) / U;
   const long long row = ((long long)blockIdx.x * kRowWarps + (threadIdx.x >> 5)) * per + lane / lanes;
-  const long long rows = (long long)tokens * c.heads * 2;
-  if (row >= rows) return;
-  const bool value = row >= rows / 2;
-  const long long r = value ? row - rows / 2 : row, t = r / c.heads;
-  const int h = int(r - t * c.heads), slot = slots[t];
-  uint32_t out[4] = {0, 0, 0, 0};
-  if (slot >= (c.n_pages << c.page_log2)) {
-    if (at == 0) atomicExch(&g_kv_status, kBadSlot);
-  } else if (slot >= 0) {
-    const int page = slot >> c.page_log2, offset = slot & ((1 << c.page_log2) - 1);
-    const uint8_t* codes = (value ? c.v : c.k) + cache_codes_at(page, h, c.heads, c.page_log2, c.D);
-    const uint32_t word = *reinterpret_cast<const uint32_t*>(
-        codes + (value ? value_word_at(offset, at, c.D) : key_word_at(offset, at, c.D)));
-    const float2 ls = lo_step<T>((value ? c.v_pair : c.k_pair)[cache_pair_at(page, h, c.heads, c.page_log2, offset)]);
+  const long long half = (long long)groups * c.heads;
+  if (row >= 2 * half) return;
+  const bool value = row >= half;
+  const long long r = value ? row - half : row;
+  const int group = int(r / c.heads), h = int(r - (long long)group * c.heads), t0 = group * U;
+  const int limit = c.n_pages << c.page_log2;
+  uint32_t word[U], pair[U];
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      out[e >> 1] |= uint32_t(DType<T>::from_float(fmaf(float((word >> (4 * e)) & 15u), ls.y, ls.x))) << (16 * (e & 1));
+  for (int u = 0; u < U; ++u) {
+    word[u] = pair[u] = 0;
+    const int slot = t0 + u < tokens ? slots[t0 + u] : -1;
+    if (slot >= limit) {
+      if (at == 0) atomicExch(&g_kv_status, kBadSlot);
+    } else if (slot >= 0) {
+      const int page = slot >> c.page_log2, offset = slot & ((1 << c.page_log2) - 1);
+      const uint8_t* codes = (value ? c.v : c.k) + cache_codes_at(page, h, c.heads, c.page_log2, c.D);
+      word[u] = *reinterpret_cast<const uint32_t*>(codes + (value ? value_word_at(offset, at, c.D) : key_word_at(offset, at, c.D)));
+      pair[u] = (value ? c.v_pair : c.k_pair)[cache_pair_at(page, h, c.heads, c.page_log2, offset)];
+    }
   }
-  reinterpret_cast<uint4*>((value ? v : k) + r * c.D)[at] = make_uint4(out[0], out[1], out[2], out[3]);
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (t0 + u >= tokens) break;
+    const float2 ls = lo_step<T>(pair[u]);
+    uint32_t out[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      out[e] = uint32_t(DType<T>::from_float(fmaf(float((word[u] >> (8 * e)) & 15u), ls.y, ls.x))) |
+               (uint32_t(DType<T>::from_float(fmaf(float((word[u] >> (8 * e + 4)) & 15u), ls.y, ls.x))) << 16);
+    reinterpret_cast<uint4*>((value ? v : k) + ((long long)(t0 + u) * c.heads + h) * c.D)[at] = make_uint4(out[0], out[1], out[2], out[3]);
+  }
 }
+
+// Tokens a warp takes: one while that leaves SMs without work, four beyond (16384 tokens x 4 heads of 256: a write
+// takes 62 us with one, 27 with four).
+inline int tokens_per_warp(long long rows, int D) { return rows * D <= 256LL * 148 * 32 ? 1 : 4; }
 
 }  // namespace
 
@@ -267,16 +328,16 @@ extern "C" int b200lut_kv_write(const b200lut_kv_cache* cache, const void* k, co
                       v_token_stride % 8 == 0 && v_head_stride % 8 == 0,
                   B200LUT_ERR_ALIGN, "kv_write: rows must be 16-byte aligned (pointers and strides)");
   if (tokens == 0) return B200LUT_OK;
-  const long long rows = 2LL * tokens * c.heads, per = (256 / c.D) * kRowWarps, grid = (rows + per - 1) / per;
+  const int U = tokens_per_warp(2LL * tokens * c.heads, c.D);
+  const long long rows = 2LL * ((tokens + U - 1LL) / U) * c.heads, per = (256 / c.D) * kRowWarps, grid = (rows + per - 1) / per;
   B200LUT_REQUIRE(grid <= 0x7fffffffLL, B200LUT_ERR_UNSUPPORTED, "kv_write: too many rows");
   const auto* kk = static_cast<const uint16_t*>(k);
   const auto* vv = static_cast<const uint16_t*>(v);
-  if (cache->dtype == B200LUT_BF16)
-    kv_write_kernel<__nv_bfloat16><<<unsigned(grid), kRowWarps * 32, 0, cudaStream_t(stream)>>>(
-        kk, vv, k_token_stride, k_head_stride, v_token_stride, v_head_stride, slots, tokens, c);
-  else
-    kv_write_kernel<__half><<<unsigned(grid), kRowWarps * 32, 0, cudaStream_t(stream)>>>(
-        kk, vv, k_token_stride, k_head_stride, v_token_stride, v_head_stride, slots, tokens, c);
+  const bool bf = cache->dtype == B200LUT_BF16;
+  auto* kernel = U == 1 ? (bf ? kv_write_kernel<__nv_bfloat16, 1> : kv_write_kernel<__half, 1>)
+                        : (bf ? kv_write_kernel<__nv_bfloat16, 4> : kv_write_kernel<__half, 4>);
+  kernel<<<unsigned(grid), kRowWarps * 32, 0, cudaStream_t(stream)>>>(kk, vv, k_token_stride, k_head_stride, v_token_stride,
+                                                                      v_head_stride, slots, tokens, c);
   B200LUT_CUDA_OK(cudaGetLastError());
   return B200LUT_OK;
 }
@@ -289,14 +350,15 @@ extern "C" int b200lut_kv_read(const b200lut_kv_cache* cache, void* k, void* v, 
   B200LUT_REQUIRE(tokens >= 0 && (tokens == 0 || (k && v && slots)), B200LUT_ERR_INVALID, "kv_read: null argument");
   B200LUT_REQUIRE(aligned16(k) && aligned16(v), B200LUT_ERR_ALIGN, "kv_read: outputs must be 16-byte aligned");
   if (tokens == 0) return B200LUT_OK;
-  const long long rows = 2LL * tokens * c.heads, per = (256 / c.D) * kRowWarps, grid = (rows + per - 1) / per;
+  const int U = tokens_per_warp(2LL * tokens * c.heads, c.D);
+  const long long rows = 2LL * ((tokens + U - 1LL) / U) * c.heads, per = (256 / c.D) * kRowWarps, grid = (rows + per - 1) / per;
   B200LUT_REQUIRE(grid <= 0x7fffffffLL, B200LUT_ERR_UNSUPPORTED, "kv_read: too many rows");
   auto* kk = static_cast<uint16_t*>(k);
   auto* vv = static_cast<uint16_t*>(v);
-  if (cache->dtype == B200LUT_BF16)
-    kv_read_kernel<__nv_bfloat16><<<unsigned(grid), kRowWarps * 32, 0, cudaStream_t(stream)>>>(kk, vv, slots, tokens, c);
-  else
-    kv_read_kernel<__half><<<unsigned(grid), kRowWarps * 32, 0, cudaStream_t(stream)>>>(kk, vv, slots, tokens, c);
+  const bool bf = cache->dtype == B200LUT_BF16;
+  auto* kernel = U == 1 ? (bf ? kv_read_kernel<__nv_bfloat16, 1> : kv_read_kernel<__half, 1>)
+                        : (bf ? kv_read_kernel<__nv_bfloat16, 4> : kv_read_kernel<__half, 4>);
+  kernel<<<unsigned(grid), kRowWarps * 32, 0, cudaStream_t(stream)>>>(kk, vv, slots, tokens, c);
   B200LUT_CUDA_OK(cudaGetLastError());
   return B200LUT_OK;
 }

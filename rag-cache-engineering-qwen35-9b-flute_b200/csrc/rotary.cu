@@ -8,10 +8,11 @@
 // angle: at position 2^20 a 32-bit product would be off by 2^-4 turns, this one by 2^-33. The rest is
 // fp32, one rounding at the end.
 //
-// Bound by memory: every element is read and written once. A head's row is D/8 lanes of 16 bytes, so a
-// warp holds 256/D rows at a time; the partner element sits R/16 lanes away (one shuffle). A warp computes
-// its token's R/2 sines once and reuses them for up to kUnroll groups of rows, whose loads are all in
-// flight before the sines are computed.
+// Bound by memory: every element is read and written once. A head's row is D/8 lanes; a lane holds four elements
+// of the first half of the rotated part and their four partners (two 8-byte loads), or eight elements that pass, so
+// that nothing is exchanged. A warp holds 256/D rows at a time; it computes its token's R/2 sines once and uses
+// them for up to seven groups of rows, whose loads are all in flight before the sines are computed (8192 tokens, 20
+// heads of 256: 51 us with partners fetched by shuffles, which made it bound by issue).
 #include "common.cuh"
 
 namespace b200lut {
@@ -35,26 +36,44 @@ struct RotaryParams {
 
 constexpr int kWarps = 4;
 
+__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
+  const __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
+  const __half2 r = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+template <typename T>
+__device__ __forceinline__ void unpack4(uint2 w, float (&v)[4]) {
+  v[0] = DType<T>::to_float(uint16_t(w.x & 0xFFFFu)), v[1] = DType<T>::to_float(uint16_t(w.x >> 16));
+  v[2] = DType<T>::to_float(uint16_t(w.y & 0xFFFFu)), v[3] = DType<T>::to_float(uint16_t(w.y >> 16));
+}
+
 template <typename T, int U>
 __global__ void __launch_bounds__(kWarps * 32) rotary_kernel(const __grid_constant__ RotaryParams p) {
-  __shared__ float2 trig[kWarps][128];
+  __shared__ __align__(16) float2 trig[kWarps][128];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long item = (long long)blockIdx.x * kWarps + warp;
   if (item >= (long long)p.T * p.chunks) return;
-  const int t = int(item / p.chunks), first = int(item % p.chunks) * U;
+  const int t = int(item / p.chunks), first = int(item - (long long)t * p.chunks) * U;
   const int lanes = p.D >> 3;                   // lanes of a row: 8, 16 or 32
   const int sub = lane / lanes, at = lane % lanes;
   const int per = 32 / lanes, heads = p.Hq + p.H;
+  const bool turned = at < (p.R >> 3);
+  // elements a .. a + 3 and b .. b + 3, partners where the lane turns them
+  const int a = turned ? 4 * at : 8 * at, b = turned ? a + (p.R >> 1) : a + 4;
 
-  uint4 raw[U];
+  uint2 xa[U], xb[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int h = (first + u) * per + sub;
-    raw[u] = make_uint4(0, 0, 0, 0);
+    xa[u] = xb[u] = make_uint2(0, 0);
     if (h < heads) {
       const int s = h >= p.Hq;
       const uint16_t* x = p.x[s] + (long long)t * p.token_stride[s] + (long long)(s ? h - p.Hq : h) * p.head_stride[s];
-      raw[u] = __ldg(reinterpret_cast<const uint4*>(x) + at);
+      xa[u] = __ldg(reinterpret_cast<const uint2*>(x + a));
+      xb[u] = __ldg(reinterpret_cast<const uint2*>(x + b));
     }
   }
   for (int i = lane; i < p.R / 2; i += 32) {
@@ -67,42 +86,51 @@ __global__ void __launch_bounds__(kWarps * 32) rotary_kernel(const __grid_consta
     trig[warp][i] = make_float2(c, s);
   }
   __syncwarp();
-  const int half = p.R >> 4;                    // lanes of half a rotated row
-  const bool turned = at < 2 * half, upper = at >= half;
-  const int partner = sub * lanes + (turned ? (upper ? at - half : at + half) : at);
-  float2 cs[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) cs[e] = turned ? trig[warp][(upper ? at - half : at) * 8 + e] : make_float2(1.f, 0.f);
-
+  float ga[4], gb[4];                           // q's gains
+  if (p.gain[0]) {
+    unpack4<T>(__ldg(reinterpret_cast<const uint2*>(p.gain[0] + a)), ga);
+    unpack4<T>(__ldg(reinterpret_cast<const uint2*>(p.gain[0] + b)), gb);
+  }
+  float c[4] = {1.f, 1.f, 1.f, 1.f}, s[4] = {0.f, 0.f, 0.f, 0.f};
+  if (turned) {
+    const float4 lo = *reinterpret_cast<const float4*>(&trig[warp][4 * at]);
+    const float4 hi = *reinterpret_cast<const float4*>(&trig[warp][4 * at + 2]);
+    c[0] = lo.x, s[0] = lo.y, c[1] = lo.z, s[1] = lo.w, c[2] = hi.x, s[2] = hi.y, c[3] = hi.z, s[3] = hi.w;
+  }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int h = (first + u) * per + sub;
-    const int s = h >= p.Hq;
-    const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
-    float v[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = DType<T>::to_float(uint16_t(w[e >> 1] >> (16 * (e & 1))));
+    const int side = h >= p.Hq;
+    float v[4], w[4];
+    unpack4<T>(xa[u], v);
+    unpack4<T>(xb[u], w);
     if (p.gain[0]) {
       float sum = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum = fmaf(v[e], v[e], sum);
+      for (int e = 0; e < 4; ++e) sum = fmaf(v[e], v[e], fmaf(w[e], w[e], sum));
       for (int o = lanes >> 1; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      const float r = rsqrtf(sum / float(p.D) + p.eps);
-      const uint4 gw = __ldg(reinterpret_cast<const uint4*>(p.gain[s]) + at);
-      const uint32_t g[4] = {gw.x, gw.y, gw.z, gw.w};
+      const float r = rsqrtf(fmaf(sum, 1.f / float(p.D), p.eps));
+      if (!side) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] *= r * DType<T>::to_float(uint16_t(g[e >> 1] >> (16 * (e & 1))));
+        for (int e = 0; e < 4; ++e) v[e] *= r * ga[e], w[e] *= r * gb[e];
+      } else {
+        float ka[4], kb[4];
+        unpack4<T>(__ldg(reinterpret_cast<const uint2*>(p.gain[1] + a)), ka);
+        unpack4<T>(__ldg(reinterpret_cast<const uint2*>(p.gain[1] + b)), kb);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] *= r * ka[e], w[e] *= r * kb[e];
+      }
     }
-    uint32_t out[4] = {0, 0, 0, 0};
+    float y[4], z[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float other = __shfl_sync(0xffffffffu, v[e], partner);
-      const float y = turned ? fmaf(v[e], cs[e].x, upper ? other * cs[e].y : -other * cs[e].y) : v[e];
-      out[e >> 1] |= uint32_t(DType<T>::from_float(y)) << (16 * (e & 1));
+    for (int e = 0; e < 4; ++e) {
+      y[e] = turned ? fmaf(v[e], c[e], -w[e] * s[e]) : v[e];
+      z[e] = turned ? fmaf(w[e], c[e], v[e] * s[e]) : w[e];
     }
     if (h < heads) {
-      uint16_t* y = p.y[s] + ((long long)t * (s ? p.H : p.Hq) + (s ? h - p.Hq : h)) * p.D;
-      reinterpret_cast<uint4*>(y)[at] = make_uint4(out[0], out[1], out[2], out[3]);
+      uint16_t* o = p.y[side] + ((long long)t * (side ? p.H : p.Hq) + (side ? h - p.Hq : h)) * p.D;
+      *reinterpret_cast<uint2*>(o + a) = make_uint2(pack2(y[0], y[1], T()), pack2(y[2], y[3], T()));
+      *reinterpret_cast<uint2*>(o + b) = make_uint2(pack2(z[0], z[1], T()), pack2(z[2], z[3], T()));
     }
   }
 }
@@ -141,8 +169,9 @@ extern "C" int b200lut_rotary(const b200lut_rotary_args* a, void* stream) {
   p.T = a->T, p.Hq = a->n_heads, p.H = a->n_kv_heads, p.D = a->D, p.R = a->R, p.eps = a->eps;
   const int per = 256 / a->D;
   p.groups = (a->n_heads + a->n_kv_heads + per - 1) / per;
-  // few tokens: one group of rows per warp, for latency; many: four, which share the sines
-  const int U = (long long)a->T * p.groups <= 148 * 32 ? 1 : 4;
+  // few tokens: one group of rows per warp, for latency; many: four or seven, which share the sines (seven where that
+  // takes fewer warps: of 20 groups three instead of five)
+  const int U = (long long)a->T * p.groups <= 148 * 32 ? 1 : (p.groups + 6) / 7 < (p.groups + 3) / 4 ? 7 : 4;
   p.chunks = (p.groups + U - 1) / U;
   const long long items = (long long)a->T * p.chunks, grid = (items + kWarps - 1) / kWarps;
   B200LUT_REQUIRE(grid <= 0x7fffffffLL, B200LUT_ERR_UNSUPPORTED, "rotary: too many rows");
@@ -150,9 +179,11 @@ extern "C" int b200lut_rotary(const b200lut_rotary_args* a, void* stream) {
   const unsigned g = unsigned(grid), n = kWarps * 32;
   if (a->dtype == B200LUT_BF16) {
     if (U == 1) rotary_kernel<__nv_bfloat16, 1><<<g, n, 0, st>>>(p);
+    else if (U == 7) rotary_kernel<__nv_bfloat16, 7><<<g, n, 0, st>>>(p);
     else rotary_kernel<__nv_bfloat16, 4><<<g, n, 0, st>>>(p);
   } else {
     if (U == 1) rotary_kernel<__half, 1><<<g, n, 0, st>>>(p);
+    else if (U == 7) rotary_kernel<__half, 7><<<g, n, 0, st>>>(p);
     else rotary_kernel<__half, 4><<<g, n, 0, st>>>(p);
   }
   B200LUT_CUDA_OK(cudaGetLastError());
