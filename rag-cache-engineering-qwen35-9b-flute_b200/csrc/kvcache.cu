@@ -1,6 +1,7 @@
 // The paged 4-bit key/value cache: the step plan (row starts, positions, page assignment and slots from the
 // requests' lengths, on the device), rows written and rows read back. Layout: kvcache.cuh.
 #include "kvcache.cuh"
+#include "packed.cuh"
 
 namespace b200lut {
 namespace {
@@ -118,20 +119,22 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Plan
 // ---- rows in ------------------------------------------------------------------------------------------
 // A row is D/8 lanes of eight elements: two shuffle reductions give lo and hi, then each lane writes the one
 // 32-bit word of codes its elements make. A warp takes the rows of U consecutive tokens, all loaded before the first is
-// worked on; four tokens whose slots are neighbours (a prompt's) make 16-byte stores of the values. Bound by memory:
-// rows are read once, codes written once.
+// worked on; four tokens whose slots are neighbours (a prompt's) make 16-byte stores of the values. Rows are read once,
+// codes written once, but the bound is issue, not memory: 16384 tokens of 4 heads of 256 take 33 us, where their 84 MB
+// would take 13. So elements stay in 16-bit pairs until the codes are made: the extremes are one packed maximum over
+// (x, -x), which keeps NaN, one shuffle moves both, and everything behind them is two elements an instruction (47 us
+// with one element an instruction).
 constexpr int kRowWarps = 4;
 constexpr float kRangeLimit = 1.329227996e36f;     // 2^120: 15 times a range below it is finite
 
-// rint(a / w) for 0 <= a <= 15 w, half to even: c is at most one off, the remainder a - c w is exact (c w and a
-// are multiples of one unit that is at least 2^-24 of it), so codes on a border, frequent with eight-bit
-// significands, are decided as the definition does. Adding 1.5 * 2^23 rounds and leaves the integer in the low bits;
-// rintf, the conversion and the IEEE division are the slow instructions of the obvious form (62 us instead of 27 for
-// 16384 tokens x 4 heads of 256, keys and values).
-__device__ __forceinline__ uint32_t code_of(float a, float w, float inv) {
-  const float m = fmaf(a, inv, 12582912.f), rem = fmaf(12582912.f - m, w, a), twice = 2.f * fabsf(rem);
-  const uint32_t n = __float_as_uint(m);
-  return (twice > w || (twice == w && (n & 1u)) ? (rem > 0.f ? n + 1u : n - 1u) : n) & 15u;
+// rint(a / w), half to even, of both halves, 0 <= a <= 15 w, with inv = 1 / w rounded; the second half's code at bit 4.
+// The quotient is the correctly rounded one (Markstein: the residual a - q w of a quotient that is off by an ulp, times
+// the rounded reciprocal, added to it), so codes on a border, frequent with eight-bit significands, are decided as the
+// definition does. Adding 1.5 * 2^23 then rounds to an integer and leaves it in the low bits.
+__device__ __forceinline__ uint32_t two_codes(float2 a, float2 minus_w, float2 inv) {
+  const float2 q = mul2(a, inv);
+  const float2 m = add2(fma2(fma2(q, minus_w, a), inv, q), make_float2(12582912.f, 12582912.f));
+  return (__float_as_uint(m.x) & 15u) | ((__float_as_uint(m.y) & 15u) << 4);
 }
 
 template <typename T, int U>
@@ -162,28 +165,25 @@ __global__ void __launch_bounds__(kRowWarps * 32) kv_write_kernel(const uint16_t
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
-    float x[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = DType<T>::to_float(uint16_t(w[e >> 1] >> (16 * (e & 1))));
-    float lo = x[0], hi = x[0], bad = x[0] - x[0];         // 0, or NaN where an element is not finite
-#pragma unroll
-    for (int e = 1; e < 8; ++e) lo = fminf(lo, x[e]), hi = fmaxf(hi, x[e]), bad += x[e] - x[e];
-    for (int o = lanes >> 1; o; o >>= 1) {
-      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    }
-    // the lanes of this row that hold one
-    const uint32_t odd = __ballot_sync(0xffffffffu, bad != 0.f) & ((lanes == 32 ? ~0u : (1u << lanes) - 1u) << (lane - at));
-    const float range = hi - lo;
-    const bool finite = odd == 0 && range < kRangeLimit;
+    // (hi, -lo) as one 16-bit pair: a NaN stays one
+    uint32_t top = max2_nan(max2_nan(w[0], w[1], T()), max2_nan(w[2], w[3], T()), T());
+    uint32_t low = max2_nan(max2_nan(w[0] ^ 0x80008000u, w[1] ^ 0x80008000u, T()),
+                            max2_nan(w[2] ^ 0x80008000u, w[3] ^ 0x80008000u, T()), T());
+    uint32_t ends = max2_nan(__byte_perm(top, low, 0x5410), __byte_perm(top, low, 0x7632), T());
+    for (int o = lanes >> 1; o; o >>= 1) ends = max2_nan(ends, __shfl_xor_sync(0xffffffffu, ends, o), T());
+    const float2 hl = unpack2(ends, T());
+    const float lo = -hl.y, range = hl.x - lo;
+    const bool finite = range < kRangeLimit;               // false for NaN too
     word[u] = 0;
     if (finite && range > 0.f) {
       // scaled by a power of two that keeps 1 / range and the products normal
       const float up = range < 1e-30f ? 1.329227996e36f : 1.f, width = range * up, inv = 1.f / width;
+      const float2 inv2 = make_float2(inv, inv), minus = make_float2(-width, -width), lo2 = make_float2(hl.y, hl.y);
+      const float2 scale = make_float2(15.f * up, 15.f * up);          // exact: up is a power of two
 #pragma unroll
-      for (int e = 0; e < 8; ++e) word[u] |= code_of(15.f * (x[e] - lo) * up, width, inv) << (4 * e);
+      for (int e = 0; e < 4; ++e) word[u] |= two_codes(mul2(add2(unpack2(w[e], T()), lo2), scale), minus, inv2) << (8 * e);
     }
-    pair[u] = finite ? uint32_t(DType<T>::from_float(lo)) | (uint32_t(DType<T>::from_float(hi)) << 16) : 0x7FFF7FFFu;
+    pair[u] = finite ? __byte_perm(ends ^ 0x80000000u, 0, 0x1032) : 0x7FFF7FFFu;       // lo in the low half
   }
   const int limit = c.n_pages << c.page_log2;
   if constexpr (U == 4) {
@@ -244,18 +244,19 @@ __global__ void __launch_bounds__(kRowWarps * 32) kv_read_kernel(uint16_t* __res
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     if (t0 + u >= tokens) break;
-    const float2 ls = lo_step<T>(pair[u]);
+    const float2 ls = lo_step<T>(pair[u]), lo2 = make_float2(ls.x, ls.x), step2 = make_float2(ls.y, ls.y);
     uint32_t out[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      out[e] = uint32_t(DType<T>::from_float(fmaf(float((word[u] >> (8 * e)) & 15u), ls.y, ls.x))) |
-               (uint32_t(DType<T>::from_float(fmaf(float((word[u] >> (8 * e + 4)) & 15u), ls.y, ls.x))) << 16);
+    for (int e = 0; e < 4; ++e) {        // 2^23 + code, less 2^23
+      const float2 n = make_float2(__uint_as_float(((word[u] >> (8 * e)) & 15u) | 0x4B000000u),
+                                   __uint_as_float(((word[u] >> (8 * e + 4)) & 15u) | 0x4B000000u));
+      out[e] = pack2(fma2(add2(n, make_float2(-8388608.f, -8388608.f)), step2, lo2), T());
+    }
     reinterpret_cast<uint4*>((value ? v : k) + ((long long)(t0 + u) * c.heads + h) * c.D)[at] = make_uint4(out[0], out[1], out[2], out[3]);
   }
 }
 
-// Tokens a warp takes: one while that leaves SMs without work, four beyond (16384 tokens x 4 heads of 256: a write
-// takes 62 us with one, 27 with four).
+// Tokens a warp takes: one while a wave of warps (32 an SM) holds every row, four beyond.
 inline int tokens_per_warp(long long rows, int D) { return rows * D <= 256LL * 148 * 32 ? 1 : 4; }
 
 }  // namespace

@@ -11,9 +11,11 @@
 // Bound by memory: every element is read and written once. A head's row is D/8 lanes; a lane holds four elements
 // of the first half of the rotated part and their four partners (two 8-byte loads), or eight elements that pass, so
 // that nothing is exchanged. A warp holds 256/D rows at a time; it computes its token's R/2 sines once and uses
-// them for up to seven groups of rows, whose loads are all in flight before the sines are computed (8192 tokens, 20
-// heads of 256: 51 us with partners fetched by shuffles, which made it bound by issue).
-#include "common.cuh"
+// them for up to seven groups of rows, whose loads are all in flight before the sines are computed. 8192 tokens of 20
+// heads of 256 with gains take 44 us, where the bytes would take 26; 51 with partners fetched by shuffles, 47 with one
+// element an instruction, 54 with registers cut to 64 for eight blocks an SM: the rest is issue and the chain of loads,
+// sum, turn and stores that each warp runs once.
+#include "packed.cuh"
 
 namespace b200lut {
 namespace {
@@ -36,20 +38,6 @@ struct RotaryParams {
 
 constexpr int kWarps = 4;
 
-__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
-  const __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-__device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
-  const __half2 r = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-template <typename T>
-__device__ __forceinline__ void unpack4(uint2 w, float (&v)[4]) {
-  v[0] = DType<T>::to_float(uint16_t(w.x & 0xFFFFu)), v[1] = DType<T>::to_float(uint16_t(w.x >> 16));
-  v[2] = DType<T>::to_float(uint16_t(w.y & 0xFFFFu)), v[3] = DType<T>::to_float(uint16_t(w.y >> 16));
-}
-
 template <typename T, int U>
 __global__ void __launch_bounds__(kWarps * 32) rotary_kernel(const __grid_constant__ RotaryParams p) {
   __shared__ __align__(16) float2 trig[kWarps][128];
@@ -65,15 +53,15 @@ __global__ void __launch_bounds__(kWarps * 32) rotary_kernel(const __grid_consta
   const int a = turned ? 4 * at : 8 * at, b = turned ? a + (p.R >> 1) : a + 4;
 
   uint2 xa[U], xb[U];
+  const uint16_t* in[2] = {p.x[0] + t * p.token_stride[0] + a, p.x[1] + t * p.token_stride[1] + a};
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int h = (first + u) * per + sub;
     xa[u] = xb[u] = make_uint2(0, 0);
     if (h < heads) {
-      const int s = h >= p.Hq;
-      const uint16_t* x = p.x[s] + (long long)t * p.token_stride[s] + (long long)(s ? h - p.Hq : h) * p.head_stride[s];
-      xa[u] = __ldg(reinterpret_cast<const uint2*>(x + a));
-      xb[u] = __ldg(reinterpret_cast<const uint2*>(x + b));
+      const uint16_t* x = h < p.Hq ? in[0] + h * p.head_stride[0] : in[1] + (h - p.Hq) * p.head_stride[1];
+      xa[u] = __ldg(reinterpret_cast<const uint2*>(x));
+      xb[u] = __ldg(reinterpret_cast<const uint2*>(x + (b - a)));
     }
   }
   for (int i = lane; i < p.R / 2; i += 32) {
@@ -86,51 +74,52 @@ __global__ void __launch_bounds__(kWarps * 32) rotary_kernel(const __grid_consta
     trig[warp][i] = make_float2(c, s);
   }
   __syncwarp();
-  float ga[4], gb[4];                           // q's gains
-  if (p.gain[0]) {
-    unpack4<T>(__ldg(reinterpret_cast<const uint2*>(p.gain[0] + a)), ga);
-    unpack4<T>(__ldg(reinterpret_cast<const uint2*>(p.gain[0] + b)), gb);
-  }
-  float c[4] = {1.f, 1.f, 1.f, 1.f}, s[4] = {0.f, 0.f, 0.f, 0.f};
+  // gains of q's four pairs of elements; the last warps of a token have k's rows too
+  float2 gain[4];
+  auto gains = [&](int side) {
+    const uint2 ga = __ldg(reinterpret_cast<const uint2*>(p.gain[side] + a));
+    const uint2 gb = __ldg(reinterpret_cast<const uint2*>(p.gain[side] + b));
+    gain[0] = unpack2(ga.x, T()), gain[1] = unpack2(ga.y, T()), gain[2] = unpack2(gb.x, T()), gain[3] = unpack2(gb.y, T());
+  };
+  if (p.gain[0]) gains(0);
+  float2 c[2], s[2];
   if (turned) {
     const float4 lo = *reinterpret_cast<const float4*>(&trig[warp][4 * at]);
     const float4 hi = *reinterpret_cast<const float4*>(&trig[warp][4 * at + 2]);
-    c[0] = lo.x, s[0] = lo.y, c[1] = lo.z, s[1] = lo.w, c[2] = hi.x, s[2] = hi.y, c[3] = hi.z, s[3] = hi.w;
+    c[0] = make_float2(lo.x, lo.z), s[0] = make_float2(lo.y, lo.w);
+    c[1] = make_float2(hi.x, hi.z), s[1] = make_float2(hi.y, hi.w);
   }
+  bool of_q = true;
+  const float share = 1.f / float(p.D);
+  uint16_t* out[2] = {p.y[0] + (long long)t * p.Hq * p.D + a, p.y[1] + (long long)t * p.H * p.D + a};
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int h = (first + u) * per + sub;
-    const int side = h >= p.Hq;
-    float v[4], w[4];
-    unpack4<T>(xa[u], v);
-    unpack4<T>(xb[u], w);
+    float2 v[4] = {unpack2(xa[u].x, T()), unpack2(xa[u].y, T()), unpack2(xb[u].x, T()), unpack2(xb[u].y, T())};
     if (p.gain[0]) {
-      float sum = 0.f;
+      float2 q = mul2(v[0], v[0]);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sum = fmaf(v[e], v[e], fmaf(w[e], w[e], sum));
+      for (int e = 1; e < 4; ++e) q = fma2(v[e], v[e], q);
+      float sum = q.x + q.y;
       for (int o = lanes >> 1; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      const float r = rsqrtf(fmaf(sum, 1.f / float(p.D), p.eps));
-      if (!side) {
+      const float r = rsqrtf(fmaf(sum, share, p.eps));
+      if (of_q && h >= p.Hq) gains(1), of_q = false;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] *= r * ga[e], w[e] *= r * gb[e];
-      } else {
-        float ka[4], kb[4];
-        unpack4<T>(__ldg(reinterpret_cast<const uint2*>(p.gain[1] + a)), ka);
-        unpack4<T>(__ldg(reinterpret_cast<const uint2*>(p.gain[1] + b)), kb);
+      for (int e = 0; e < 4; ++e) v[e] = mul2(v[e], mul2(make_float2(r, r), gain[e]));
+    }
+    if (turned) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] *= r * ka[e], w[e] *= r * kb[e];
+      for (int e = 0; e < 2; ++e) {
+        const float2 ws = mul2(v[e + 2], s[e]);
+        const float2 y = fma2(v[e], c[e], make_float2(-ws.x, -ws.y));
+        v[e + 2] = fma2(v[e + 2], c[e], mul2(v[e], s[e]));
+        v[e] = y;
       }
     }
-    float y[4], z[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      y[e] = turned ? fmaf(v[e], c[e], -w[e] * s[e]) : v[e];
-      z[e] = turned ? fmaf(w[e], c[e], v[e] * s[e]) : w[e];
-    }
     if (h < heads) {
-      uint16_t* o = p.y[side] + ((long long)t * (side ? p.H : p.Hq) + (side ? h - p.Hq : h)) * p.D;
-      *reinterpret_cast<uint2*>(o + a) = make_uint2(pack2(y[0], y[1], T()), pack2(y[2], y[3], T()));
-      *reinterpret_cast<uint2*>(o + b) = make_uint2(pack2(z[0], z[1], T()), pack2(z[2], z[3], T()));
+      uint16_t* o = h < p.Hq ? out[0] + h * p.D : out[1] + (h - p.Hq) * p.D;
+      *reinterpret_cast<uint2*>(o) = make_uint2(pack2(v[0], T()), pack2(v[1], T()));
+      *reinterpret_cast<uint2*>(o + (b - a)) = make_uint2(pack2(v[2], T()), pack2(v[3], T()));
     }
   }
 }
@@ -170,7 +159,7 @@ extern "C" int b200lut_rotary(const b200lut_rotary_args* a, void* stream) {
   const int per = 256 / a->D;
   p.groups = (a->n_heads + a->n_kv_heads + per - 1) / per;
   // few tokens: one group of rows per warp, for latency; many: four or seven, which share the sines (seven where that
-  // takes fewer warps: of 20 groups three instead of five)
+  // takes fewer warps: of 20 groups three instead of five, 44 us against 45)
   const int U = (long long)a->T * p.groups <= 148 * 32 ? 1 : (p.groups + 6) / 7 < (p.groups + 3) / 4 ? 7 : 4;
   p.chunks = (p.groups + U - 1) / U;
   const long long items = (long long)a->T * p.chunks, grid = (items + kWarps - 1) / kWarps;
