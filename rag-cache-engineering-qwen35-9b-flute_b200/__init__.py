@@ -10,6 +10,7 @@ from .palettized_modules import (FusedPalettizedMLP, KGroupedPalettizedLinear,  
                                  PalettizedEmbedding, PalettizedLinear,
                                  SplitQKV,
                                  reference_dequant, set_programmatic_launch)
+from .attention import PalettizedAttention                                       # noqa: F401
 from .artifacts import (load_metadata, load_palettized_embedding, load_palettized_weight,  # noqa: F401
                         load_tied_pair, replace_linear_with_palettized)
 from .lut_export import export_luts, import_luts, iter_palettized_linears      # noqa: F401
@@ -18,5 +19,5 @@ from . import flute_extended                                                    
 
 __all__ = ["load_quant_model", "load_palettized_weight", "replace_linear_with_palettized",
            "load_palettized_embedding", "load_tied_pair", "export_luts", "import_luts",
-           "iter_palettized_linears", "load_metadata", "PalettizedLinear", "PalettizedEmbedding", "KGroupedPalettizedLinear", "SplitQKV", "FusedPalettizedMLP", "reference_dequant",
+           "iter_palettized_linears", "load_metadata", "PalettizedLinear", "PalettizedEmbedding", "KGroupedPalettizedLinear", "SplitQKV", "PalettizedAttention", "FusedPalettizedMLP", "reference_dequant",
            "set_programmatic_launch", "fht", "kvcache", "rotary", "idxN", "synthetic", "flute_extended"]

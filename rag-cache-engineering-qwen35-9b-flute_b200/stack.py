@@ -9,9 +9,11 @@ as Q 2048 + K 2048 + V 4096 rows, in_proj_z 4096, out_proj 4096; 8 full-attentio
 layers with q 8192, k 1024, v 1024, o 4096; every layer an MLP 4096 -> 12288 ->
 4096), 248 modules, 6 912 212 992 weights, 4-bit codes, group 128.
 
-Attention, recurrence, norms and residual adds are excluded (they are not part of
-the palettized linear path): every projection group of a step reads the step's
-activation rows x [M, 4096]; the MLP chain gate/up -> SiLU*mul -> down is real.
+Recurrence, norms and residual adds are excluded (they are not part of the palettized
+linear path): every projection group of a step reads the step's activation rows x
+[M, 4096]; the MLP chain gate/up -> SiLU*mul -> down is real. So is, with an
+AttentionState, the chain of a full-attention layer: q/k/v -> rotary -> 4-bit cache ->
+attention over the requests' tokens -> o; without one its output projection reads x too.
 
 Column-parallel sharding: rank r of G owns output rows [r*N/G, (r+1)*N/G) of every
 projection (contiguous bytes in the tile-major code buffer). Sharded outputs that
@@ -30,7 +32,10 @@ import torch
 import torch.nn as nn
 
 from . import _lib, exchange, synthetic
+from .attention import attend_projected
+from .kvcache import KVCache4, StepPlan, plan_step
 from .palettized_modules import FusedPalettizedMLP, PalettizedLinear, SplitQKV
+from .rotary import AxisRotary
 
 HIDDEN = 4096
 INTERMEDIATE = 12288
@@ -38,6 +43,8 @@ N_LAYERS = 32
 FULL_ATTENTION_EVERY = 4          # layers 3, 7, ... are full attention (8 of 32)
 LINEAR_ATTN = (("q", 2048), ("k", 2048), ("v", 4096), ("z", 4096))
 FULL_ATTN = (("q", 8192), ("k", 1024), ("v", 1024))
+HEAD_DIM = 256                    # 16 query heads with a gate each, 4 key and value heads
+ROTARY_DIM, ROTARY_THETA = 64, 1e7
 
 
 def layer_kind(i: int) -> str:
@@ -210,7 +217,7 @@ class LinearStack(nn.Module):
             launches.append(("fht", src, dst, signs, None, None, None, None))
             outs_rot.append(dst)
             return dst, None
-        outs_rot = []
+        outs_rot, qkv = [], {}
         for L in self.layers:
             heads = L.heads()
             total = sum(m.N for m in heads)
@@ -221,6 +228,7 @@ class LinearStack(nn.Module):
                 off += m.N
             xr, inp = rotated(x, "heads")
             launches.append(("heads", xr, _lib.make_segments(descs), len(descs), _lib.EPI_NONE, descs, None, inp))
+            qkv[L] = hbuf
             o = L.out()
             obuf = torch.empty(M, o.N, dtype=dt, device=dev)
             od = [o._segment_desc(obuf)]
@@ -253,7 +261,7 @@ class LinearStack(nn.Module):
             outs += [hbuf, obuf, act, ybuf]
         if push and sentinel:
             arena.ready(dev)
-        plan = {"x": x, "launches": launches, "buffers": outs, "y": outs[-1], "arena": arena,
+        plan = {"x": x, "launches": launches, "buffers": outs, "qkv": qkv, "y": outs[-1], "arena": arena,
                 "sentinel": bool(push and sentinel),
                 "rotated": outs_rot}
         self._plans[M] = plan
@@ -309,12 +317,32 @@ class LinearStack(nn.Module):
             self.__dict__["_scratch_buf"] = buf
         return buf
 
-    def step(self, M: int, flags: int = 0, gather=None) -> torch.Tensor:
+    def step(self, M: int, flags: int = 0, gather=None, attention: Optional["AttentionState"] = None,
+             fresh: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Run every projection once on the plan's activation buffer; returns the
-        last layer's down_proj output (this rank's columns)."""
+        last layer's down_proj output (this rank's columns). With `attention` the rows are the
+        requests' next tokens (fresh[b] of request b, one request after another; without fresh one
+        of each), and a full-attention layer's output projection reads its attention."""
         plan = self._plan(M)
+        if attention is None:
+            if fresh is not None:
+                raise ValueError("fresh says whose tokens the rows are: it needs an AttentionState")
+            for entry in plan["launches"]:
+                self.run_launch(entry, M, flags, gather)
+            return plan["y"]
+        if attention.stack is not self:
+            raise ValueError("the AttentionState belongs to another stack")
+        step, full = attention.plan(M, fresh), 0
+        layers = iter(self.layers)
         for entry in plan["launches"]:
+            if entry[0] == "heads":
+                layer = next(layers)
+            elif entry[0] == "out" and layer.kind == "full":
+                entry = (entry[0], attention.attend(full, qkv, step, fresh is None), *entry[2:])
+                full += 1
             self.run_launch(entry, M, flags, gather)
+            if entry[0] == "heads":
+                qkv = plan["qkv"][layer]
         return plan["y"]
 
     def check_status(self) -> None:
@@ -379,6 +407,62 @@ class LinearStack(nn.Module):
                     n += 1
                     i = j
         return n
+
+
+class AttentionState:
+    """The attention of a LinearStack's full-attention layers: a cache a layer and one page table for `requests`
+    requests of up to `max_len` tokens each, all memory taken at once.
+
+        state = AttentionState(stack, requests=8, max_len=4096)
+        stack.step(T, attention=state, fresh=fresh)     # prompts: fresh[b] rows of request b (int32 [requests])
+        stack.step(8, attention=state)                  # decode: one row of each request
+
+    A request that is full is no longer served: its rows mean nothing, the others go on."""
+
+    def __init__(self, stack: LinearStack, requests: int, max_len: int, page_size: int = 64,
+                 rotary: Optional[AxisRotary] = None, window: int = 0, sinks: int = 0):
+        if stack.world > 1 or stack.rotate:
+            raise ValueError("AttentionState: attention runs on one rank's whole, unrotated projections")
+        if requests < 1 or max_len < 1 or window < 0 or sinks < 0:
+            raise ValueError("AttentionState: requests and max_len must be positive, window and sinks not negative")
+        layers = [L for L in stack.layers if L.kind == "full"]
+        if not layers:
+            raise ValueError(f"AttentionState: none of the stack's {len(stack.layers)} layers has full attention")
+        self.stack = stack
+        self.n_heads, self.n_kv_heads = layers[0].o_proj.K // HEAD_DIM, layers[0].qkv.k_proj.N // HEAD_DIM
+        width = -(-int(max_len) // page_size)
+        self.caches = [KVCache4(requests * width, self.n_kv_heads, HEAD_DIM, page_size=page_size, dtype=stack.dtype,
+                                device=stack.device) for _ in layers]
+        self.rotary = (AxisRotary(ROTARY_DIM, theta=ROTARY_THETA) if rotary is None else rotary).to(stack.device)
+        ints = dict(dtype=torch.int32, device=stack.device)
+        self.block_table = torch.zeros(requests, width, **ints)
+        self.free_pages = torch.arange(requests * width, **ints)
+        self.taken, self.kv_len = torch.zeros(1, **ints), torch.zeros(requests, **ints)
+        self._ones = torch.ones(requests, **ints)
+        self.window, self.sinks, self._outs = int(window), int(sinks), {}
+
+    def plan(self, rows: int, fresh: Optional[torch.Tensor]) -> StepPlan:
+        """The plan of a step of `rows` rows, which counts them in (on the device, in the stream's order)."""
+        if fresh is None and rows != self.kv_len.shape[0]:
+            raise ValueError(f"without fresh there is one row per request: {rows} rows, {self.kv_len.shape[0]} requests")
+        step = plan_step(self.kv_len, self._ones if fresh is None else fresh, self.block_table, self.free_pages, self.taken,
+                         self.caches[0].page_size, rows)
+        self.kv_len.copy_(step.kv_len)
+        self.taken.copy_(step.taken)
+        return step
+
+    def out(self, layer: int, rows: int) -> torch.Tensor:
+        """Where the result [rows, n_heads, head_dim] of full-attention layer `layer` goes (stable, as the plan's buffers)."""
+        if (layer, rows) not in self._outs:
+            self._outs[layer, rows] = torch.zeros(rows, self.n_heads, HEAD_DIM, dtype=self.stack.dtype, device=self.stack.device)
+        return self._outs[layer, rows]
+
+    def attend(self, layer: int, qkv: torch.Tensor, step: StepPlan, one_row_each: bool) -> torch.Tensor:
+        out = self.out(layer, qkv.shape[0])
+        if not one_row_each:
+            out.zero_()              # rows of no request are not written
+        return attend_projected(qkv, self.n_heads, self.caches[layer], self.block_table, step, self.rotary, gated=True,
+                                window=self.window, sinks=self.sinks, one_row_each=one_row_each, out=out).flatten(1)
 
 
 def _pair(segs, i, epi):

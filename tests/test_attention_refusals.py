@@ -5,6 +5,7 @@ from __future__ import annotations
 import copy
 import ctypes
 import pickle
+import types
 
 import pytest
 import torch
@@ -168,3 +169,23 @@ def test_c_attend():
     assert L.b200lut_attend_workspace_bytes(16, 4, 256, 0) > L.b200lut_attend_workspace_bytes(16, 4, 256, 1) > 0
     for bad in ((0, 1, 64), (4, 3, 64), (4, 0, 64), (4, 2, 96)):
         assert L.b200lut_attend_workspace_bytes(*bad, 1) == 0
+
+
+def test_module_arguments():
+    def lin(n, k=256):
+        return types.SimpleNamespace(N=n, K=k)
+
+    def qkv(q, k, v):
+        return types.SimpleNamespace(q_proj=lin(q), k_proj=lin(k), v_proj=lin(v))
+    rot = pkg.rotary.AxisRotary(64)
+    good = dict(qkv=qkv(512, 128, 128), o_proj=lin(256, 256), rotary=rot, head_dim=64, gated=True)
+    attn = pkg.PalettizedAttention(**good)
+    assert (attn.n_heads, attn.n_kv_heads, attn.head_dim) == (4, 2, 64)
+    g = torch.ones(64)
+    for kw, text in ((dict(head_dim=96), "head_dim must be"), (dict(qkv=qkv(512, 128, 64)), "do not make"),
+                     (dict(qkv=qkv(384, 128, 128)), "do not make"), (dict(qkv=qkv(512, 96, 96)), "do not make"),
+                     (dict(qkv=qkv(65 * 128, 64, 64)), "do not make"), (dict(gated=False), "o_proj reads"),
+                     (dict(rotary=pkg.rotary.AxisRotary(128)), "larger than head_dim"), (dict(q_gain=g), "come together"),
+                     (dict(q_gain=g, k_gain=torch.ones(32)), "k_gain must be"), (dict(window=-1), "not be negative")):
+        with pytest.raises(ValueError, match=text):
+            pkg.PalettizedAttention(**{**good, **kw})
