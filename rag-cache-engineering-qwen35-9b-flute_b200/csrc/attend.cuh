@@ -11,7 +11,9 @@
 // holds bf16's eight bits exactly down to 2^-28 of the largest element (and fp16's eleven to 2^-25).
 // p * step is rounded to fp16 (2^-12) after division by a power of two >= the largest step so far. With w its
 // rounded value the result is formed as sum w c - 7.5 sum w + sum p (lo + 7.5 step): the rounding then acts on
-// c - 7.5, at most half as large as c (against lo + step c: error of an fp16 result 2.9 times as large).
+// c - 7.5, at most half as large as c. With sum w c and lo the error of an fp16 result was 2.9 times its own rounding;
+// so it is 1.5 times (a bf16 result's is its rounding, 1.01 times), which the kernel for few rows brings to 1.0 with a
+// second product and the one for many rows, whose shared memory has no room for another operand, leaves.
 #pragma once
 
 #include "kvcache.cuh"
