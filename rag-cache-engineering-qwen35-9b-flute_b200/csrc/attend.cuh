@@ -13,7 +13,7 @@
 // rounded value the result is formed as sum w c - 7.5 sum w + sum p (lo + 7.5 step): the rounding then acts on
 // c - 7.5, at most half as large as c. With sum w c and lo the error of an fp16 result was 2.9 times its own rounding;
 // so it is 1.5 times (a bf16 result's is its rounding, 1.01 times), which the kernel for few rows brings to 1.0 with a
-// second product and the one for many rows, whose shared memory has no room for another operand, leaves.
+// second product. The one for many rows leaves it: its softmax warps, which bound it, would issue a third more.
 #pragma once
 
 #include "kvcache.cuh"

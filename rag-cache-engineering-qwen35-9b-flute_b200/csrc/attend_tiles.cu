@@ -218,7 +218,7 @@ __device__ __forceinline__ void next_part(const AttendParams& p, Work* w, long l
     if (++w->h == p.c.heads) {
       w->h = 0;
       do w->rq = tiles_request(p, ++w->b);
-      while (w->rq.rows == 0);
+      while (w->rq.rows == 0 && w->b + 1 < p.B);
     }
   }
   open_part(p, w, w->item_at, stop);

@@ -1,5 +1,7 @@
 // The paged 4-bit key/value cache: the step plan (row starts, positions, page assignment and slots from the
 // requests' lengths, on the device), rows written and rows read back. Layout: kvcache.cuh.
+#include <type_traits>
+
 #include "kvcache.cuh"
 #include "packed.cuh"
 
@@ -120,10 +122,10 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Plan
 // A row is D/8 lanes of eight elements: two shuffle reductions give lo and hi, then each lane writes the one
 // 32-bit word of codes its elements make. A warp takes the rows of U consecutive tokens, all loaded before the first is
 // worked on; four tokens whose slots are neighbours (a prompt's) make 16-byte stores of the values. Rows are read once,
-// codes written once, but the bound is issue, not memory: 16384 tokens of 4 heads of 256 take 33 us, where their 84 MB
-// would take 13. So elements stay in 16-bit pairs until the codes are made: the extremes are one packed maximum over
-// (x, -x), which keeps NaN, one shuffle moves both, and everything behind them is two elements an instruction (47 us
-// with one element an instruction).
+// codes written once, but the bound is issue, not memory: 16384 tokens of 4 heads of 256 take 28 us (reading them back
+// 17), where their 84 MB would take 13. So elements stay in 16-bit pairs until the codes are made: the extremes are one
+// packed maximum over (x, -x), which keeps NaN, one shuffle moves both, and everything behind them is two elements an
+// instruction (47 us with one element an instruction, 33 with the head's width as an argument).
 constexpr int kRowWarps = 4;
 constexpr float kRangeLimit = 1.329227996e36f;     // 2^120: 15 times a range below it is finite
 
@@ -137,17 +139,17 @@ __device__ __forceinline__ uint32_t two_codes(float2 a, float2 minus_w, float2 i
   return (__float_as_uint(m.x) & 15u) | ((__float_as_uint(m.y) & 15u) << 4);
 }
 
-template <typename T, int U>
+template <typename T, int D, int U>
 __global__ void __launch_bounds__(kRowWarps * 32) kv_write_kernel(const uint16_t* __restrict__ k, const uint16_t* __restrict__ v,
                                                                   long long kt, long long kh, long long vt, long long vh,
                                                                   const int* __restrict__ slots, int tokens, CacheView c) {
-  const int lane = threadIdx.x & 31, lanes = c.D >> 3, per = 32 / lanes, at = lane % lanes;
-  const int groups = (tokens + U - 1) / U;
-  const long long row = ((long long)blockIdx.x * kRowWarps + (threadIdx.x >> 5)) * per + lane / lanes;
-  const long long half = (long long)groups * c.heads;
+  constexpr int lanes = D / 8, per = 32 / lanes;
+  const int lane = threadIdx.x & 31, at = lane % lanes;
+  const unsigned row = (blockIdx.x * kRowWarps + (threadIdx.x >> 5)) * per + lane / lanes;
+  const unsigned half = (unsigned(tokens) + U - 1) / U * unsigned(c.heads);      // 2 half < 2^31
   const bool in = row < 2 * half, value = row >= half;
-  const long long r = in ? (value ? row - half : row) : 0;
-  const int group = int(r / c.heads), h = int(r - (long long)group * c.heads), t0 = group * U;
+  const unsigned r = in ? (value ? row - half : row) : 0, group = r / unsigned(c.heads);
+  const int h = int(r - group * c.heads), t0 = int(group) * U;
   int slot[U];
   uint4 raw[U];
 #pragma unroll
@@ -170,6 +172,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) kv_write_kernel(const uint16_t
     uint32_t low = max2_nan(max2_nan(w[0] ^ 0x80008000u, w[1] ^ 0x80008000u, T()),
                             max2_nan(w[2] ^ 0x80008000u, w[3] ^ 0x80008000u, T()), T());
     uint32_t ends = max2_nan(__byte_perm(top, low, 0x5410), __byte_perm(top, low, 0x7632), T());
+#pragma unroll
     for (int o = lanes >> 1; o; o >>= 1) ends = max2_nan(ends, __shfl_xor_sync(0xffffffffu, ends, o), T());
     const float2 hl = unpack2(ends, T());
     const float lo = -hl.y, range = hl.x - lo;
@@ -191,7 +194,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) kv_write_kernel(const uint16_t
     if (value && slot[0] >= 0 && slot[0] < limit && (slot[0] & 3) == 0 && slot[1] == slot[0] + 1 && slot[2] == slot[0] + 2 &&
         slot[3] == slot[0] + 3) {
       const int page = slot[0] >> c.page_log2, offset = slot[0] & ((1 << c.page_log2) - 1);
-      *reinterpret_cast<uint4*>(c.v + cache_codes_at(page, h, c.heads, c.page_log2, c.D) + value_word_at(offset, at, c.D)) =
+      *reinterpret_cast<uint4*>(c.v + cache_codes_at(page, h, c.heads, c.page_log2, D) + value_word_at(offset, at, D)) =
           make_uint4(word[0], word[1], word[2], word[3]);
       if (at == 0)
         *reinterpret_cast<uint4*>(c.v_pair + cache_pair_at(page, h, c.heads, c.page_log2, offset)) =
@@ -207,25 +210,25 @@ __global__ void __launch_bounds__(kRowWarps * 32) kv_write_kernel(const uint16_t
       continue;
     }
     const int page = slot[u] >> c.page_log2, offset = slot[u] & ((1 << c.page_log2) - 1);
-    uint8_t* codes = (value ? c.v : c.k) + cache_codes_at(page, h, c.heads, c.page_log2, c.D);
-    *reinterpret_cast<uint32_t*>(codes + (value ? value_word_at(offset, at, c.D) : key_word_at(offset, at, c.D))) = word[u];
+    uint8_t* codes = (value ? c.v : c.k) + cache_codes_at(page, h, c.heads, c.page_log2, D);
+    *reinterpret_cast<uint32_t*>(codes + (value ? value_word_at(offset, at, D) : key_word_at(offset, at, D))) = word[u];
     if (at == 0) (value ? c.v_pair : c.k_pair)[cache_pair_at(page, h, c.heads, c.page_log2, offset)] = pair[u];
   }
 }
 
 // ---- rows out -----------------------------------------------------------------------------------------
 // The same shape: U tokens of a row's lane, all words under way before the first is unpacked.
-template <typename T, int U>
+template <typename T, int D, int U>
 __global__ void __launch_bounds__(kRowWarps * 32) kv_read_kernel(uint16_t* __restrict__ k, uint16_t* __restrict__ v,
                                                                  const int* __restrict__ slots, int tokens, CacheView c) {
-  const int lane = threadIdx.x & 31, lanes = c.D >> 3, per = 32 / lanes, at = lane % lanes;
-  const int groups = (tokens + U - 1) / U;
-  const long long row = ((long long)blockIdx.x * kRowWarps + (threadIdx.x >> 5)) * per + lane / lanes;
-  const long long half = (long long)groups * c.heads;
+  constexpr int lanes = D / 8, per = 32 / lanes;
+  const int lane = threadIdx.x & 31, at = lane % lanes;
+  const unsigned row = (blockIdx.x * kRowWarps + (threadIdx.x >> 5)) * per + lane / lanes;
+  const unsigned half = (unsigned(tokens) + U - 1) / U * unsigned(c.heads);      // 2 half < 2^31
   if (row >= 2 * half) return;
   const bool value = row >= half;
-  const long long r = value ? row - half : row;
-  const int group = int(r / c.heads), h = int(r - (long long)group * c.heads), t0 = group * U;
+  const unsigned r = value ? row - half : row, group = r / unsigned(c.heads);
+  const int h = int(r - group * c.heads), t0 = int(group) * U;
   const int limit = c.n_pages << c.page_log2;
   uint32_t word[U], pair[U];
 #pragma unroll
@@ -236,8 +239,8 @@ __global__ void __launch_bounds__(kRowWarps * 32) kv_read_kernel(uint16_t* __res
       if (at == 0) atomicExch(&g_kv_status, kBadSlot);
     } else if (slot >= 0) {
       const int page = slot >> c.page_log2, offset = slot & ((1 << c.page_log2) - 1);
-      const uint8_t* codes = (value ? c.v : c.k) + cache_codes_at(page, h, c.heads, c.page_log2, c.D);
-      word[u] = *reinterpret_cast<const uint32_t*>(codes + (value ? value_word_at(offset, at, c.D) : key_word_at(offset, at, c.D)));
+      const uint8_t* codes = (value ? c.v : c.k) + cache_codes_at(page, h, c.heads, c.page_log2, D);
+      word[u] = *reinterpret_cast<const uint32_t*>(codes + (value ? value_word_at(offset, at, D) : key_word_at(offset, at, D)));
       pair[u] = (value ? c.v_pair : c.k_pair)[cache_pair_at(page, h, c.heads, c.page_log2, offset)];
     }
   }
@@ -252,7 +255,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) kv_read_kernel(uint16_t* __res
                                    __uint_as_float(((word[u] >> (8 * e + 4)) & 15u) | 0x4B000000u));
       out[e] = pack2(fma2(add2(n, make_float2(-8388608.f, -8388608.f)), step2, lo2), T());
     }
-    reinterpret_cast<uint4*>((value ? v : k) + ((long long)(t0 + u) * c.heads + h) * c.D)[at] = make_uint4(out[0], out[1], out[2], out[3]);
+    reinterpret_cast<uint4*>((value ? v : k) + ((long long)(t0 + u) * c.heads + h) * D)[at] = make_uint4(out[0], out[1], out[2], out[3]);
   }
 }
 
@@ -331,12 +334,17 @@ extern "C" int b200lut_kv_write(const b200lut_kv_cache* cache, const void* k, co
   if (tokens == 0) return B200LUT_OK;
   const int U = tokens_per_warp(2LL * tokens * c.heads, c.D);
   const long long rows = 2LL * ((tokens + U - 1LL) / U) * c.heads, per = (256 / c.D) * kRowWarps, grid = (rows + per - 1) / per;
-  B200LUT_REQUIRE(grid <= 0x7fffffffLL, B200LUT_ERR_UNSUPPORTED, "kv_write: too many rows");
+  B200LUT_REQUIRE(rows <= 0x7fffff00LL && tokens <= 0x7fffff00, B200LUT_ERR_UNSUPPORTED, "kv_write: too many rows");
   const auto* kk = static_cast<const uint16_t*>(k);
   const auto* vv = static_cast<const uint16_t*>(v);
   const bool bf = cache->dtype == B200LUT_BF16;
-  auto* kernel = U == 1 ? (bf ? kv_write_kernel<__nv_bfloat16, 1> : kv_write_kernel<__half, 1>)
-                        : (bf ? kv_write_kernel<__nv_bfloat16, 4> : kv_write_kernel<__half, 4>);
+  const auto pick = [&](auto d) {
+    constexpr int D = decltype(d)::value;
+    return U == 1 ? (bf ? kv_write_kernel<__nv_bfloat16, D, 1> : kv_write_kernel<__half, D, 1>)
+                  : (bf ? kv_write_kernel<__nv_bfloat16, D, 4> : kv_write_kernel<__half, D, 4>);
+  };
+  auto* kernel = c.D == 64 ? pick(std::integral_constant<int, 64>()) : c.D == 128 ? pick(std::integral_constant<int, 128>())
+                                                                                 : pick(std::integral_constant<int, 256>());
   kernel<<<unsigned(grid), kRowWarps * 32, 0, cudaStream_t(stream)>>>(kk, vv, k_token_stride, k_head_stride, v_token_stride,
                                                                       v_head_stride, slots, tokens, c);
   B200LUT_CUDA_OK(cudaGetLastError());
@@ -353,12 +361,17 @@ extern "C" int b200lut_kv_read(const b200lut_kv_cache* cache, void* k, void* v, 
   if (tokens == 0) return B200LUT_OK;
   const int U = tokens_per_warp(2LL * tokens * c.heads, c.D);
   const long long rows = 2LL * ((tokens + U - 1LL) / U) * c.heads, per = (256 / c.D) * kRowWarps, grid = (rows + per - 1) / per;
-  B200LUT_REQUIRE(grid <= 0x7fffffffLL, B200LUT_ERR_UNSUPPORTED, "kv_read: too many rows");
+  B200LUT_REQUIRE(rows <= 0x7fffff00LL && tokens <= 0x7fffff00, B200LUT_ERR_UNSUPPORTED, "kv_read: too many rows");
   auto* kk = static_cast<uint16_t*>(k);
   auto* vv = static_cast<uint16_t*>(v);
   const bool bf = cache->dtype == B200LUT_BF16;
-  auto* kernel = U == 1 ? (bf ? kv_read_kernel<__nv_bfloat16, 1> : kv_read_kernel<__half, 1>)
-                        : (bf ? kv_read_kernel<__nv_bfloat16, 4> : kv_read_kernel<__half, 4>);
+  const auto pick = [&](auto d) {
+    constexpr int D = decltype(d)::value;
+    return U == 1 ? (bf ? kv_read_kernel<__nv_bfloat16, D, 1> : kv_read_kernel<__half, D, 1>)
+                  : (bf ? kv_read_kernel<__nv_bfloat16, D, 4> : kv_read_kernel<__half, D, 4>);
+  };
+  auto* kernel = c.D == 64 ? pick(std::integral_constant<int, 64>()) : c.D == 128 ? pick(std::integral_constant<int, 128>())
+                                                                                 : pick(std::integral_constant<int, 256>());
   kernel<<<unsigned(grid), kRowWarps * 32, 0, cudaStream_t(stream)>>>(kk, vv, slots, tokens, c);
   B200LUT_CUDA_OK(cudaGetLastError());
   return B200LUT_OK;

@@ -12,9 +12,12 @@
 // of the first half of the rotated part and their four partners (two 8-byte loads), or eight elements that pass, so
 // that nothing is exchanged. A warp holds 256/D rows at a time; it computes its token's R/2 sines once and uses
 // them for up to seven groups of rows, whose loads are all in flight before the sines are computed. 8192 tokens of 20
-// heads of 256 with gains take 44 us, where the bytes would take 26; 51 with partners fetched by shuffles, 47 with one
-// element an instruction, 54 with registers cut to 64 for eight blocks an SM: the rest is issue and the chain of loads,
-// sum, turn and stores that each warp runs once.
+// heads of 256 with gains take 40 us, where the bytes would take 26; 51 with partners fetched by shuffles, 47 with one
+// element an instruction, 44 with the head's width as an argument, ten more with registers cut to 64 for eight blocks
+// an SM: the rest is issue and the chain of loads, sum, turn and stores that each warp runs once. Without gains, 4093
+// tokens of 40 heads of 128: 16 us, the bytes 13.
+#include <type_traits>
+
 #include "packed.cuh"
 
 namespace b200lut {
@@ -38,16 +41,15 @@ struct RotaryParams {
 
 constexpr int kWarps = 4;
 
-template <typename T, int U>
+template <typename T, int D, int U>
 __global__ void __launch_bounds__(kWarps * 32) rotary_kernel(const __grid_constant__ RotaryParams p) {
   __shared__ __align__(16) float2 trig[kWarps][128];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long item = (long long)blockIdx.x * kWarps + warp;
-  if (item >= (long long)p.T * p.chunks) return;
-  const int t = int(item / p.chunks), first = int(item - (long long)t * p.chunks) * U;
-  const int lanes = p.D >> 3;                   // lanes of a row: 8, 16 or 32
-  const int sub = lane / lanes, at = lane % lanes;
-  const int per = 32 / lanes, heads = p.Hq + p.H;
+  const unsigned item = blockIdx.x * kWarps + warp;        // T * chunks < 2^31
+  const int t = int(item / unsigned(p.chunks)), first = int(item - unsigned(t) * p.chunks) * U;
+  if (t >= p.T) return;
+  constexpr int lanes = D / 8, per = 32 / lanes;           // lanes of a row: 8, 16 or 32
+  const int sub = lane / lanes, at = lane % lanes, heads = p.Hq + p.H;
   const bool turned = at < (p.R >> 3);
   // elements a .. a + 3 and b .. b + 3, partners where the lane turns them
   const int a = turned ? 4 * at : 8 * at, b = turned ? a + (p.R >> 1) : a + 4;
@@ -90,8 +92,8 @@ __global__ void __launch_bounds__(kWarps * 32) rotary_kernel(const __grid_consta
     c[1] = make_float2(hi.x, hi.z), s[1] = make_float2(hi.y, hi.w);
   }
   bool of_q = true;
-  const float share = 1.f / float(p.D);
-  uint16_t* out[2] = {p.y[0] + (long long)t * p.Hq * p.D + a, p.y[1] + (long long)t * p.H * p.D + a};
+  const float share = 1.f / D;
+  uint16_t* out[2] = {p.y[0] + (long long)t * p.Hq * D + a, p.y[1] + (long long)t * p.H * D + a};
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int h = (first + u) * per + sub;
@@ -101,6 +103,7 @@ __global__ void __launch_bounds__(kWarps * 32) rotary_kernel(const __grid_consta
 #pragma unroll
       for (int e = 1; e < 4; ++e) q = fma2(v[e], v[e], q);
       float sum = q.x + q.y;
+#pragma unroll
       for (int o = lanes >> 1; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       const float r = rsqrtf(fmaf(sum, share, p.eps));
       if (of_q && h >= p.Hq) gains(1), of_q = false;
@@ -117,7 +120,7 @@ __global__ void __launch_bounds__(kWarps * 32) rotary_kernel(const __grid_consta
       }
     }
     if (h < heads) {
-      uint16_t* o = h < p.Hq ? out[0] + h * p.D : out[1] + (h - p.Hq) * p.D;
+      uint16_t* o = h < p.Hq ? out[0] + h * D : out[1] + (h - p.Hq) * D;
       *reinterpret_cast<uint2*>(o) = make_uint2(pack2(v[0], T()), pack2(v[1], T()));
       *reinterpret_cast<uint2*>(o + (b - a)) = make_uint2(pack2(v[2], T()), pack2(v[3], T()));
     }
@@ -159,22 +162,22 @@ extern "C" int b200lut_rotary(const b200lut_rotary_args* a, void* stream) {
   const int per = 256 / a->D;
   p.groups = (a->n_heads + a->n_kv_heads + per - 1) / per;
   // few tokens: one group of rows per warp, for latency; many: four or seven, which share the sines (seven where that
-  // takes fewer warps: of 20 groups three instead of five, 44 us against 45)
+  // takes fewer warps: of 20 groups three instead of five: a microsecond in 45)
   const int U = (long long)a->T * p.groups <= 148 * 32 ? 1 : (p.groups + 6) / 7 < (p.groups + 3) / 4 ? 7 : 4;
   p.chunks = (p.groups + U - 1) / U;
   const long long items = (long long)a->T * p.chunks, grid = (items + kWarps - 1) / kWarps;
-  B200LUT_REQUIRE(grid <= 0x7fffffffLL, B200LUT_ERR_UNSUPPORTED, "rotary: too many rows");
+  B200LUT_REQUIRE(items <= 0x7fffff00LL, B200LUT_ERR_UNSUPPORTED, "rotary: too many rows");
   const cudaStream_t st = cudaStream_t(stream);
-  const unsigned g = unsigned(grid), n = kWarps * 32;
-  if (a->dtype == B200LUT_BF16) {
-    if (U == 1) rotary_kernel<__nv_bfloat16, 1><<<g, n, 0, st>>>(p);
-    else if (U == 7) rotary_kernel<__nv_bfloat16, 7><<<g, n, 0, st>>>(p);
-    else rotary_kernel<__nv_bfloat16, 4><<<g, n, 0, st>>>(p);
-  } else {
-    if (U == 1) rotary_kernel<__half, 1><<<g, n, 0, st>>>(p);
-    else if (U == 7) rotary_kernel<__half, 7><<<g, n, 0, st>>>(p);
-    else rotary_kernel<__half, 4><<<g, n, 0, st>>>(p);
-  }
+  const bool bf = a->dtype == B200LUT_BF16;
+  const auto pick = [&](auto d) {
+    constexpr int D = decltype(d)::value;
+    return U == 1   ? (bf ? rotary_kernel<__nv_bfloat16, D, 1> : rotary_kernel<__half, D, 1>)
+           : U == 4 ? (bf ? rotary_kernel<__nv_bfloat16, D, 4> : rotary_kernel<__half, D, 4>)
+                    : (bf ? rotary_kernel<__nv_bfloat16, D, 7> : rotary_kernel<__half, D, 7>);
+  };
+  auto* kernel = a->D == 64 ? pick(std::integral_constant<int, 64>()) : a->D == 128 ? pick(std::integral_constant<int, 128>())
+                                                                                   : pick(std::integral_constant<int, 256>());
+  kernel<<<unsigned(grid), kWarps * 32, 0, st>>>(p);
   B200LUT_CUDA_OK(cudaGetLastError());
   return B200LUT_OK;
 }

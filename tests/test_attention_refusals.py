@@ -165,6 +165,7 @@ def test_c_attend():
         refused(call(args(**kw), AT, big, None), 5, "16-byte")
     refused(call(args(), None, big, None), 4, "workspace")
     refused(call(args(), AT, 64, None), 4, "workspace")
+    refused(call(args(T=1 << 30), AT, big, None), 2, "too many rows")
     assert call(args(T=0), None, 0, None) == 0 and call(args(B=0), None, 0, None) == 0
     assert L.b200lut_attend_workspace_bytes(16, 4, 256, 0) > L.b200lut_attend_workspace_bytes(16, 4, 256, 1) > 0
     for bad in ((0, 1, 64), (4, 3, 64), (4, 0, 64), (4, 2, 96)):
