@@ -110,7 +110,8 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Plan
         } else {
           page = *entry;
         }
-        if (page >= 0) slot = (page << p.page_log2) + (pos & (P - 1));
+        // a page that is none: a slot that a write reports
+        if (page >= 0) slot = page > (INT32_MAX >> p.page_log2) ? INT32_MAX : (page << p.page_log2) + (pos & (P - 1));
       }
     }
     p.positions[t] = pos;
@@ -122,7 +123,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Plan
 // A row is D/8 lanes of eight elements: two shuffle reductions give lo and hi, then each lane writes the one
 // 32-bit word of codes its elements make. A warp takes the rows of U consecutive tokens, all loaded before the first is
 // worked on; four tokens whose slots are neighbours (a prompt's) make 16-byte stores of the values. Rows are read once,
-// codes written once, but the bound is issue, not memory: 16384 tokens of 4 heads of 256 take 28 us (reading them back
+// codes written once, but the bound is issue, not memory: 16384 tokens of 4 heads of 256 take 27 us (reading them back
 // 17), where their 84 MB would take 13. So elements stay in 16-bit pairs until the codes are made: the extremes are one
 // packed maximum over (x, -x), which keeps NaN, one shuffle moves both, and everything behind them is two elements an
 // instruction (47 us with one element an instruction, 33 with the head's width as an argument).
@@ -132,7 +133,8 @@ constexpr float kRangeLimit = 1.329227996e36f;     // 2^120: 15 times a range be
 // rint(a / w), half to even, of both halves, 0 <= a <= 15 w, with inv = 1 / w rounded; the second half's code at bit 4.
 // The quotient is the correctly rounded one (Markstein: the residual a - q w of a quotient that is off by an ulp, times
 // the rounded reciprocal, added to it), so codes on a border, frequent with eight-bit significands, are decided as the
-// definition does. Adding 1.5 * 2^23 then rounds to an integer and leaves it in the low bits.
+// definition does. (a itself is rounded where x and lo lie far apart: there a quotient within 2^-20 of a border may go
+// to either side.) Adding 1.5 * 2^23 then rounds to an integer and leaves it in the low bits.
 __device__ __forceinline__ uint32_t two_codes(float2 a, float2 minus_w, float2 inv) {
   const float2 q = mul2(a, inv);
   const float2 m = add2(fma2(fma2(q, minus_w, a), inv, q), make_float2(12582912.f, 12582912.f));
@@ -181,10 +183,11 @@ __global__ void __launch_bounds__(kRowWarps * 32) kv_write_kernel(const uint16_t
     if (finite && range > 0.f) {
       // scaled by a power of two that keeps 1 / range and the products normal
       const float up = range < 1e-30f ? 1.329227996e36f : 1.f, width = range * up, inv = 1.f / width;
-      const float2 inv2 = make_float2(inv, inv), minus = make_float2(-width, -width), lo2 = make_float2(hl.y, hl.y);
-      const float2 scale = make_float2(15.f * up, 15.f * up);          // exact: up is a power of two
+      const float by = 15.f * up;                          // products with it are exact
+      const float2 inv2 = make_float2(inv, inv), minus = make_float2(-width, -width), scale = make_float2(by, by);
+      const float2 low = make_float2(-lo * by, -lo * by);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) word[u] |= two_codes(mul2(add2(unpack2(w[e], T()), lo2), scale), minus, inv2) << (8 * e);
+      for (int e = 0; e < 4; ++e) word[u] |= two_codes(fma2(unpack2(w[e], T()), scale, low), minus, inv2) << (8 * e);
     }
     pair[u] = finite ? __byte_perm(ends ^ 0x80000000u, 0, 0x1032) : 0x7FFF7FFFu;       // lo in the low half
   }

@@ -209,6 +209,20 @@ def test_pages_outside_the_cache_are_hidden_and_reported():
             close(y, want, tol, str(bad))
 
 
+def test_offsets_beyond_32_bits():
+    H, D, page, L = 4, 256, 64, 1000
+    far, near = pkg.kvcache.KVCache4(150000, H, D, page_size=page), pkg.kvcache.KVCache4(16, H, D, page_size=page)
+    assert far.k_codes.numel() > 2 ** 32
+    pages = torch.arange(16, **INT)
+    slots = (pages.long()[:, None] * page + torch.arange(page, device="cuda")).flatten()[:L].int()
+    k, v = (torch.randn(L, H, D, device="cuda").bfloat16() for _ in range(2))
+    far.write(k, v, slots + (150000 - 16) * page)
+    near.write(k, v, slots)
+    for rows in (1, 70):
+        q, start, n = torch.randn(rows, 2 * H, D, device="cuda").bfloat16(), torch.tensor([0, rows], **INT), torch.tensor([L], **INT)
+        assert torch.equal(far.attend(q, pages[None] + (150000 - 16), n, start), near.attend(q, pages[None], n, start))
+
+
 def test_strides():
     b = Batch([100, 37, 5], [1, 20, 5], 8, 2, 128, 32, gate=True)
     want = b.check()

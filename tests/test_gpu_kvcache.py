@@ -105,6 +105,15 @@ def test_plan_of_many_requests_and_overflowing_counts():
     assert p.row_start.tolist() == [0] + [100] * B
 
 
+def test_plan_of_pages_that_are_none():
+    dev = dict(dtype=torch.int32, device="cuda")
+    table = torch.tensor([[3, 2 ** 31 - 1], [2 ** 27, -1], [-7, -1]], **dev)
+    step = kv.plan_step(torch.tensor([17, 1, 2], **dev), torch.tensor([1, 2, 1], **dev), table, torch.arange(4, **dev),
+                        torch.zeros(1, **dev), 16, 4)
+    # slots of pages beyond every cache do not wrap into one: writes skip and report them; negative pages have no slot
+    assert step.slots.tolist() == [2 ** 31 - 1, 2 ** 31 - 1, 2 ** 31 - 1, -1]
+
+
 def test_plan_captured_and_replayed():
     dev = dict(dtype=torch.int32, device="cuda")
     cached, fresh = torch.tensor([15, 31], **dev), torch.tensor([1, 1], **dev)
