@@ -123,21 +123,30 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Plan
 // A row is D/8 lanes of eight elements: two shuffle reductions give lo and hi, then each lane writes the one
 // 32-bit word of codes its elements make. A warp takes the rows of U consecutive tokens, all loaded before the first is
 // worked on; four tokens whose slots are neighbours (a prompt's) make 16-byte stores of the values. Rows are read once,
-// codes written once, but the bound is issue, not memory: 16384 tokens of 4 heads of 256 take 27 us (reading them back
+// codes written once, but the bound is issue, not memory: 16384 tokens of 4 heads of 256 take 31 us (reading them back
 // 17), where their 84 MB would take 13. So elements stay in 16-bit pairs until the codes are made: the extremes are one
 // packed maximum over (x, -x), which keeps NaN, one shuffle moves both, and everything behind them is two elements an
-// instruction (47 us with one element an instruction, 33 with the head's width as an argument).
+// instruction (47 us with one element an instruction, 33 with the head's width as an argument, 27 without the decisions in
+// 64 bits that borders need).
 constexpr int kRowWarps = 4;
 constexpr float kRangeLimit = 1.329227996e36f;     // 2^120: 15 times a range below it is finite
 
 // rint(a / w), half to even, of both halves, 0 <= a <= 15 w, with inv = 1 / w rounded; the second half's code at bit 4.
 // The quotient is the correctly rounded one (Markstein: the residual a - q w of a quotient that is off by an ulp, times
 // the rounded reciprocal, added to it), so codes on a border, frequent with eight-bit significands, are decided as the
-// definition does. (a itself is rounded where x and lo lie far apart: there a quotient within 2^-20 of a border may go
-// to either side.) Adding 1.5 * 2^23 then rounds to an integer and leaves it in the low bits.
-__device__ __forceinline__ uint32_t two_codes(float2 a, float2 minus_w, float2 inv) {
-  const float2 q = mul2(a, inv);
-  const float2 m = add2(fma2(fma2(q, minus_w, a), inv, q), make_float2(12582912.f, 12582912.f));
+// definition does. Adding 1.5 * 2^23 then rounds to an integer and leaves it in the low bits. `far`: the largest
+// distance of a quotient from its code.
+template <bool kFar>
+__device__ __forceinline__ uint32_t two_codes(float2 a, float2 minus_w, float2 inv, float* far) {
+  const float2 magic = make_float2(12582912.f, 12582912.f);
+  float2 q = mul2(a, inv);
+  q = fma2(fma2(q, minus_w, a), inv, q);
+  const float2 m = add2(q, magic);
+  if constexpr (kFar) {
+    const float2 n = add2(m, make_float2(-12582912.f, -12582912.f));
+    const float2 d = add2(q, make_float2(-n.x, -n.y));
+    *far = fmaxf(*far, fmaxf(fabsf(d.x), fabsf(d.y)));
+  }
   return (__float_as_uint(m.x) & 15u) | ((__float_as_uint(m.y) & 15u) << 4);
 }
 
@@ -186,8 +195,28 @@ __global__ void __launch_bounds__(kRowWarps * 32) kv_write_kernel(const uint16_t
       const float by = 15.f * up;                          // products with it are exact
       const float2 inv2 = make_float2(inv, inv), minus = make_float2(-width, -width), scale = make_float2(by, by);
       const float2 low = make_float2(-lo * by, -lo * by);
+      // a has more than fp32's 24 bits where x and lo lie more than 2^12 apart (fp16, of longer significands: 2^8). What
+      // then comes near to a border is decided in 64 bits: in fp16 any such quotient (one warp in some hundred); in bf16
+      // the rows where it can happen, those with an end far below the other and those whose zero lies at a border.
+      constexpr bool kFar = std::is_same<T, __half>::value;
+      float far = 0.f;
+      if constexpr (!kFar) {
+        const float ends_lo = fminf(fabsf(lo), fabsf(hl.x)), zero = low.x * inv;
+        if (ends_lo < 4.8828125e-4f * fmaxf(fabsf(lo), fabsf(hl.x)) ? ends_lo != 0.f : fabsf(zero - rintf(zero)) > 0.496f) far = 1.f;
+      }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) word[u] |= two_codes(fma2(unpack2(w[e], T()), scale, low), minus, inv2) << (8 * e);
+      for (int e = 0; e < 4; ++e)
+        word[u] |= two_codes<kFar>(fma2(unpack2(w[e], T()), scale, low), minus, inv2, &far) << (8 * e);
+      if (far > 0.49999f) {
+        word[u] = 0;
+#pragma unroll 1
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t pair_of = e < 2 ? w[0] : e < 4 ? w[1] : e < 6 ? w[2] : w[3];
+          const float2 x = unpack2(pair_of, T());
+          const double q = 15.0 * (double(e & 1 ? x.y : x.x) - double(lo)) / (double(hl.x) - double(lo));
+          word[u] |= uint32_t(__double2int_rn(q)) << (4 * e);
+        }
+      }
     }
     pair[u] = finite ? __byte_perm(ends ^ 0x80000000u, 0, 0x1032) : 0x7FFF7FFFu;       // lo in the low half
   }

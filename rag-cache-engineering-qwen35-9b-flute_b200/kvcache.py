@@ -7,10 +7,9 @@
 
 A row is the head_dim elements of one token and key/value head: its smallest and largest element lo and hi are
 kept exactly, an element is the code rint(15 (x - lo) / (hi - lo)) (half to even) and stands for lo + code (hi -
-lo) / 15 (fp32 arithmetic: an element whose quotient lies within 2^-20 of the middle between two codes may get
-either). A row with a NaN, an infinity or a range of 2^120 and more reads as NaN. Rows whose elements are spread
-evenly lose least: rotate heads with outlier elements first (fht.fht_block on queries and keys alike leaves
-every score as it is).
+lo) / 15. A row with a NaN, an infinity or a range of 2^120 and more reads as NaN. Rows whose elements are
+spread evenly lose least: rotate heads with outlier elements first (fht.fht_block on queries and keys alike
+leaves every score as it is).
 
 Everything that follows the requests' lengths is on the device: no call waits for the GPU, and all of them
 can be captured into CUDA graphs.

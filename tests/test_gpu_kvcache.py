@@ -203,6 +203,24 @@ def test_borders_and_constant_rows():
         assert got.min() == ends.min() and got.max() == ends.max()
 
 
+def test_quotients_next_to_a_border():
+    # 15 (x - lo) of more than 24 bits: 6.50000004, which is 6.5 in fp32
+    lo, hi, near = -2.177734375, 2.83984375, -0.0034503936767578125
+    x = torch.full((4, 1, 64), lo, device="cuda", dtype=torch.float16)
+    x[..., 1], x[:2, :, 5], x[2:, :, 7] = hi, near, near
+    cache = kv.KVCache4(2, 1, 64, page_size=16, dtype=torch.float16)
+    k, v = round_trip(cache, x, x.flip(-1), torch.arange(4, device="cuda").int())
+    assert (k[0, 0, 5] > 0.16) and torch.equal(v, k.flip(-1))
+    # bf16: a tiny element of a symmetric row, and a row with a tiny smallest element
+    x = torch.full((4, 1, 64), -2.484375, device="cuda", dtype=torch.bfloat16)
+    x[..., 1], x[:, 0, 5] = 2.484375, torch.tensor([-4.9e-8, 4.9e-8, 0.0, -1e-12])
+    y = torch.full((4, 1, 64), 1e-6, device="cuda", dtype=torch.bfloat16)
+    y[..., 1], y[..., 5], y[..., 6] = 30.0, 15.0, 1.0
+    cache = kv.KVCache4(2, 1, 64, page_size=16)
+    k, v = round_trip(cache, x, y, torch.arange(4, device="cuda").int())
+    assert (k[:, 0, 5] > 0).tolist() == [False, True, True, False] and (v[:, 0, 6] < 0.1).all()
+
+
 def test_extreme_rows():
     for dtype in (torch.bfloat16, torch.float16):
         info = torch.finfo(dtype)
