@@ -1,7 +1,7 @@
 // Attention over the 4-bit cache for few rows per request (single tokens): mma.sync on codes, split over tokens.
 //
 // A work item is 8 NT rows (query heads of one key/value head, times new tokens) of one request. Its visible
-// tokens are cut into tiles of 16; all items' tiles form one line that is dealt to the blocks in equal
+// tokens are cut into tiles of 16 or 32; all items' tiles form one line that is dealt to the blocks in equal
 // contiguous shares, whatever the requests' lengths. The warps of a block take the tiles of its share in turn,
 // each with a running maximum and sum of its own, and join in shared memory; items that span blocks are
 // joined by a second kernel in the order of the blocks (deterministic, no atomics).
@@ -35,9 +35,10 @@ constexpr float kMinStep = 7.888609e-31f;   // 2^-100
 template <int D, int NT>
 struct Shape {
   static constexpr int kRows = 8 * NT;
-  // 16-token pieces of a warp's step. One: with two the loop has 1100 instructions at 256 elements, more than the
-  // scheduler's instruction cache holds, and takes 134 us where it takes 111 (64 sequences of up to 8192 tokens).
-  static constexpr int kSub = 1;
+  // 16-token pieces of a warp's step. Two halve what a step costs besides its products (32 ragged sequences of up to 8192
+  // tokens, 8 heads of 64: 44 us against 50), but at 256 elements the loop then has 1100 instructions, more than the
+  // scheduler's instruction cache holds: 134 us where one takes 111 (64 sequences, 4 heads).
+  static constexpr int kSub = D == 256 ? 1 : 2;
   static constexpr int kTile = 16 * kSub;
   static constexpr int kWarps = 8;
   static constexpr int kBlocks = NT == 1 ? 2 : 1;              // per SM
@@ -45,7 +46,7 @@ struct Shape {
   static constexpr int kPieces = D >= 128 ? D / 64 : 1;        // 16-byte key pieces per lane and tile
   static constexpr int kPart = 16 * D + 512;                   // bytes of 16 tokens: keys, values, pairs
   static constexpr int kStage = kSub * kPart;
-  static constexpr int kStages = D == 256 ? 2 : D == 128 ? 4 : 6;
+  static constexpr int kStages = D == 64 ? 3 : 2;
   static constexpr int kFold = kRows * (D + 4) * 4;            // a warp's partial result, in its ring's place
   static constexpr int kRing = kStages * kStage > kFold ? kStages * kStage : kFold;
   static constexpr int kQ = NT * D * 16;                       // query fragments
