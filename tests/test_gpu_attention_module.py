@@ -190,6 +190,34 @@ def test_stack_with_attention():
     stack.check_status()
 
 
+def test_stack_with_programmatic_launches():
+    stack = st.LinearStack(n_layers=8)
+    x = stack._plan(4)["x"]
+    rows = torch.randn(6, 4, st.HIDDEN, device="cuda").to(stack.dtype)
+
+    def run(flags, captured):
+        state, outs = st.AttentionState(stack, requests=4, max_len=40, page_size=16), []
+        if captured:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                stack.step(4, flags, attention=state)
+        for r in rows:
+            x.copy_(r)
+            if captured:
+                graph.replay()
+            else:
+                stack.step(4, flags, attention=state)
+            outs.append([state.out(i, 4).clone() for i in range(2)] + [b.clone() for b in stack._plan(4)["buffers"]])
+        torch.cuda.synchronize()
+        return outs
+
+    want = run(0, False)
+    for captured in (False, True):
+        got = run(pkg._lib.FLAG_PDL, captured)
+        assert all(torch.equal(a, b) for w, g in zip(want, got) for a, b in zip(w, g))
+    stack.check_status()
+
+
 def test_refusals():
     stack = st.LinearStack(n_layers=4)
     state = st.AttentionState(stack, requests=3, max_len=20)
