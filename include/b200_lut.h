@@ -584,12 +584,13 @@ typedef struct b200lut_kv_cache {
 /* What a step of a paged cache needs, from the requests' lengths on the device, in one launch.
  * Request b has cached[b] tokens and brings fresh[b] more (negative counts as 0). In the order of
  * the requests, pages that it does not have yet are taken from free_pages[*taken ..] and entered
- * into its row of block_table. A request whose pages do not fit its row or the free list, or whose
- * rows would end behind max_tokens, is not served: it gets no page and its slots are -1.
+ * into its row of block_table. A request whose pages do not fit its row or the free list, whose rows
+ * would end behind max_tokens, or that would pass 2^31 - 1 tokens, is not served: it gets no page and
+ * its slots are -1.
  * Results: row_start [B + 1] (clamped to max_tokens), kv_len [B] (cached + fresh where served, else
  * cached), positions and slots [max_tokens] (0 and -1 behind the last row; -1 also where the row
  * holds a negative page), taken_out [1], served [B] (bytes, 0 or 1). Calling it again with the same
- * inputs gives the same results. B <= 8192; cached + fresh < 2^31. */
+ * inputs gives the same results. B <= 8192. */
 typedef struct b200lut_kv_plan_args {
   const int32_t* cached;
   const int32_t* fresh;

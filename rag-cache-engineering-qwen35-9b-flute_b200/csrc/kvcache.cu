@@ -56,7 +56,8 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Plan
     }
     tok += before;
     const long long have = (cached + P - 1) >> p.page_log2, want = (cached + fresh + P - 1) >> p.page_log2;
-    const bool fits = b < p.B && want <= p.width && tok <= p.max_tokens;
+    // positions and lengths are 32-bit: past them a page index would be negative
+    const bool fits = b < p.B && want <= p.width && tok <= p.max_tokens && cached + fresh <= INT32_MAX;
     const long long need = fits ? want - have : 0;
     long long pg = need;
     for (int o = 1; o < 32; o <<= 1) {
@@ -99,7 +100,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Plan
       const int b = lo, cached = max(0, p.cached[b]);
       // of a request that is not the first in a clamped sum, the start is exact whenever t lies in it
       const int start = b ? end[b - 1] : 0;
-      pos = cached + (t - start);
+      pos = int(min((long long)cached + (t - start), (long long)INT32_MAX));
       if (base[b] != kUnserved) {
         const int j = pos >> p.page_log2;
         int* entry = p.table + (long long)b * p.width + j;
