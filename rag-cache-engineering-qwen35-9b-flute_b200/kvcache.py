@@ -28,6 +28,7 @@ from .rotary import check_heads, rows16
 __all__ = ["KVCache4", "StepPlan", "plan_step"]
 
 PAGE_SIZES = (16, 32, 64, 128, 256)
+INT_MAX = 2 ** 31 - 1
 
 
 class StepPlan(NamedTuple):
@@ -232,7 +233,7 @@ class KVCache4:
             a = _lib.AttendArgs(ctypes.pointer(self._view), q.data_ptr(), _lib.ptr(gate), out.data_ptr(),
                                 block_table.data_ptr(), kv_len.data_ptr(), _lib.ptr(row_start), q.stride(0), q.stride(1),
                                 gate.stride(0) if gate is not None else 0, gate.stride(1) if gate is not None else 0,
-                                out.stride(0), out.stride(1), block_table.stride(0), T, B, width, Hq, int(window),
-                                int(sinks), scale)
+                                out.stride(0), out.stride(1), block_table.stride(0), T, B, width, Hq, min(int(window), INT_MAX),
+                                min(int(sinks), INT_MAX), scale)      # no cache holds more tokens
             _lib.check(L.b200lut_attend(ctypes.byref(a), ws.data_ptr(), ws.numel(), _lib._stream(q)))
         return out

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from conftest import load_pkg
+from test_gpu_attend import Batch
 
 pkg = load_pkg()
 kv = pkg.kvcache
@@ -31,3 +32,17 @@ def test_plan_of_requests_that_would_pass_the_largest_length():
         assert step.slots.tolist() == [3 * page + 2] + want
         assert step.positions.min().item() >= 0
     assert (table == 3).all()
+
+
+@pytest.mark.parametrize("rows", (1, 30))
+def test_windows_and_sinks_beyond_32_bits(rows):
+    b = Batch([500], [rows], 4, 2, 128, 16)
+    want = b.check()
+    for window in (2 ** 31 - 1, 2 ** 31, 2 ** 32, 2 ** 32 + 100, 2 ** 70):
+        assert torch.equal(b.run(window=window), want), window
+        assert torch.equal(b.run(window=window, sinks=window), want), window
+    few = b.check(window=100)
+    assert not torch.equal(few, want)
+    for sinks in (2 ** 31, 2 ** 32, 2 ** 32 + 3, 2 ** 70):             # every token is among the first so many
+        assert torch.equal(b.run(window=100, sinks=sinks), b.run(window=100, sinks=500)), sinks
+        b.check(window=100, sinks=sinks)
