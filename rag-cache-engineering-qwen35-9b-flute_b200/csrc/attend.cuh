@@ -78,7 +78,7 @@ struct Span {
   __device__ Span() {}
   __device__ __forceinline__ Span(int first, int last, int len, int window, int sinks) {
     const int hi = min(len, last + 1);                       // tokens below hi
-    const int lo = window ? max(0, first - window + 1) : 0;
+    const int lo = window && first >= window ? first - window + 1 : 0;      // rows before the sequence: no difference wraps
     const int s = min(min(sinks, lo), max(hi, 0));
     sink_tiles = (s + kTile - 1) / kTile;
     main0 = max(lo / kTile, sink_tiles);
@@ -89,7 +89,7 @@ struct Span {
 };
 
 __device__ __forceinline__ bool token_seen(int j, int pos, int len, int window, int sinks) {
-  return j <= pos && j < len && (window == 0 || j > pos - window || j < sinks);
+  return j <= pos && j < len && (window == 0 || pos - j < window || j < sinks);
 }
 
 template <typename T>

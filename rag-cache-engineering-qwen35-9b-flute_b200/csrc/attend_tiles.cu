@@ -477,7 +477,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
         auto seen = [&](int c, int i, int k, int e) {
           const int col = 16 * c + 8 * i + 2 * t4 + e, j = first + col;
           return ((info[ps].valid[2 * half + (col >> 5)] >> (col & 31)) & 1u) && j <= pos[k] &&
-                 (p.window == 0 || j > pos[k] - p.window || j < p.sinks);
+                 (p.window == 0 || pos[k] - j < p.window || j < p.sinks);
         };
         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
         if (whole) {
@@ -816,7 +816,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
         }
       };
       auto seen = [&](int tok, int pg) {
-        return pg >= 0 && tok <= w.last_pos && (p.window == 0 || tok > w.first_pos - p.window || tok < p.sinks);
+        return pg >= 0 && tok <= w.last_pos && (p.window == 0 || w.first_pos < p.window || tok > w.first_pos - p.window || tok < p.sinks);
       };
       auto pairs = [&](int t) {                  // checks the pages too
         const int first = w.span.id(w.i0 + t) * kTile;

@@ -46,3 +46,15 @@ def test_windows_and_sinks_beyond_32_bits(rows):
     for sinks in (2 ** 31, 2 ** 32, 2 ** 32 + 3, 2 ** 70):             # every token is among the first so many
         assert torch.equal(b.run(window=100, sinks=sinks), b.run(window=100, sinks=500)), sinks
         b.check(window=100, sinks=sinks)
+
+
+@pytest.mark.parametrize("lengths,rows", [([5, 20], [9, 2]), ([2, 40], [3, 1]), ([0, 7], [1, 30])])
+def test_windows_near_two_to_the_31_with_rows_before_the_sequence(lengths, rows):
+    for D, Hq, H in ((128, 4, 2), (64, 2, 1), (256, 16, 1)):
+        b = Batch(lengths, rows, Hq, H, D, 16)
+        want = b.run()
+        assert want.any()
+        for window in (2 ** 31 - 1, 2 ** 31 - 2, 2 ** 31 - 9, 2 ** 30):
+            assert torch.equal(b.run(window=window), want), window
+            assert torch.equal(b.run(window=window, sinks=3), want), window
+    assert status() == 0
