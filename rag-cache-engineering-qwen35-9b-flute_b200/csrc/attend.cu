@@ -395,8 +395,9 @@ attend_rows_kernel(const __grid_constant__ AttendParams p) {
                 x[s][n][e] = fmaf(kk.y, (acc[s][n][0][e] + acc[s][n][1][e]) * qf[n][e & 1], kk.x * qs[n][e & 1]);
               }
           }
-          const bool whole = (missing & ((1u << kSub) - 1u)) == 0 && first + kTile <= first_pos + 1 && first + kTile <= rq.len &&
-                             (p.window == 0 || first > last_pos - p.window || first + kTile <= p.sinks);
+          // (first + kTile can be 2^31)
+          const bool whole = (missing & ((1u << kSub) - 1u)) == 0 && first <= first_pos + 1 - kTile && first <= rq.len - kTile &&
+                             (p.window == 0 || first > last_pos - p.window || first <= p.sinks - kTile);
           uint32_t hidden = 0;
           if (!whole) {
 #pragma unroll

@@ -80,11 +80,13 @@ struct Span {
     const int hi = min(len, last + 1);                       // tokens below hi
     const int lo = window && first >= window ? first - window + 1 : 0;      // rows before the sequence: no difference wraps
     const int s = min(min(sinks, lo), max(hi, 0));
-    sink_tiles = (s + kTile - 1) / kTile;
+    sink_tiles = tiles_of(s);
     main0 = max(lo / kTile, sink_tiles);
-    const int main1 = (max(hi, 0) + kTile - 1) / kTile;
+    const int main1 = tiles_of(max(hi, 0));
     tiles = max(1, sink_tiles + max(0, main1 - main0));
   }
+  // up to 2^31 - 1 tokens: the sum n + kTile - 1 would wrap
+  static __device__ __forceinline__ int tiles_of(int n) { return int((unsigned(n) + (kTile - 1)) / kTile); }
   __device__ __forceinline__ int id(int i) const { return i < sink_tiles ? i : main0 + i - sink_tiles; }
 };
 

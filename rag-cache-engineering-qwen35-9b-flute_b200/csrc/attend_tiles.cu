@@ -872,8 +872,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
           info[ps].sig = sig;
 #pragma unroll
           for (int j = 0; j < 4; ++j) info[ps].valid[j] = valid[j];
-          info[ps].whole = all && first + kTile <= w.first_pos + 1 &&
-                           (p.window == 0 || first > w.last_pos - p.window || first + kTile <= p.sinks);
+          info[ps].whole = all && first <= w.first_pos + 1 - kTile &&      // (first + kTile can be 2^31)
+                           (p.window == 0 || first > w.last_pos - p.window || first <= p.sinks - kTile);
         }
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(bar(kPrmFull + ps));

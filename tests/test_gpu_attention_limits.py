@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from conftest import load_pkg
+from helpers_attention import attend64, close, values64
 from test_gpu_attend import Batch
 
 pkg = load_pkg()
@@ -57,4 +58,26 @@ def test_windows_near_two_to_the_31_with_rows_before_the_sequence(lengths, rows)
         for window in (2 ** 31 - 1, 2 ** 31 - 2, 2 ** 31 - 9, 2 ** 30):
             assert torch.equal(b.run(window=window), want), window
             assert torch.equal(b.run(window=window, sinks=3), want), window
+    assert status() == 0
+
+
+@pytest.mark.parametrize("rows", (1, 2, 60))
+def test_the_longest_sequences(rows):
+    # a table of 2^23 pages of 256 tokens that names eight pages over and over; windows keep what is read short
+    H, D, page, window = 1, 64, 256, 700
+    cache = kv.KVCache4(8, H, D, page_size=page)
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    k, v = (torch.randn(8 * page, H, D, device="cuda", generator=g).bfloat16() for _ in range(2))
+    cache.write(k, v, torch.arange(8 * page, **INT))
+    table = (torch.arange(2 ** 23, **INT) % 8)[None]
+    q = torch.randn(rows, 2, D, device="cuda", generator=g).bfloat16()
+    start = torch.tensor([0, rows], **INT)
+    for short in (1, 2, 17, 130, 300):
+        n = 2 ** 31 - short
+        y = cache.attend(q, table, torch.tensor([n], **INT), None if rows == 1 else start, window=window)
+        # the last tokens as they lie in a short sequence: 2^31 is a multiple of what the table repeats
+        lies = torch.arange(8 * page - short - rows - window, 8 * page - short, device="cuda")
+        pos = torch.arange(window, window + rows, device="cuda")
+        want, tol = attend64(q, values64(k[lies]), values64(v[lies]), pos, D ** -0.5, window)
+        close(y, want, tol, str(short))
     assert status() == 0
