@@ -30,7 +30,6 @@ constexpr int kBadPage = 0x6200;
 constexpr int kItemCost = 24;
 constexpr float kLazy = 8.f;           // the running maximum may lag by this many powers of two
 constexpr uint32_t kOnes = 0x3C003C00u;     // two halves of 1
-constexpr float kMinStep = 7.888609e-31f;   // 2^-100
 
 template <int D, int NT>
 struct Shape {
@@ -90,10 +89,6 @@ __device__ __forceinline__ float ex2(float x) {
 __device__ __forceinline__ uint32_t half2_of(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
-}
-// the power of two >= x (x > 0, normal)
-__device__ __forceinline__ float pow2_above(float x) {
-  return __uint_as_float((__float_as_uint(x) + 0x007FFFFFu) & 0x7F800000u);
 }
 
 // Tiles of all items of request b (its row tiles are equal but for what they see).
@@ -317,7 +312,6 @@ attend_rows_kernel(const __grid_constant__ AttendParams p) {
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e) ws[n][e] = 0.f;
-        float sig = 0.f, inv_sig = 0.f;
 
         for (int k = 0; k < iters; ++k) {
           cp_wait<S::kStages - 2>();
@@ -417,44 +411,53 @@ attend_rows_kernel(const __grid_constant__ AttendParams p) {
               if (!seen[1]) v[s][1] = make_float2(0.f, 0.f);
             }
           }
-          float big = v[0][0].y;                 // largest step
+          float mid[kSub][2], big = kMinStep;    // the lane's largest token
 #pragma unroll
-          for (int s = 0; s < kSub; ++s) big = fmaxf(big, fmaxf(v[s][0].y, v[s][1].y));
-          bool grow = big > sig || sig == 0.f;
+          for (int s = 0; s < kSub; ++s)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              mid[s][i] = fmaf(7.5f, v[s][i].y, v[s][i].x);
+              big = fmaxf(big, token_size(v[s][i].y, mid[s][i]));
+            }
+          const float room = kLazy - size_in_m(big);
+          bool grow = false;
 #pragma unroll
           for (int s = 0; s < kSub; ++s)
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) grow |= x[s][n][e] > m[n][e & 1] + kLazy;
+              for (int e = 0; e < 4; ++e) grow |= x[s][n][e] > m[n][e & 1] + room;
           if (__any_sync(0xffffffffu, grow)) {
-            float vs = fmaxf(big, kMinStep);
+            float size[kSub][2];
 #pragma unroll
-            for (int s = 16; s; s >>= 1) vs = fmaxf(vs, __shfl_xor_sync(0xffffffffu, vs, s));
-            const float sig_new = fmaxf(sig, pow2_above(vs));
-            const float beta = sig / sig_new;
-            sig = sig_new;
-            inv_sig = 1.f / sig;
+            for (int s = 0; s < kSub; ++s)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) size[s][i] = size_in_m(token_size(v[s][i].y, mid[s][i]));
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
-                float top = fmaxf(x[0][n][e], x[0][n][e + 2]);
-                if constexpr (kSub == 2) top = fmaxf(top, fmaxf(x[kSub - 1][n][e], x[kSub - 1][n][e + 2]));
+                float top = fmaxf(x[0][n][e] + size[0][0], x[0][n][e + 2] + size[0][1]);
+                if constexpr (kSub == 2)
+                  top = fmaxf(top, fmaxf(x[kSub - 1][n][e] + size[kSub - 1][0], x[kSub - 1][n][e + 2] + size[kSub - 1][1]));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
                 const float m_new = fmaxf(m[n][e], top);
-                const float alpha = m_new == -INFINITY ? 1.f : ex2(m[n][e] - m_new);
+                const float root = m_new == -INFINITY ? 1.f : ex2(0.5f * (m[n][e] - m_new)), alpha = root * root;
                 m[n][e] = m_new;
-                l[n][e] *= alpha;
+                l[n][e] = l[n][e] * root * root;
                 pm[n][e] *= alpha;
-                const float ab = alpha * beta;
 #pragma unroll
-                for (int i = 0; i < D / 16; ++i) o[n][i][e] *= ab, o[n][i][e + 2] *= ab;
-                ws[n][e] *= ab;
+                for (int i = 0; i < D / 16; ++i) o[n][i][e] *= alpha, o[n][i][e + 2] *= alpha;
+                ws[n][e] *= alpha;
               }
           }
+          float off[NT][2];
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) off[n][e] = m[n][e] == -INFINITY ? 0.f : m[n][e];
           uint32_t bf[kSub][NT][2], rest[kSub][NT][2];
 #pragma unroll
           for (int s = 0; s < kSub; ++s)
@@ -463,13 +466,11 @@ attend_rows_kernel(const __grid_constant__ AttendParams p) {
               float w[4];
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                const float2 vv = v[s][e >> 1];
-                const float mm = m[n][e & 1];
-                const float pr = ex2(x[s][n][e] - (mm == -INFINITY ? 0.f : mm));
+                const float pr = ex2(x[s][n][e] - off[n][e & 1]);
                 const bool none = (hidden >> ((s * NT + n) * 4 + e)) & 1u;
                 l[n][e & 1] += pr;
-                pm[n][e & 1] += none ? 0.f : pr * fmaf(7.5f, vv.y, vv.x);
-                w[e] = none ? 0.f : pr * (vv.y * inv_sig);
+                pm[n][e & 1] += none ? 0.f : pr * mid[s][e >> 1];
+                w[e] = none ? 0.f : pr * v[s][e >> 1].y;
               }
               const uint32_t h0 = half2_of(w[0], w[1]), h1 = half2_of(w[2], w[3]);
               bf[s][n][0] = transpose8x8(h0);
@@ -525,10 +526,10 @@ attend_rows_kernel(const __grid_constant__ AttendParams p) {
             }
             const int r = n * 8 + 2 * t4 + e;
             if (g == 0) warp_ml[warp * kRows + r] = make_float2(m[n][e], l[n][e]);
-            const float back = 16777216.f * sig, mid = fmaf(-7.5f * sig, ws[n][e], pm[n][e]);
+            const float mid = fmaf(-7.5f, ws[n][e], pm[n][e]);
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) {
-              const float f = i & 1 ? back * 0.0625f : back;
+              const float f = i & 1 ? 1048576.f : 16777216.f;
               const int d = (i >> 2) * 64 + 8 * g + (i & 3);
               fold[r * (D + 4) + d] = fmaf(o[n][i][e], f, mid);
               fold[r * (D + 4) + d + 4] = fmaf(o[n][i][e + 2], f, mid);
@@ -546,9 +547,9 @@ attend_rows_kernel(const __grid_constant__ AttendParams p) {
 #pragma unroll
           for (int w = 0; w < kWarps; ++w) {
             const float2 ml = warp_ml[w * kRows + r];
-            const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : ex2(ml.x - top);
+            const float root = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : ex2(0.5f * (ml.x - top)), f = root * root;
             const float* part = reinterpret_cast<const float*>(ring + w * S::kRing) + r * (D + 4) + d;
-            sum = fmaf(ml.y, f, sum);
+            sum = fmaf(ml.y * root, root, sum);
             a = fmaf(part[0], f, a);
             c = fmaf(part[1], f, c);
           }
@@ -623,8 +624,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const __gr
           const float2 z = *reinterpret_cast<const float2*>(o + i);
           v[i] = z.x, v[i + 1] = z.y;
         }
-        const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : ex2(ml.x - top);
-        sum = fmaf(ml.y, f, sum);
+        const float root = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : ex2(0.5f * (ml.x - top)), f = root * root;
+        sum = fmaf(ml.y * root, root, sum);
 #pragma unroll
         for (int i = 0; i < kPer; ++i) x[i] = fmaf(v[i], f, x[i]);
       }

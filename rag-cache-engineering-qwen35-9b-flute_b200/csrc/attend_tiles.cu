@@ -13,8 +13,12 @@
 //   warp 21     one thread issues S = Q K^T (128 x 128, fp32 in tensor memory, two buffers) and O += P V (128 x D).
 //   warps 0-7   softmax, two warps for 32 rows (64 tokens each): scores from tensor memory, the token's two parameters
 //               applied as packed pairs, P back into the place of S as fp16 (the A operand of the second product).
-//               The running maximum may lag by 2^8 before O is rescaled, which then waits for the products in flight.
+//               The running maximum may lag by 2^8 before O is rescaled, which then waits for the products in flight. It is
+//               that of score + token's size (attend.cuh): bounded by the tile's largest score and size where the sizes are
+//               alike and every row sees them, by a pass of its own over the tile elsewhere.
 // Tensor memory: O in columns 0 .. D - 1, S in 256 .. 383 and 384 .. 511.
+#include <climits>
+
 #include "attend.cuh"
 #include "packed.cuh"
 #include "tc05.cuh"
@@ -34,7 +38,6 @@ constexpr int kParamStages = 4;
 // shares: an item's units are its cost, then its tiles.
 constexpr int kItemCost = 7;
 constexpr float kLazy = 8.f;
-constexpr float kMinStep = 7.888609e-31f;   // 2^-100
 constexpr int kBadPage = 0x6200;
 
 template <int D>
@@ -42,15 +45,16 @@ struct Shape {
   static constexpr int kStages = D == 256 ? 1 : 2;
   static constexpr int kOperand = 256 * D;                       // bytes of 128 x D halves
   static constexpr int kQ = 0, kK = kOperand, kV = kK + kStages * kOperand;
-  static constexpr int kParam = kV + kStages * kOperand;         // [stage][64 token pairs] of a, a, lo, lo and s, s, mid, mid
-  static constexpr int kParamBytes = 2 * 64 * 16;
+  // [stage][64 token pairs] of the keys' step, step, lo, lo; the values' step, step, mid, mid; then their sizes
+  static constexpr int kParam = kV + kStages * kOperand;
+  static constexpr int kParamBytes = 2 * 64 * 16 + 64 * 8;
   static constexpr int kEnd = kParam + kParamStages * kParamBytes;
   static constexpr int kSmem = kEnd + 1024;                      // the base is rounded up to 1024
 };
 
 struct TileInfo {
-  float sig;                   // power of two >= the largest step so far
-  int whole;                   // every row sees every token
+  float size;                  // of its largest token, as it adds to m
+  int whole;                   // every row sees every token; 2: and no token's size is below 2^-8 of the largest
   uint32_t valid[4];           // tokens that some row may see
   int page[8];                 // of each 16 tokens; -1: none
 };
@@ -59,9 +63,6 @@ __device__ __forceinline__ float ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
-}
-__device__ __forceinline__ float pow2_above(float x) {
-  return __uint_as_float((__float_as_uint(x) + 0x007FFFFFu) & 0x7F800000u);
 }
 __device__ __forceinline__ uint32_t half2_of(float2 a) {
   uint32_t r;
@@ -425,7 +426,6 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
         m_run[k] = -INFINITY;
         l2[k] = pm2[k] = make_float2(0.f, 0.f);
       }
-      float sig_run = 0.f;
       for (int t = 0; t < w.count; ++t) {
         const uint32_t m = w.n0 + uint32_t(t);
         const int ps = int(m % kParamStages), first = w.span.id(w.i0 + t) * kTile + 64 * half;
@@ -434,8 +434,9 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
         tc::fence_after_sync();
         const uint32_t mine = lane_base + 256 + 128 * (m & 1) + 64 * half;
         const float4* prm = reinterpret_cast<const float4*>(raw_sm + base_off + S::kParam + ps * S::kParamBytes) + 32 * half + t4;
-        const bool whole = info[ps].whole != 0;
-        const float sig_new = info[ps].sig;
+        const int state = info[ps].whole;
+        const bool whole = state != 0;
+        const float2* sizes = reinterpret_cast<const float2*>(raw_sm + base_off + S::kParam + ps * S::kParamBytes + 2048) + 32 * half + t4;
         auto pair = [](float x) { return make_float2(x, x); };
         // O's rows times ab: the two warps of a row do half of its columns each; the products in flight have to be through
         auto rescale = [&](const float (&ab)[4]) {
@@ -480,6 +481,9 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
                  (p.window == 0 || pos[k] - j < p.window || j < p.sinks);
         };
         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        // The maximum so far serves unless a score and its token's size are more than 2^8 above it.
+        bool look = !whole;
+        const bool even = state == 2;
         if (whole) {
 #pragma unroll 1
           for (int c = 0; c < 2; ++c) {
@@ -498,27 +502,39 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
                 top[k] = max3(top[k], y.x, y.y);
               }
           }
-        } else {
+          // a bound by the tile's largest token; it serves where the tokens' sizes are alike
+          bool over = false;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            top[k] = fmaf(top[k], qf[k], info[ps].size);
+            over |= top[k] > m_run[k] + kLazy;
+          }
+          look = pair_any(pair_bar, over);
+        }
+        if (look && !even) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) top[k] = -INFINITY;
 #pragma unroll 1
           for (int c = 0; c < 4; ++c) {
             fetch(c);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               const float4 kk = prm[8 * c + 4 * i];
+              const float2 size = sizes[8 * c + 4 * i];
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
-                const float2 y = score(kk, i, k);
+                const float2 y = fma2(score(kk, i, k), pair(qf[k]), size);
                 if (seen(c, i, k, 0)) top[k] = fmaxf(top[k], y.x);
                 if (seen(c, i, k, 1)) top[k] = fmaxf(top[k], y.y);
               }
             }
           }
-        }
-        // ---- the maximum so far serves unless a score of the tile is more than 2^8 above it
-        bool grow = sig_new != sig_run;
+          bool grow = false;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) grow = grow || top[k] * qf[k] > m_run[k] + kLazy;
-        if (pair_any(pair_bar, grow)) {
+          for (int k = 0; k < 4; ++k) grow = grow || top[k] > m_run[k] + kLazy;
+          look = pair_any(pair_bar, grow);
+        }
+        if (look) {
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 1));
@@ -529,14 +545,13 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
           float ab[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const float m_new = fmaxf(m_run[k], fmaxf(top[k], half_top[half ^ 1][row0 + g + 8 * k]) * qf[k]);
-            const float alpha = m_new == -INFINITY ? 1.f : ex2(m_run[k] - m_new);
-            ab[k] = alpha * (sig_run / sig_new);
+            const float m_new = fmaxf(m_run[k], fmaxf(top[k], half_top[half ^ 1][row0 + g + 8 * k]));
+            const float root = m_new == -INFINITY ? 1.f : ex2(0.5f * (m_run[k] - m_new));
+            ab[k] = root * root;
             m_run[k] = m_new;
-            l2[k] = mul2(l2[k], pair(alpha));
-            pm2[k] = mul2(pm2[k], pair(alpha));
+            l2[k] = mul2(mul2(l2[k], pair(root)), pair(root));
+            pm2[k] = mul2(pm2[k], pair(ab[k]));
           }
-          sig_run = sig_new;
           if (t > 0) rescale(ab);
         }
         // ---- P, at the head of this half's scores: columns that this warp has read by then
@@ -615,7 +630,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
       wait_pv(last);
       tc::fence_after_sync();
       const float l = half_sum[0][r].x + half_sum[1][r].x, pm = half_sum[0][r].y + half_sum[1][r].y;
-      const float back = 16777216.f * sig_run, inv = l == 0.f ? 0.f : 1.f / l;
+      const float back = 16777216.f, inv = l == 0.f ? 0.f : 1.f / l;
       const bool starts = w.i0 == 0, ends = w.i1 == w.span.tiles;
       const long long slot = 2LL * blockIdx.x + (starts ? 1 : 0);
       const int at = token_of(p, w.r0 + r), head = w.h * p.G + w.r0 + r - at * p.G;
@@ -804,7 +819,6 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
     const int page_mask = (1 << p.c.page_log2) - 1;
     items([&]() {
       const int* table = p.table + (long long)w.b * p.table_ld;
-      float sig = 0.f;                           // running power of two of the item
       int page[4], page_next[4];                 // this tile's, the next one's
       uint32_t kp[4], vp[4];                     // pairs of this tile
       auto pages = [&](int t, int (&to)[4]) {
@@ -841,7 +855,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
         const uint32_t m = w.n0 + uint32_t(t);
         const int ps = int(m % kParamStages), first = w.span.id(w.i0 + t) * kTile;
         float2 kk[4], vv[4];
-        float top = kMinStep;
+        int size[4], top = INT_MIN, least = INT_MAX;
         uint32_t valid[4];
         bool all = true;
 #pragma unroll
@@ -849,31 +863,32 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
           kk[j] = lo_step<T>(kp[j]), vv[j] = lo_step<T>(vp[j]);
           valid[j] = __ballot_sync(0xffffffffu, seen(first + 32 * j + lane, page[j]));
           all = all && valid[j] == 0xffffffffu;
-          top = fmaxf(top, vv[j].y);
+          size[j] = exponent_above(token_size(vv[j].y, fmaf(8.f, vv[j].y, vv[j].x)));
+          top = max(top, size[j]), least = min(least, size[j]);
         }
         int now[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) now[j] = page[j], page[j] = page_next[j];
         if (t + 1 < w.count) pairs(t + 1);      // under way while this tile's are written
         if (t + 2 < w.count) pages(t + 2, page_next);
-        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        sig = fmaxf(sig, pow2_above(top));
-        const float inv = 1.f / sig;
+        top = __reduce_max_sync(0xffffffffu, top), least = __reduce_min_sync(0xffffffffu, least);
         if (m >= kParamStages) wait(kPrmEmpty + ps, (m / kParamStages - 1) & 1u, tc::kStatusWaitEmpty);
         float* prm = reinterpret_cast<float*>(raw_sm + base_off + S::kParam + ps * S::kParamBytes);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int c = 32 * j + lane, at = (c >> 1) * 4 + (c & 1);
           prm[at] = kk[j].y, prm[at + 2] = kk[j].x;
-          prm[256 + at] = vv[j].y * inv, prm[256 + at + 2] = fmaf(8.f, vv[j].y, vv[j].x);
+          prm[256 + at] = vv[j].y, prm[256 + at + 2] = fmaf(8.f, vv[j].y, vv[j].x);
+          prm[512 + c] = float(size[j] - 7);
           if ((lane & 15) == 0) info[ps].page[2 * j + (lane >> 4)] = now[j];
         }
         if (lane == 0) {
-          info[ps].sig = sig;
+          info[ps].size = float(top - 7);
 #pragma unroll
           for (int j = 0; j < 4; ++j) info[ps].valid[j] = valid[j];
-          info[ps].whole = all && first <= w.first_pos + 1 - kTile &&      // (first + kTile can be 2^31)
+          const bool whole = all && first <= w.first_pos + 1 - kTile &&      // (first + kTile can be 2^31)
                            (p.window == 0 || first > w.last_pos - p.window || first <= p.sinks - kTile);
+          info[ps].whole = !whole ? 0 : top - least <= 8 ? 2 : 1;
         }
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(bar(kPrmFull + ps));

@@ -190,7 +190,7 @@ class KVCache4:
         h // (n_heads / n_kv_heads). scale: head_dim ** -0.5 unless given. gate: the result is multiplied by
         sigmoid(gate). Where nothing is visible the result is zero; rows that belong to no request are not written.
         A token on a page outside the cache counts as hidden and raises the device status (0x6200). The sums over tokens
-        are fp32 and divided at the end: values beyond 2^88 can come out infinite."""
+        are fp32 and divided at the end."""
         done = _lib.host.attend(self._native, q, block_table, kv_len, row_start,
                                 self.head_dim ** -0.5 if scale is None else scale, window, sinks, gate, out)
         if done is not None:
