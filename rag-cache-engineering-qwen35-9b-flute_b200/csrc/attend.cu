@@ -30,6 +30,9 @@ constexpr int kBadPage = 0x6200;
 constexpr int kItemCost = 24;
 constexpr float kLazy = 8.f;           // the running maximum may lag by this many powers of two
 constexpr uint32_t kOnes = 0x3C003C00u;     // two halves of 1
+// Scores and m are held divided by 2^13: the factor between a product of codes and its score, about 2^11 times the row's
+// largest element, then stays finite for every row that bf16 holds. The divisions are exact.
+constexpr float kScoreUnit = 8192.f;
 
 template <int D, int NT>
 struct Shape {
@@ -270,7 +273,7 @@ attend_rows_kernel(const __grid_constant__ AttendParams p) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             v[e] = DType<T>::to_float(uint16_t(u[e >> 1] >> (16 * (e & 1))));
-            top = fmaxf(top, fabsf(v[e])), sum += v[e];
+            top = fmaxf(top, fabsf(v[e])), sum = fmaf(v[e], kSumUnit, sum);
           }
           for (int o = 16; o; o >>= 1) {
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -286,7 +289,7 @@ attend_rows_kernel(const __grid_constant__ AttendParams p) {
             o.z = half2_of(v[2] * f, v[6] * f), o.w = half2_of(v[3] * f * 0.0625f, v[7] * f * 0.0625f);
             reinterpret_cast<uint4*>(sq)[((r >> 3) * S::kWords + w) * 32 + (r & 7) * 4 + tig] = o;
           }
-          if (lane == 0) row_k[r] = make_float2(p.scale * 16777216.f / f, p.scale * sum);
+          if (lane == 0) row_k[r] = make_float2(p.scale * (16777216.f / kScoreUnit / f), p.scale * sum * (1.f / kScoreUnit / kSumUnit));
         }
         __syncthreads();
 
@@ -419,7 +422,7 @@ attend_rows_kernel(const __grid_constant__ AttendParams p) {
               mid[s][i] = fmaf(7.5f, v[s][i].y, v[s][i].x);
               big = fmaxf(big, token_size(v[s][i].y, mid[s][i]));
             }
-          const float room = kLazy - size_in_m(big);
+          const float room = (kLazy - size_in_m(big)) * (1.f / kScoreUnit);
           bool grow = false;
 #pragma unroll
           for (int s = 0; s < kSub; ++s)
@@ -432,7 +435,7 @@ attend_rows_kernel(const __grid_constant__ AttendParams p) {
 #pragma unroll
             for (int s = 0; s < kSub; ++s)
 #pragma unroll
-              for (int i = 0; i < 2; ++i) size[s][i] = size_in_m(token_size(v[s][i].y, mid[s][i]));
+              for (int i = 0; i < 2; ++i) size[s][i] = size_in_m(token_size(v[s][i].y, mid[s][i])) * (1.f / kScoreUnit);
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -444,7 +447,7 @@ attend_rows_kernel(const __grid_constant__ AttendParams p) {
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
                 const float m_new = fmaxf(m[n][e], top);
-                const float root = m_new == -INFINITY ? 1.f : ex2(0.5f * (m[n][e] - m_new)), alpha = root * root;
+                const float root = m_new == -INFINITY ? 1.f : ex2(0.5f * kScoreUnit * (m[n][e] - m_new)), alpha = root * root;
                 m[n][e] = m_new;
                 l[n][e] = l[n][e] * root * root;
                 pm[n][e] *= alpha;
@@ -453,11 +456,11 @@ attend_rows_kernel(const __grid_constant__ AttendParams p) {
                 ws[n][e] *= alpha;
               }
           }
-          float off[NT][2];
+          float off[NT][2];                      // of a score beyond fp32 the weight is infinite or NaN
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) off[n][e] = m[n][e] == -INFINITY ? 0.f : m[n][e];
+            for (int e = 0; e < 2; ++e) off[n][e] = m[n][e] == -INFINITY ? 0.f : fmaxf(-3e38f, m[n][e] * -kScoreUnit);
           uint32_t bf[kSub][NT][2], rest[kSub][NT][2];
 #pragma unroll
           for (int s = 0; s < kSub; ++s)
@@ -466,7 +469,7 @@ attend_rows_kernel(const __grid_constant__ AttendParams p) {
               float w[4];
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                const float pr = ex2(x[s][n][e] - off[n][e & 1]);
+                const float pr = ex2(fmaf(x[s][n][e], kScoreUnit, off[n][e & 1]));
                 const bool none = (hidden >> ((s * NT + n) * 4 + e)) & 1u;
                 l[n][e & 1] += pr;
                 pm[n][e & 1] += none ? 0.f : pr * mid[s][e >> 1];
@@ -547,7 +550,7 @@ attend_rows_kernel(const __grid_constant__ AttendParams p) {
 #pragma unroll
           for (int w = 0; w < kWarps; ++w) {
             const float2 ml = warp_ml[w * kRows + r];
-            const float root = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : ex2(0.5f * (ml.x - top)), f = root * root;
+            const float root = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : ex2(0.5f * kScoreUnit * (ml.x - top)), f = root * root;
             const float* part = reinterpret_cast<const float*>(ring + w * S::kRing) + r * (D + 4) + d;
             sum = fmaf(ml.y * root, root, sum);
             a = fmaf(part[0], f, a);
@@ -562,7 +565,7 @@ attend_rows_kernel(const __grid_constant__ AttendParams p) {
             *reinterpret_cast<uint32_t*>(p.out + tok * p.out_token + (long long)head * p.out_head + d) = lo | (hi << 16);
           } else {
             *reinterpret_cast<float2*>(p.part_o + (slot * kRows + r) * D + d) = make_float2(a, c);
-            if (d == 0) p.part_ml[slot * kRows + r] = make_float2(top, sum);
+            if (d == 0) p.part_ml[slot * kRows + r] = make_float2(top * kScoreUnit, sum);
           }
         }
         if (starts && !ends && tid == 0) {

@@ -7,7 +7,8 @@
 // the probabilities, not the elements: nothing of K or V is rounded. A code needs one AND to become an
 // operand: in the low bits of a half it is the subnormal c * 2^-24, four bits higher c * 2^-20, both exact,
 // and the powers of two go into q and the result.
-// q is multiplied by the power of two that puts its row's largest element into [2^13, 2^14): fp16 then
+// q is multiplied by the power of two that puts its row's largest element into [2^13, 2^14), in the kernel for many
+// rows into [2^15, 2^16): fp16 then
 // holds bf16's eight bits exactly down to 2^-28 of the largest element (and fp16's eleven to 2^-25).
 // The weights w = p * step of the second product are rounded to fp16 (2^-11). p is 2^(s - m) with an m of the row's own
 // that follows s + log2(step) over the tokens the row sees (exponents rounded up, a lag of 2^8 allowed): w stays below
@@ -24,6 +25,9 @@
 #include "kvcache.cuh"
 
 namespace b200lut {
+
+// Sums of a row's elements are held in units of 2^9: finite for every row, and exact for the smallest elements too.
+constexpr float kSumUnit = 1.f / 512.f;
 
 struct AttendParams {
   const uint16_t* q;

@@ -38,6 +38,10 @@ constexpr int kParamStages = 4;
 // shares: an item's units are its cost, then its tiles.
 constexpr int kItemCost = 7;
 constexpr float kLazy = 8.f;
+// A row is scaled to [2^15, 2^16) and the keys' parameters are held multiplied by 2^6: the factor between what the two
+// make and a score, about 2^3 scale times the row's largest element, is finite for every row that bf16 holds (up to a
+// scale of 1/8, for the larger ones up to 2^127 / (8 scale)). Nearly equal keys beyond 2^122 have no room for it.
+constexpr float kKeyUnit = 64.f;
 constexpr int kBadPage = 0x6200;
 
 template <int D>
@@ -371,14 +375,14 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             v[e] = DType<T>::to_float(uint16_t(u[e >> 1] >> (16 * (e & 1))));
-            top = fmaxf(top, fabsf(v[e])), sum += v[e];
+            top = fmaxf(top, fabsf(v[e])), sum = fmaf(v[e], kSumUnit, sum);
           }
           for (int o = 16; o; o >>= 1) {
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
             sum += __shfl_xor_sync(0xffffffffu, sum, o);
           }
           const int ex = int(__float_as_uint(top) >> 23);
-          const int fe = ex == 255 || top == 0.f ? 127 : max(24, min(254, 127 + 13 + 127 - ex));   // 2^24 / f stays finite
+          const int fe = ex == 255 || top == 0.f ? 127 : min(254, 127 + 15 + 127 - ex);
           const float f = __uint_as_float(uint32_t(fe) << 23), fs = p.scale < 0.f ? -f : f;
           if (lane < kChunks) {
             uint32_t o[4];
@@ -390,7 +394,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
             sts128(sm + S::kQ + (lane >> 3) * (kRows * 128) + r * 128 + (((lane & 7) ^ (r & 7)) << 4), o[0], o[1], o[2], o[3]);
           }
           if (lane == 0)
-            row_k[r] = make_float2(fmaxf(fabsf(p.scale) * (16777216.f / f), 1.17549435e-38f), sum * fs * 5.9604645e-8f);
+            row_k[r] = make_float2(fmaxf(fabsf(p.scale) * 512.f * (32768.f / kKeyUnit / f), 1.17549435e-38f),
+                                   sum * fs * (5.9604645e-8f / kSumUnit));
         }
       }
       tc::fence_proxy_async();
@@ -877,7 +882,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int c = 32 * j + lane, at = (c >> 1) * 4 + (c & 1);
-          prm[at] = kk[j].y, prm[at + 2] = kk[j].x;
+          prm[at] = kk[j].y * kKeyUnit, prm[at + 2] = kk[j].x * kKeyUnit;
           prm[256 + at] = vv[j].y, prm[256 + at + 2] = fmaf(8.f, vv[j].y, vv[j].x);
           prm[512 + c] = float(size[j] - 7);
           if ((lane & 15) == 0) info[ps].page[2 * j + (lane >> 4)] = now[j];

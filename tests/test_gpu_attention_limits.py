@@ -81,3 +81,20 @@ def test_the_longest_sequences(rows):
         want, tol = attend64(q, values64(k[lies]), values64(v[lies]), pos, D ** -0.5, window)
         close(y, want, tol, str(short))
     assert status() == 0
+
+
+@pytest.mark.parametrize("D,Hq,H", [(64, 2, 1), (128, 4, 1), (256, 8, 2)])
+@pytest.mark.parametrize("rows", (1, 40))
+def test_queries_up_to_the_largest(rows, D, Hq, H):
+    # queries of up to 2^127 over keys so small that the scores are ordinary
+    for e in (63, 64, 110, 117, 119, 121, 124, 126):
+        b = Batch([200, 30], [rows, 1], Hq, H, D, 16, seed=e)
+        b.q[0] = (b.q[0].float().clamp(-1.99, 1.99) * 2.0 ** e).bfloat16()
+        b.q[-1] = b.q[-1].abs().clamp(0.5, 1.99)                       # their plain sum passes what fp32 holds
+        b.q[-1] = (b.q[-1].float() * 2.0 ** 126).bfloat16()
+        b.k[0] = (b.k[0].float() * 2.0 ** -e).bfloat16()
+        b.k[1] = (b.k[1].float() * 2.0 ** -126).bfloat16()
+        b.cache.write(torch.cat(b.k), torch.cat(b.v), b.slots)
+        y = b.check()
+        assert y.isfinite().all()
+        b.check(scale=-0.3)
