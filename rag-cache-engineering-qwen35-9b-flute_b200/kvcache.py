@@ -221,8 +221,10 @@ class KVCache4:
             gate = self._rows("gate", gate, Hq)
         if out is None:
             out = torch.empty(T, Hq, D, dtype=self.dtype, device=self.device)
-        elif (tuple(out.shape) != (T, Hq, D) or out.dtype != self.dtype or out.device != self.device
-              or rows16(out) is not out):
+        to = None
+        if tuple(out.shape) == (T, Hq, D) and out.dtype == self.dtype and out.device == self.device:
+            to = rows16(out)
+        if to is None or to.data_ptr() != out.data_ptr():
             raise ValueError(f"out must be [{T}, {Hq}, {D}] {self.dtype} on {self.device} with 16-byte rows")
         if T == 0 or B == 0:
             return out
@@ -230,10 +232,10 @@ class KVCache4:
         with _lib._on_device(self.device):
             # a buffer of the current stream (of the capture's pool under capture): calls never share one
             ws = torch.empty(L.b200lut_attend_workspace_bytes(Hq, self.n_kv_heads, D, int(row_start is None)), dtype=torch.uint8, device=self.device)
-            a = _lib.AttendArgs(ctypes.pointer(self._view), q.data_ptr(), _lib.ptr(gate), out.data_ptr(),
+            a = _lib.AttendArgs(ctypes.pointer(self._view), q.data_ptr(), _lib.ptr(gate), to.data_ptr(),
                                 block_table.data_ptr(), kv_len.data_ptr(), _lib.ptr(row_start), q.stride(0), q.stride(1),
                                 gate.stride(0) if gate is not None else 0, gate.stride(1) if gate is not None else 0,
-                                out.stride(0), out.stride(1), block_table.stride(0), T, B, width, Hq, min(int(window), INT_MAX),
+                                to.stride(0), to.stride(1), block_table.stride(0), T, B, width, Hq, min(int(window), INT_MAX),
                                 min(int(sinks), INT_MAX), scale)      # no cache holds more tokens
             _lib.check(L.b200lut_attend(ctypes.byref(a), ws.data_ptr(), ws.numel(), _lib._stream(q)))
         return out

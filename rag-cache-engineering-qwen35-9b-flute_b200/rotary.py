@@ -21,9 +21,13 @@ __all__ = ["AxisRotary"]
 def rows16(x: torch.Tensor) -> torch.Tensor:
     """x [T, heads, D] as the kernels read it: 16-byte rows, any token and head stride (a copy where
     its strides or its address do not allow that)."""
+    if x.shape[0] == 1 or x.shape[1] == 1:          # the stride of a single token or head says nothing, and may be anything
+        token, head = (0 if n == 1 else s for n, s in zip(x.shape[:2], x.stride()))
+        if (token, head) != x.stride()[:2]:
+            x = x.as_strided(x.shape, (token, head, x.stride(2)))
     if x.stride(2) == 1 and x.stride(0) % 8 == 0 and x.stride(1) % 8 == 0 and x.data_ptr() % 16 == 0:
         return x
-    return x.contiguous() if x.data_ptr() % 16 == 0 or not x.is_contiguous() else x.clone()
+    return torch.empty(x.shape, dtype=x.dtype, device=x.device).copy_(x)
 
 
 def check_heads(name: str, x: torch.Tensor, heads: Optional[int], D: Optional[int]) -> None:

@@ -98,3 +98,37 @@ def test_queries_up_to_the_largest(rows, D, Hq, H):
         y = b.check()
         assert y.isfinite().all()
         b.check(scale=-0.3)
+
+
+def test_single_tokens_and_heads_in_rows_of_odd_strides():
+    bf = torch.bfloat16
+    rot = pkg.rotary.AxisRotary(64, theta=1e4)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    wide = torch.randn(5, 4 * 128 + 1 * 128 + 3, device="cuda", generator=g).to(bf)
+    q, k = wide[:, :512].unflatten(1, (4, 128))[:1], wide[:, 512:640].unflatten(1, (1, 128))[:1]
+    assert q.stride(0) % 8 and k.stride(0) % 8 and q.is_contiguous()
+    pos = torch.tensor([77], device="cuda")
+    for _ in range(2):                                  # with and without the rotation's tables in place
+        assert all(torch.equal(a, b) for a, b in zip(rot(q, k, pos), rot(q.clone(memory_format=torch.contiguous_format).reshape(1, 4, 128),
+                                                                         torch.empty_like(k).copy_(k), pos)))
+    cache, plain = (kv.KVCache4(2, 1, 128, page_size=16) for _ in range(2))
+    slot = torch.tensor([5], **INT)
+    cache.write(k, k, slot)
+    dense = torch.empty(1, 1, 128, device="cuda", dtype=bf).copy_(k)
+    plain.write(dense, dense, slot)
+    assert all(torch.equal(a, b) for a, b in zip(cache.read(slot), plain.read(slot))) and cache.read(slot)[0].any()
+    table, n = torch.tensor([[0]], **INT), torch.tensor([6], **INT)
+    dense = torch.empty(1, 4, 128, device="cuda", dtype=bf).copy_(q)
+    want = plain.attend(dense, table, n, gate=dense)
+    out = torch.zeros(2, 4 * 128 + 1, device="cuda", dtype=bf)
+    to = out[:, :512].unflatten(1, (4, 128))[:1]
+    assert to.stride(0) % 8
+    assert torch.equal(cache.attend(q, table, n, gate=q), want)
+    assert cache.attend(q, table, n, gate=q, out=to) is to and torch.equal(to, want) and not out[1].any() and not out[0, 512]
+    odd = torch.zeros(2 * 513, device="cuda", dtype=bf)[1:].as_strided((1, 4, 128), (513, 128, 1))
+    with pytest.raises(ValueError, match="16-byte"):
+        cache.attend(q, table, n, out=odd)
+    # one head, odd strides between tokens' heads
+    one = torch.randn(3, 2, 136, device="cuda", generator=g).to(bf)[:, :1, :128]
+    cache.write(one, one, torch.arange(3, **INT))
+    assert cache.read(torch.arange(3, **INT))[0].any()
