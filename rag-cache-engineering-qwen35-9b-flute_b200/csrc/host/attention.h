@@ -275,7 +275,7 @@ PyObject* rotary(Guard&& guarded, Context&& context, PyObject* const* a, Py_ssiz
       if (a[3 + i] == Py_None) continue;
       const at::Tensor* t = gain[i];
       if (!t || !t->is_cuda() || t->get_device() != device || t->scalar_type() != st || t->dim() != 1 || t->size(0) != D ||
-          t->stride(0) != 1 || (reinterpret_cast<uintptr_t>(t->const_data_ptr()) & 15))
+          t->stride(0) != 1 || !plain(*t) || (reinterpret_cast<uintptr_t>(t->const_data_ptr()) & 15))
         Py_RETURN_NONE;
     }
     if (!context(device, false, &x)) Py_RETURN_NONE;

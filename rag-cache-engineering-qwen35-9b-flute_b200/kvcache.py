@@ -23,7 +23,7 @@ from typing import NamedTuple, Optional, Tuple
 import torch
 
 from . import _lib
-from .rotary import check_heads, rows16
+from .rotary import check_heads, check_no_grad, rows16
 
 __all__ = ["KVCache4", "StepPlan", "plan_step"]
 
@@ -199,6 +199,8 @@ class KVCache4:
             raise ValueError(f"q must be [tokens, a multiple of {self.n_kv_heads} heads, {self.head_dim}], got {tuple(q.shape)}")
         q = self._rows("q", q, q.shape[1])
         T, Hq, D = q.shape
+        if out is not None:
+            check_no_grad("out", out)
         if Hq // self.n_kv_heads > 64:
             raise ValueError(f"at most 64 query heads per key/value head, got {Hq // self.n_kv_heads}")
         _ints("block_table", block_table, (None, None), self.device)

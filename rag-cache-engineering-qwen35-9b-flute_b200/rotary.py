@@ -30,6 +30,11 @@ def rows16(x: torch.Tensor) -> torch.Tensor:
     return torch.empty(x.shape, dtype=x.dtype, device=x.device).copy_(x)
 
 
+def check_no_grad(name: str, x: torch.Tensor) -> None:
+    if x.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{name} requires grad: autograd is not served on the attention side")
+
+
 def check_heads(name: str, x: torch.Tensor, heads: Optional[int], D: Optional[int]) -> None:
     _lib._need_cuda(x, name)
     if x.dim() != 3 or (heads is not None and x.shape[1] != heads) or (D is not None and x.shape[2] != D):
@@ -37,8 +42,7 @@ def check_heads(name: str, x: torch.Tensor, heads: Optional[int], D: Optional[in
                          f"{'head_dim' if D is None else D}], got {tuple(x.shape)}")
     if x.dtype not in (torch.bfloat16, torch.float16):
         raise TypeError(f"{name} must be bfloat16 or float16, got {x.dtype}")
-    if x.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError(f"{name} requires grad: autograd is not served on the attention side")
+    check_no_grad(name, x)
 
 
 class AxisRotary:
@@ -102,7 +106,8 @@ class AxisRotary:
                  k_gain: Optional[torch.Tensor] = None, eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor]:
         """q [tokens, heads, D] and k [tokens, kv_heads, D], D in {64, 128, 256}, rotated into new
         contiguous tensors. positions: int32 or int64, [axes, tokens] or [tokens]. q_gain, k_gain: [D] in
-        q's dtype, both or neither."""
+        q's dtype, both or neither. Nothing is differentiated: inputs and gains that require grad are refused
+        while grad mode is on."""
         tables = self._tables.get(q.device)
         if tables is not None:
             done = _lib.host.rotary(q, k, positions, q_gain, k_gain, eps, *tables, self.axes)
@@ -123,6 +128,7 @@ class AxisRotary:
             for name, g in (("q_gain", q_gain), ("k_gain", k_gain)):
                 if tuple(g.shape) != (D,) or g.dtype != q.dtype or g.device != q.device:
                     raise ValueError(f"{name} must be [{D}] in q's dtype on q's device")
+                check_no_grad(name, g)
             q_gain, k_gain = (g.contiguous() if g.data_ptr() % 16 == 0 else g.clone() for g in (q_gain, k_gain))
         q, k = rows16(q), rows16(k)
         if positions.stride(-1) != 1 and T > 1:
