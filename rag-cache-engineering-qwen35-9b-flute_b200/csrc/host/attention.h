@@ -2,6 +2,8 @@
 // rule. Anything else returns None, nothing launched, and the Python route converts it or refuses it.
 #pragma once
 
+#include <c10/core/AutogradState.h>
+
 #include "route.h"
 
 namespace b200host {
@@ -24,7 +26,11 @@ inline void cache_dealloc(PyObject* o) {
 
 inline const at::Tensor* tensor_of(PyObject* o) { return THPVariable_Check(o) ? &THPVariable_Unpack(o) : nullptr; }
 
-inline bool plain(const at::Tensor& t) { return !(t.requires_grad() && c10::GradMode::is_enabled()); }
+// no gradient to lose, backward or forward
+inline bool plain(const at::Tensor& t) {
+  return !(t.requires_grad() && c10::GradMode::is_enabled()) &&
+         !(t._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode());
+}
 
 // [tokens, heads, D] in `scalar` with rows of 16 bytes.
 inline bool head_rows(const at::Tensor& t, at::ScalarType scalar, int device, int64_t heads, int64_t D) {

@@ -12,6 +12,7 @@ import threading
 from typing import Optional, Sequence, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -33,6 +34,8 @@ def rows16(x: torch.Tensor) -> torch.Tensor:
 def check_no_grad(name: str, x: torch.Tensor) -> None:
     if x.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{name} requires grad: autograd is not served on the attention side")
+    if torch._C._is_fwd_grad_enabled() and forward_ad.unpack_dual(x).tangent is not None:
+        raise RuntimeError(f"{name} carries a forward-mode tangent: autograd is not served on the attention side")
 
 
 def check_heads(name: str, x: torch.Tensor, heads: Optional[int], D: Optional[int]) -> None:

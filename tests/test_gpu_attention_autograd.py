@@ -3,6 +3,7 @@ from __future__ import annotations
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from conftest import load_pkg
 
@@ -37,3 +38,27 @@ def test_results_into_a_buffer_that_requires_grad():
         cache.attend(q, t, n, out=out)
     with torch.no_grad():
         assert cache.attend(q, t, n, out=out) is out
+
+
+def test_forward_mode_tangents():
+    rot = pkg.rotary.AxisRotary(64).to("cuda")
+    cache = pkg.kvcache.KVCache4(2, 2, 64, page_size=16)
+    q, k, g = rows(3, 4), rows(3, 2), torch.ones(64, dtype=torch.bfloat16, device="cuda")
+    pos, slots = torch.arange(3, device="cuda"), torch.arange(3, **INT)
+    table, n, start = torch.zeros(1, 1, **INT), torch.full((1,), 3, **INT), torch.tensor([0, 3], **INT)
+    with forward_ad.dual_level():
+        def dual(x):
+            return forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: rot(dual(q), k, pos), lambda: rot(q, dual(k), pos), lambda: rot(q, k, pos, dual(g), g),
+                     lambda: rot(q, k, pos, g, dual(g)), lambda: cache.write(dual(k), k, slots), lambda: cache.write(k, dual(k), slots),
+                     lambda: cache.attend(dual(q), table, n, start), lambda: cache.attend(q, table, n, start, gate=dual(q)),
+                     lambda: cache.attend(q, table, n, start, out=dual(q.clone()))):
+            with pytest.raises(RuntimeError, match="tangent"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="tangent"):     # no_grad leaves forward mode on
+                call()
+            with torch.inference_mode():
+                call()
+        rot(q, k, pos)                                 # others' tangents are no matter
+        cache.write(k, k, slots)
+        cache.attend(q, table, n, start)
