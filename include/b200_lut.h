@@ -77,7 +77,9 @@ const char* b200lut_last_error(void);
  * with its tensor memory freed and its output undefined). Synchronises the device
  * read; clears the word. No counterpart in the reference (its kernels never wait).
  * 0x6000: an embedding gather met an id outside its table (that row was written as zeros);
- * 0x6100: a slot, 0x6200: a page outside a key/value cache; 0x63xx: a wait of the attention over it. */
+ * 0x6100: a slot, 0x6200: a page outside a key/value cache; 0x63xx: a wait of the attention over it.
+ * The words of slots and pages are cleared one at a time, when they are returned: 0 says that nothing
+ * is left. */
 int b200lut_device_status(void);
 
 /* Number of SMs of the current device (used by the split policy). */

@@ -733,11 +733,12 @@ size_t workspace_bytes_of(int G, int D, bool one_row_each, int sms) {
 
 }  // namespace
 
-int attend_status_take() {
+int attend_page_take() {
   int v = 0, zero = 0;
   if (cudaMemcpyFromSymbol(&v, g_attend_status, sizeof(int)) != cudaSuccess) return -1;
   if (v != 0) cudaMemcpyToSymbol(g_attend_status, &zero, sizeof(int));
-  return v;
+  const int tiles = attend_tiles_page_take();        // one word to the caller
+  return v != 0 ? v : tiles;
 }
 
 }  // namespace b200lut

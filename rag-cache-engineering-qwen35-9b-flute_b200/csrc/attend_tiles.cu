@@ -26,7 +26,8 @@
 namespace b200lut {
 namespace {
 
-__device__ int g_tiles_status = 0;
+__device__ int g_tiles_status = 0;       // of a wait that gave up
+__device__ int g_tiles_page = 0;         // of a page outside the cache
 constexpr int kRows = 128, kTile = 128;
 constexpr int kThreads = 768, kWarps = kThreads / 32;
 constexpr int kValueWarp = 8, kKeyWarp = 16, kParamWarp = 20, kProductWarp = 21;
@@ -843,7 +844,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
         for (int j = 0; j < 4; ++j) {
           const int tok = first + 32 * j + lane;
           if (tok < w.rq.len && unsigned(page[j]) >= unsigned(p.c.n_pages)) {
-            atomicExch(&g_tiles_status, kBadPage);
+            atomicExch(&g_tiles_page, kBadPage);
             page[j] = -1;
           }
           kp[j] = vp[j] = 0;
@@ -971,7 +972,13 @@ int attend_tiles_status_take() {
   int v = 0, zero = 0;
   if (cudaMemcpyFromSymbol(&v, g_tiles_status, sizeof(int)) != cudaSuccess) return -1;
   if (v != 0) cudaMemcpyToSymbol(g_tiles_status, &zero, sizeof(int));
-  return v == kBadPage || v == 0 ? v : 0x6300 + v;
+  return v == 0 ? 0 : 0x6300 + v;
+}
+int attend_tiles_page_take() {
+  int v = 0, zero = 0;
+  if (cudaMemcpyFromSymbol(&v, g_tiles_page, sizeof(int)) != cudaSuccess) return -1;
+  if (v != 0) cudaMemcpyToSymbol(g_tiles_page, &zero, sizeof(int));
+  return v;
 }
 
 int attend_tiles(const AttendParams& p, int dtype, int blocks, cudaStream_t st) {

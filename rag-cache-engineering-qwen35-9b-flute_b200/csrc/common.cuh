@@ -103,9 +103,11 @@ long long gemm_wait_cycles();
 bool cluster_gemm_serves(int M, int row_tiles, int K, int bits, int group_size, int chain_limit);
 // Status word of the embedding gather (an id outside the table): value and clear.
 int embed_status_take();
-// Status words of the key/value cache (a slot outside it) and of the attention over it (a page outside it).
+// Status words of the key/value cache (a slot outside it) and of the attention over it: a wait that gave up, a page
+// outside the cache (attend_page_take: of both kernels).
 int kv_status_take();
-int attend_status_take();
 int attend_tiles_status_take();
+int attend_tiles_page_take();
+int attend_page_take();
 
 }  // namespace b200lut

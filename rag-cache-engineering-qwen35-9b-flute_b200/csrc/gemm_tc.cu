@@ -1037,7 +1037,8 @@ using namespace b200lut;
 
 // Device-side status of the library's kernels on the current device (0 = none). A
 // non-zero value means a bounded wait ran out inside a kernel (tensor-core pipeline codes,
-// or 0x7000 + rank for an exchange wait on that rank's push); cleared by this call.
+// or 0x7000 + rank for an exchange wait on that rank's push), or an id, a slot or a page that is none.
+// What waits and ids left is cleared by this call; a slot's and a page's word stays until it is returned.
 extern "C" int b200lut_device_status(void) {
   int v = 0, zero = 0;
   if (cudaMemcpyFromSymbol(&v, g_gemm_status, sizeof(int)) != cudaSuccess) return -1;
@@ -1045,10 +1046,11 @@ extern "C" int b200lut_device_status(void) {
   const int e = b200lut::exchange_status_take();
   const int g = b200lut::embed_status_take();
   const int c = b200lut::gemm_cluster_status_take();
-  const int s = b200lut::kv_status_take();
-  const int a = b200lut::attend_status_take();
-  const int at = b200lut::attend_tiles_status_take();
-  return v != 0 ? v : c != 0 ? c : e != 0 ? e : g != 0 ? g : s != 0 ? s : at != 0 ? at : a;
+  const int t = b200lut::attend_tiles_status_take();
+  const int first = v != 0 ? v : c != 0 ? c : e != 0 ? e : t != 0 ? t : g;
+  if (first != 0) return first;
+  const int slot = b200lut::kv_status_take();
+  return slot != 0 ? slot : b200lut::attend_page_take();
 }
 
 namespace {

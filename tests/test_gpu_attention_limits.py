@@ -132,3 +132,17 @@ def test_single_tokens_and_heads_in_rows_of_odd_strides():
     one = torch.randn(3, 2, 136, device="cuda", generator=g).to(bf)[:, :1, :128]
     cache.write(one, one, torch.arange(3, **INT))
     assert cache.read(torch.arange(3, **INT))[0].any()
+
+
+@pytest.mark.parametrize("rows", (1, 40))
+def test_a_bad_slot_does_not_hide_a_bad_page(rows):
+    b = Batch([80], [rows], 8, 2, 128, 16)
+    assert status() == 0
+    b.cache.write(b.k[0][:2], b.v[0][:2], torch.tensor([-1, b.cache.n_pages * 16], **INT))
+    b.table[0, 1] = b.cache.n_pages
+    b.run()
+    assert [status() for _ in range(3)] == [0x6100, 0x6200, 0]
+    two = Batch([80, 300], [1, 40], 8, 2, 128, 16)          # both kernels of one call: one word
+    two.table[:, 1] = -1
+    two.run()
+    assert [status() for _ in range(2)] == [0x6200, 0]
