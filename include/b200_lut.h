@@ -626,8 +626,8 @@ int b200lut_kv_read(const b200lut_kv_cache* cache, void* k, void* v, const int32
  * row at position p sees the tokens j <= p with window == 0, j > p - window or j < sinks. Query
  * head h reads key/value head h / (n_heads / n_kv_heads). out = softmax(scale q k^T) v, times
  * sigmoid(gate) with a gate; zeros where nothing is visible. Rows of q that belong to no request
- * are not written. row_start NULL: one row per request (T == B). Tokens on a page outside the
- * cache count as hidden and raise the device status (0x6200). */
+ * are not written. row_start NULL: one row per request (T == B). Visible tokens on a page outside
+ * the cache count as hidden and raise the device status (0x6200). */
 typedef struct b200lut_attend_args {
   const b200lut_kv_cache* cache;
   const void* q;

@@ -250,7 +250,10 @@ attend_rows_kernel(const __grid_constant__ AttendParams p) {
                 cp4(pd + 12, vp_at + pair + 2);
               } else {
                 bad |= bit;
-                if (first < rq.len && lane == 0) atomicExch(&g_attend_status, kBadPage);
+                // a page that no row sees a token of (behind the window, say) may be anything
+                if (lane == 0 && first < rq.len && first <= last_pos &&
+                    (p.window == 0 || first_pos < p.window || first + 15 > first_pos - p.window || first < p.sinks))
+                  atomicExch(&g_attend_status, kBadPage);
               }
             }
           }

@@ -843,12 +843,13 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const __grid_
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int tok = first + 32 * j + lane;
-          if (tok < w.rq.len && unsigned(page[j]) >= unsigned(p.c.n_pages)) {
-            atomicExch(&g_tiles_page, kBadPage);
+          const bool visible = seen(tok, 0);       // a page that no row sees may be anything
+          if (unsigned(page[j]) >= unsigned(p.c.n_pages)) {
+            if (visible) *static_cast<volatile int*>(&g_tiles_page) = kBadPage;      // (whoever writes writes this)
             page[j] = -1;
           }
           kp[j] = vp[j] = 0;
-          if (seen(tok, page[j])) {
+          if (visible && page[j] >= 0) {
             const long long at = cache_pair_at(page[j], w.h, p.c.heads, p.c.page_log2, tok & page_mask);
             kp[j] = __ldg(p.c.k_pair + at), vp[j] = __ldg(p.c.v_pair + at);
           }

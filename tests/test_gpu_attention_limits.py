@@ -146,3 +146,20 @@ def test_a_bad_slot_does_not_hide_a_bad_page(rows):
     two.table[:, 1] = -1
     two.run()
     assert [status() for _ in range(2)] == [0x6200, 0]
+
+
+@pytest.mark.parametrize("Hq,H,D,page", [(4, 2, 64, 16), (8, 2, 128, 16), (8, 2, 256, 32), (2, 1, 128, 64)])
+@pytest.mark.parametrize("rows", (1, 3, 50))
+def test_pages_that_no_row_sees_may_be_given_away(rows, Hq, H, D, page):
+    for n in (500, 507, 511, 530):
+        for window, sinks in ((20, 0), (33, 4), (100, 70)):
+            b = Batch([n, 40], [rows, 1], Hq, H, D, page, seed=n)
+            want = b.run(window=window, sinks=sinks)
+            assert status() == 0
+            kept = -(-sinks // page)
+            b.table[0, kept:(n - rows - window + 1) // page] = -1
+            assert torch.equal(b.run(window=window, sinks=sinks), want)
+            assert status() == 0
+            b.table[0, (n - rows - window + 1) // page] = -1            # the first row sees a token of it
+            b.run(window=window, sinks=sinks)
+            assert status() == 0x6200 and status() == 0
