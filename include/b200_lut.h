@@ -640,7 +640,7 @@ typedef struct b200lut_attend_args {
   int64_t out_token_stride, out_head_stride, table_stride;
   int T, B, width, n_heads;
   int window, sinks;
-  float scale;
+  float scale;                 /* below 2^127 */
 } b200lut_attend_args;
 /* one_row_each: the call comes without row_start. 0 on invalid sizes. */
 size_t b200lut_attend_workspace_bytes(int n_heads, int n_kv_heads, int head_dim, int one_row_each);

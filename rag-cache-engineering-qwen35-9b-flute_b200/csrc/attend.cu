@@ -765,6 +765,7 @@ extern "C" int b200lut_attend(const b200lut_attend_args* a, void* workspace, siz
                   "attend: at most 64 query heads per key/value head (got %d)", a->n_heads / p.c.heads);
   B200LUT_REQUIRE(a->window >= 0 && a->sinks >= 0 && a->width >= 1 && a->B <= 65536, B200LUT_ERR_INVALID,
                   "attend: window and sinks must not be negative, width must be positive, B at most 65536");
+  B200LUT_REQUIRE(fabsf(a->scale) < 1.7014118e38f, B200LUT_ERR_INVALID, "attend: scale must be finite, below 2^127");
   if (a->T == 0 || a->B == 0) return B200LUT_OK;
   B200LUT_REQUIRE(a->q && a->out && a->block_table && a->kv_len, B200LUT_ERR_INVALID, "attend: null argument");
   B200LUT_REQUIRE(a->row_start || a->T == a->B, B200LUT_ERR_INVALID,

@@ -162,7 +162,7 @@ PyObject* attend(Guard&& guarded, Context&& context, PyObject* const* a, Py_ssiz
   const double scale = PyFloat_AS_DOUBLE(a[5]);
   int over = 0, over2 = 0;
   const long window = PyLong_AsLongAndOverflow(a[6], &over), sinks = PyLong_AsLongAndOverflow(a[7], &over2);
-  if (over || over2 || window < 0 || sinks < 0 || window > 0x7fffffff || sinks > 0x7fffffff || !std::isfinite(scale)) Py_RETURN_NONE;
+  if (over || over2 || window < 0 || sinks < 0 || window > 0x7fffffff || sinks > 0x7fffffff || !(std::fabs(scale) < 0x1p127)) Py_RETURN_NONE;
   return guarded([&]() -> PyObject* {
     Cache* c = cache_of(a[0]);
     const at::Tensor *q = tensor_of(a[1]), *table = tensor_of(a[2]), *len = tensor_of(a[3]), *start = tensor_of(a[4]),

@@ -17,7 +17,6 @@ can be captured into CUDA graphs.
 from __future__ import annotations
 
 import ctypes
-import math
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -214,8 +213,8 @@ class KVCache4:
         if window < 0 or sinks < 0 or width < 1:
             raise ValueError("window and sinks must not be negative, and block_table needs some width")
         scale = D ** -0.5 if scale is None else float(scale)
-        if not math.isfinite(scale):
-            raise ValueError(f"scale must be finite, got {scale}")
+        if not abs(scale) < 2.0 ** 127:              # 32 bits hold it, times log2(e) too
+            raise ValueError(f"scale must be finite, below 2^127, got {scale}")
         if width > 1 and block_table.stride(1) != 1:
             block_table = block_table.contiguous()
         if gate is not None:

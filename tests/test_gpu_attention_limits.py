@@ -163,3 +163,12 @@ def test_pages_that_no_row_sees_may_be_given_away(rows, Hq, H, D, page):
             b.table[0, (n - rows - window + 1) // page] = -1            # the first row sees a token of it
             b.run(window=window, sinks=sinks)
             assert status() == 0x6200 and status() == 0
+
+
+def test_scales_that_32_bits_do_not_hold():
+    b = Batch([40], [1], 4, 2, 128, 16)
+    for scale in (1e300, -1e39, 2.0 ** 127, float("inf")):
+        with pytest.raises(ValueError, match="scale"):
+            b.run(scale=scale)
+    b.q.mul_(2.0 ** -100)
+    b.check(scale=2.0 ** 96)
