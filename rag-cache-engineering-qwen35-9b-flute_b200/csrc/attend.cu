@@ -9,7 +9,8 @@
 // Operands: the tokens are the M = 16 side of mma.m16n8k16, the rows its N = 8 side, so a tile of codes is
 // unpacked once and eight rows ride for free.
 //   S^T[token, row] = K[token, :] q[row, :]     A = keys: lane (g, t) holds 16 tokens' rows g and g + 8
-//   O^T[dim, row]  += V^T[dim, token] P^T       A = values: lane (g, t) holds elements 8 g .. 8 g + 7 of four tokens
+//   O^T[dim, row]  += V^T[dim, token] P^T       A = values: lane (g, t) holds elements 8 g .. 8 g + 7 of four tokens;
+//                                               their codes at c * 2^-22 and c * 2^-18 (kTop: all at c * 2^-18)
 // Row s of A stands for token pi(s) = 4 (s / 2 % 4) + s % 2 + 2 (s / 8) of the tile, so that the four tokens of a
 // value lane are adjacent in memory; P^T comes out of S^T by two 8 x 8 transposes of half pairs.
 // Every lane copies exactly the 16-byte pieces it will read (cp.async into a ring of its own): no barrier in
@@ -115,10 +116,18 @@ __global__ void __launch_bounds__(Shape<D, NT>::kWarps * 32, Shape<D, NT>::kBloc
 attend_rows_kernel(const __grid_constant__ AttendParams p) {
   using S = Shape<D, NT>;
   constexpr int kRows = S::kRows, kWarps = S::kWarps, kTile = S::kTile, kSub = S::kSub;
-  // Weights are rounded to fp16 for the products: 2^-12 of each, little beside a bf16 result's rounding of 2^-9, but as
-  // much as an fp16 result's own. There a second product takes what the rounding left: the error against 64 bits falls
-  // from 1.5 times the result's rounding to that rounding, for 0.3 us of 20 (16 sequences behind a window of 4096).
+  // Weights are rounded to fp16 for the products: 2^-11 of each, little beside a bf16 result's rounding of 2^-8, but as
+  // much as an fp16 result's own. There a second product takes what the rounding left: 0.3 us of 20 (16 sequences behind
+  // a window of 4096).
   constexpr bool kSplit = std::is_same<T, __half>::value;
+  // The matrix unit aligns the products of a step by the exponents that their operands are written with, and drops what
+  // lies 2^-25 below the largest: of a subnormal the bits that it does not have are lost besides. Codes as the low four
+  // bits lose what is 2^-6 below (1 + 2^-10 times 15 and 1, measured), so light weights beside a heavy one came out short:
+  // over 131072 tokens the error was 1.10 times a bf16 result's rounding and 2.6 times an fp16 one's (64 elements). So
+  // values' codes stand two bits higher, 1.01 times, for one shift more a word; for fp16 results all at the mantissa's top
+  // (1.00 times), four shifts instead of one. Neither shows in the times (53.4, 94.3 and 24.6 us; all codes at the top for
+  // bf16: 55.3 and 97.7). Keys' codes stay: scores of products alike in size lose nothing that shows.
+  constexpr bool kTop = kSplit;
   extern __shared__ __align__(128) uint8_t sm[];
   uint16_t* sq = reinterpret_cast<uint16_t*>(sm);
   uint8_t* ring = sm + S::kQ;
@@ -496,24 +505,20 @@ attend_rows_kernel(const __grid_constant__ AttendParams p) {
 #pragma unroll
             for (int s = 0; s < kSub; ++s) {
               const uint4 c = lds128(at + s * S::kPart + S::kPieces * 512 + i * 512);
-              uint32_t x01 = __byte_perm(c.x, c.y, 0x5410), y01 = __byte_perm(c.x, c.y, 0x7632);
-              uint32_t x23 = __byte_perm(c.z, c.w, 0x5410), y23 = __byte_perm(c.z, c.w, 0x7632);
+              const uint32_t x01 = __byte_perm(c.x, c.y, 0x5410), y01 = __byte_perm(c.x, c.y, 0x7632);
+              const uint32_t x23 = __byte_perm(c.z, c.w, 0x5410), y23 = __byte_perm(c.z, c.w, 0x7632);
+              auto code = [](uint32_t x, int j) {          // code j of each half, high in the mantissa
+                if (kTop) return (j == 0 ? x << 6 : j == 1 ? x << 2 : j == 2 ? x >> 2 : x >> 6) & 0x03C003C0u;
+                return (j < 2 ? x << 2 : x >> 6) & (j & 1 ? 0x03C003C0u : 0x003C003Cu);
+              };
 #pragma unroll
-              for (int j = 0; j < 2; ++j) {
+              for (int j = 0; j < 4; ++j) {
+                const uint32_t a0 = code(x01, j), a1 = code(y01, j), a2 = code(x23, j), a3 = code(y23, j);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                  mma16(o[n][i * 4 + 2 * j], x01 & 0x000F000Fu, y01 & 0x000F000Fu, x23 & 0x000F000Fu, y23 & 0x000F000Fu,
-                        bf[s][n][0], bf[s][n][1]);
-                  mma16(o[n][i * 4 + 2 * j + 1], x01 & 0x00F000F0u, y01 & 0x00F000F0u, x23 & 0x00F000F0u,
-                        y23 & 0x00F000F0u, bf[s][n][0], bf[s][n][1]);
-                  if constexpr (kSplit) {
-                    mma16(o[n][i * 4 + 2 * j], x01 & 0x000F000Fu, y01 & 0x000F000Fu, x23 & 0x000F000Fu, y23 & 0x000F000Fu,
-                          rest[s][n][0], rest[s][n][1]);
-                    mma16(o[n][i * 4 + 2 * j + 1], x01 & 0x00F000F0u, y01 & 0x00F000F0u, x23 & 0x00F000F0u,
-                          y23 & 0x00F000F0u, rest[s][n][0], rest[s][n][1]);
-                  }
+                  mma16(o[n][i * 4 + j], a0, a1, a2, a3, bf[s][n][0], bf[s][n][1]);
+                  if constexpr (kSplit) mma16(o[n][i * 4 + j], a0, a1, a2, a3, rest[s][n][0], rest[s][n][1]);
                 }
-                x01 >>= 8, y01 >>= 8, x23 >>= 8, y23 >>= 8;
               }
             }
         }
@@ -535,7 +540,7 @@ attend_rows_kernel(const __grid_constant__ AttendParams p) {
             const float mid = fmaf(-7.5f, ws[n][e], pm[n][e]);
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) {
-              const float f = i & 1 ? 1048576.f : 16777216.f;
+              const float f = kTop || (i & 1) ? 262144.f : 4194304.f;
               const int d = (i >> 2) * 64 + 8 * g + (i & 3);
               fold[r * (D + 4) + d] = fmaf(o[n][i][e], f, mid);
               fold[r * (D + 4) + d + 4] = fmaf(o[n][i][e + 2], f, mid);

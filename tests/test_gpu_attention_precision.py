@@ -1,6 +1,8 @@
 """What a row's result may depend on, and how closely: attention on the GPU against bounds from the row's own weights."""
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -79,3 +81,33 @@ def test_large_and_small_values(rows):
     b.v[0][250:] = 0
     store(b)
     check(b, b.run())
+
+
+@pytest.mark.parametrize("dtype", (torch.float16, torch.bfloat16))
+@pytest.mark.parametrize("D,G", [(64, 1), (128, 4), (256, 2), (128, 12)])
+@pytest.mark.parametrize("L", (16, 96, 640))
+def test_light_weights_beside_heavy_ones(L, D, G, dtype):
+    # one token in 16 weighs 2^10 to 2^14 times the others and has nothing but zeros: the result is the others' sum.
+    # Scores are multiples of one number, exact up to its rounding, so that little is lost on the way to the second product
+    g = torch.Generator().manual_seed(L + D)
+    k, v = torch.full((L, 1, D), 7.0), torch.randint(-7, 9, (L, 1, D), generator=g).float()
+    k[..., 0], k[..., 1], k[..., 2] = 0, 15, torch.randint(0, 4, (L, 1), generator=g).float()
+    heavy = torch.arange(L) % 16 == torch.randint(0, 16, (1,), generator=g)
+    k[heavy, :, 2], v[heavy] = 15, 0
+    v[..., 0], v[..., 1] = -7, 8                              # every row: a step of 1, zero at code 7
+    q = torch.zeros(1, G, D)
+    q[..., 2] = 1
+    cache = pkg.kvcache.KVCache4(-(-L // 16), 1, D, page_size=16, dtype=dtype)
+    cache.write(k.to(dtype).cuda(), v.to(dtype).cuda(), torch.arange(L, dtype=torch.int32, device="cuda"))
+    table = torch.arange(cache.n_pages, dtype=torch.int32, device="cuda")[None]
+    y = cache.attend(q.to(dtype).cuda(), table, torch.tensor([L], dtype=torch.int32, device="cuda"), scale=0.9 * math.log(2)).double().cpu()
+    p = torch.softmax(k[:, 0, 2].double() * 0.9 * math.log(2), 0)
+    want = (p @ v[:, 0].double()).expand(1, G, D)
+    # in steps: each product off by 2^-24 of 15 heavy weights (fp16: codes are normal numbers) or by 2^-16 of a heavy
+    # weight (codes of four bits, two above the lowest), 16 a group; fp32 sums of at most 15, one a group and 40 at the ends.
+    # bf16: the weights' own rounding, 2^-11 of half a step for the heavy ones and of 7.5 for what the others weigh (2^-6)
+    drop = 16 * (15 * 2.0 ** -24 if dtype == torch.float16 else 2.0 ** -16)
+    if dtype == torch.bfloat16:
+        drop += 2.0 ** -11 * (0.5 + 7.5 * 2.0 ** -6)
+    tol = drop + 15 * (L / 16 + 40) * 2.0 ** -24 + 15 * 2.0 ** -22 + torch.finfo(dtype).eps / 2 * want.abs() + 2.0 ** -25
+    close(y[..., 2:], want[..., 2:], tol[..., 2:])
