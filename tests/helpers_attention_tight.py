@@ -41,3 +41,22 @@ def attend_tight(q, k, v, pos, scale, window=0, sinks=0, split=False):
         out[:, h] = o
         tol[:, h] = err[:, None] + 2 * reach[:, None] * spread + (unit(q.dtype) + 2.0 ** -20) * o.abs() + floor(q.dtype)
     return out, tol
+
+
+def counted_values(L, D):
+    """Values [L, D] by which a result counts its tokens: all of 16-token tile t is 8 at element t % D, -7 at t + 1 and 0
+    elsewhere (fifteen steps of 1). Under equal weights a tile's absence moves an element by 128 / L."""
+    v = torch.zeros(L, D, dtype=torch.float64)
+    t = torch.arange(L) // 16
+    v[torch.arange(L), t % D], v[torch.arange(L), (t + 1) % D] = 8, -7
+    return v
+
+
+def counted_want(v, lengths, dtype):
+    """Means of the first lengths[i] of counted_values, and their bound. All weights of a row are alike, so their rounding
+    to fp16 is one factor, 2^-11, of what codes are away from 7.5 or 8 on average, which is at most 1 plus the mean; fp32
+    sums of parts: 2^-18 of that; 2^-20 of the parameters' sizes; the result's rounding."""
+    total = v.cumsum(0)[lengths - 1]
+    want = total / lengths[:, None]
+    tol = (2.0 ** -11 + 2.0 ** -18) * (1 + want.abs()) + 2.0 ** -20 * 8 + unit(dtype) * want.abs() + floor(dtype)
+    return want, tol
