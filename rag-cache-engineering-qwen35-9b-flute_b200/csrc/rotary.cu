@@ -40,6 +40,7 @@ struct RotaryParams {
 };
 
 constexpr int kWarps = 4;
+constexpr float kHuge = 8.470329e-22f;           // 2^-70
 
 template <typename T, int D, int U>
 __global__ void __launch_bounds__(kWarps * 32) rotary_kernel(const __grid_constant__ RotaryParams p) {
@@ -105,7 +106,19 @@ __global__ void __launch_bounds__(kWarps * 32) rotary_kernel(const __grid_consta
       float sum = q.x + q.y;
 #pragma unroll
       for (int o = lanes >> 1; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      const float r = rsqrtf(fmaf(sum, share, p.eps));
+      float r = rsqrtf(fmaf(sum, share, p.eps));
+      // squares of elements from 2^60 on pass fp32: such a head's are summed again in units of 2^-70
+      if (__builtin_expect(__any_sync(0xffffffffu, sum > 3.4e38f), 0)) {
+        float again = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 w = mul2(v[e], make_float2(kHuge, kHuge));
+          again = fmaf(w.x, w.x, fmaf(w.y, w.y, again));
+        }
+#pragma unroll 1
+        for (int o = lanes >> 1; o; o >>= 1) again += __shfl_xor_sync(0xffffffffu, again, o);
+        if (sum > 3.4e38f) r = rsqrtf(again * share) * kHuge;
+      }
       if (of_q && h >= p.Hq) gains(1), of_q = false;
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = mul2(v[e], mul2(make_float2(r, r), gain[e]));

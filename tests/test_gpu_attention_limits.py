@@ -172,3 +172,24 @@ def test_scales_that_32_bits_do_not_hold():
             b.run(scale=scale)
     b.q.mul_(2.0 ** -100)
     b.check(scale=2.0 ** 96)
+
+
+@pytest.mark.parametrize("D,R", [(64, 32), (128, 128), (256, 64)])
+def test_norm_of_heads_whose_squares_pass_32_bits(D, R):
+    from helpers_attention import rotate64
+    rot = pkg.rotary.AxisRotary(R, theta=1e4)
+    g = torch.Generator(device="cuda").manual_seed(D)
+    for T in (1, 9, 3000):
+        q, k = (torch.randn(T, n, D, device="cuda", generator=g) for n in (5, 2))
+        size = torch.randint(55, 125, (T, 5, 1), device="cuda", generator=g)
+        q = (q * torch.where(size % 3 == 0, 0, size).float().exp2()).bfloat16()
+        k = (k * 2.0 ** 62).bfloat16()
+        gains = [(1 + 0.1 * torch.randn(D, device="cuda", generator=g)).bfloat16() for _ in range(2)]
+        pos = torch.arange(T, device="cuda")
+        for x, y, gain in zip((q, k), rot(q, k, pos, *gains), gains):
+            want, tol = rotate64(x, pos[None], R, 1e4, rot.axis, gain)
+            close(y, want, tol)
+    q = torch.zeros(1, 1, D, device="cuda", dtype=torch.bfloat16)
+    q[0, 0, R - 1] = float("inf")                           # 0 times infinity stays NaN, the others are zero
+    y = rot(q, k[:1], pos[:1], *gains)[0]
+    assert y.isnan().any() and (y.isnan() | (y == 0)).all()
