@@ -74,9 +74,11 @@ def plan_step(cached: torch.Tensor, fresh: torch.Tensor, block_table: torch.Tens
         raise ValueError(f"page_size must be one of {PAGE_SIZES}, got {page_size}")
     if not block_table.is_contiguous():
         raise ValueError("block_table is written in place: it must be contiguous")
-    if B < 1 or B > 8192 or block_table.shape[1] < 1 or max_tokens < 1:
-        raise ValueError(f"plan_step: 1 to 8192 requests, a block_table of some width and max_tokens >= 1 wanted, "
-                         f"got {B}, {block_table.shape[1]}, {max_tokens}")
+    if B < 1 or B > 8192 or not 1 <= block_table.shape[1] <= INT_MAX or not 1 <= max_tokens <= INT_MAX:
+        raise ValueError(f"plan_step: 1 to 8192 requests, a block_table of some width and max_tokens >= 1 wanted, both below "
+                         f"2^31, got {B}, {block_table.shape[1]}, {max_tokens}")
+    if free_pages.shape[0] > INT_MAX:
+        raise ValueError(f"plan_step: fewer than 2^31 free pages wanted, got {free_pages.shape[0]}")
     return _plan_route(cached, fresh, block_table, free_pages, taken, page_size, max_tokens)
 
 
@@ -210,8 +212,8 @@ class KVCache4:
             row_start = _ints("row_start", row_start, (B + 1,), self.device).contiguous()
         elif T != B:
             raise ValueError(f"without row_start there is one row per request: {T} rows, {B} requests")
-        if window < 0 or sinks < 0 or width < 1:
-            raise ValueError("window and sinks must not be negative, and block_table needs some width")
+        if window < 0 or sinks < 0 or not 1 <= width <= INT_MAX:
+            raise ValueError("window and sinks must not be negative, and block_table needs some width, below 2^31")
         scale = D ** -0.5 if scale is None else float(scale)
         if not abs(scale) < 2.0 ** 127:              # 32 bits hold it, times log2(e) too
             raise ValueError(f"scale must be finite, below 2^127, got {scale}")

@@ -193,3 +193,16 @@ def test_norm_of_heads_whose_squares_pass_32_bits(D, R):
     q[0, 0, R - 1] = float("inf")                           # 0 times infinity stays NaN, the others are zero
     y = rot(q, k[:1], pos[:1], *gains)[0]
     assert y.isnan().any() and (y.isnan() | (y == 0)).all()
+
+
+def test_sizes_that_32_bits_do_not_hold():
+    i = torch.zeros(3, **INT)
+    for room in (2 ** 31, 2 ** 32 + 8, 2 ** 64):
+        with pytest.raises(ValueError, match="2\\^31"):
+            kv.plan_step(i, i, torch.zeros(3, 2, **INT), i, i[:1], page_size=16, max_tokens=room)
+    wide = i[:1].expand(1, 2 ** 32 + 1)                     # one element, read as so many
+    with pytest.raises(ValueError, match="2\\^31"):
+        kv.plan_step(i[:1], i[:1], torch.zeros(1, 2, **INT), wide[0], i[:1], page_size=16, max_tokens=8)
+    cache = kv.KVCache4(2, 1, 64, page_size=16)
+    with pytest.raises(ValueError, match="2\\^31"):
+        cache.attend(torch.zeros(1, 1, 64, device="cuda", dtype=torch.bfloat16), wide, i[:1])
