@@ -588,7 +588,7 @@ typedef struct b200lut_kv_cache {
  * the requests, pages that it does not have yet are taken from free_pages[*taken ..] and entered
  * into its row of block_table. A request whose pages do not fit its row or the free list, whose rows
  * would end behind max_tokens, or that would pass 2^31 - 1 tokens, is not served: it gets no page and
- * its slots are -1.
+ * its slots are -1. What it asks of the free list counts for the requests behind it.
  * Results: row_start [B + 1] (clamped to max_tokens), kv_len [B] (cached + fresh where served, else
  * cached), positions and slots [max_tokens] (0 and -1 behind the last row; -1 also where the row
  * holds a negative page), taken_out [1], served [B] (bytes, 0 or 1). Calling it again with the same

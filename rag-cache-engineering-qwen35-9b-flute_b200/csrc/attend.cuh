@@ -6,16 +6,18 @@
 // so the matrix products run on the 4-bit codes themselves and a token's two parameters enter the scores and
 // the probabilities, not the elements: nothing of K or V is rounded. A code needs one AND to become an
 // operand: in the low bits of a half it is the subnormal c * 2^-24, four bits higher c * 2^-20, both exact,
-// and the powers of two go into q and the result.
-// q is multiplied by the power of two that puts its row's largest element into [2^13, 2^14), in the kernel for many
-// rows into [2^15, 2^16): fp16 then
-// holds bf16's eight bits exactly down to 2^-28 of the largest element (and fp16's eleven to 2^-25).
+// and the powers of two go into q and the result. (The sum of products is another matter: the values' codes of the
+// kernel for few rows stand higher, see there.)
+// q is multiplied by the power of two that puts its row's largest element into [2^13, 2^14), in the kernel for many rows
+// into [2^15, 2^16): fp16 then holds bf16's eight bits exactly down to 2^-28 of the largest element (and fp16's eleven to
+// 2^-25).
 // The weights w = p * step of the second product are rounded to fp16 (2^-11). p is 2^(s - m) with an m of the row's own
 // that follows s + log2(step) over the tokens the row sees (exponents rounded up, a lag of 2^8 allowed): w stays below
-// 2^15 and only weights 2^-20 below the row's largest are subnormal. Nothing that a row does not see, and nothing that
-// weighs nothing in it, enters m. (Divided by the largest step of all tokens in the row's tiles, weights lost the bits by
-// which a hidden value was larger: of 300 tokens the error grew from 1.8e-3 to 2.1e-3 beside one 2^16 times larger, to
-// 1.4e-2 at 2^20. An m of the row's own costs the tile kernel 2 % and the row kernel 1.5 %.)
+// 2^15, and the largest is 2^6 or more (2^-2 in the kernel for many rows, which takes a tile's largest score and largest
+// step together where its steps are within 2^8), so that what is lost of a subnormal weight is 2^-23 of the largest at
+// most. Nothing that a row does not see, and nothing that weighs nothing in it, enters m. (Divided by the largest step of
+// all tokens in the row's tiles, weights lost the bits by which a hidden value was larger: of 300 tokens the error grew
+// from 1.8e-3 to 2.1e-3 beside one 2^16 times larger, to 1.4e-2 at 2^20.)
 // With w the rounded weight the result is formed as sum w c - 7.5 sum w + sum p (lo + 7.5 step) (the kernel for many rows:
 // 8): the rounding then acts on c - 7.5, at most half as large as c. With sum w c and lo the error of an fp16 result was
 // 2.9 times its own rounding; so it is 1.45 to 1.57 times (512 rows over 2048 tokens, 256 and 64 elements; a bf16

@@ -56,7 +56,8 @@ def plan_step(cached: torch.Tensor, fresh: torch.Tensor, block_table: torch.Tens
     brings fresh[b] more; block_table [B, width] gets the pages it takes from free_pages[taken ..], in the order of
     the requests. All int32 CUDA tensors. A request whose pages do not fit its row of block_table or what is left
     of the free list, whose rows would end behind max_tokens, or that would pass 2^31 - 1 tokens, is not served: it
-    takes no page and its slots are -1. The caller goes on with the returned kv_len and taken; the same call again gives the same result."""
+    takes no page and its slots are -1. What one asks of the free list counts for those behind it: once it has run out, only
+    requests that need no page are served. The caller goes on with the returned kv_len and taken; the same call again gives the same result."""
     _lib._need_cuda(cached, "cached")
     done = _lib.host.kv_plan(cached, fresh, block_table, free_pages, taken, page_size, max_tokens) \
         if page_size in PAGE_SIZES else None
