@@ -53,7 +53,8 @@ class PalettizedAttention(nn.Module):
 
     qkv: a SplitQKV whose q_proj gives n_heads * head_dim rows, or, gated, 2 * head_dim a head: the query and then a
     gate by whose sigmoid the head's result is multiplied. q_gain, k_gain [head_dim]: gains of an RMS norm of every
-    head in front of the rotation (both or neither; detached, or under no_grad: nothing is differentiated). window, sinks, scale: as KVCache4.attend."""
+    head in front of the rotation (both or neither; detached, or under no_grad: nothing is differentiated). window, sinks,
+    scale: as KVCache4.attend."""
 
     def __init__(self, qkv, o_proj, rotary: AxisRotary, head_dim: int, gated: bool = False,
                  q_gain: Optional[torch.Tensor] = None, k_gain: Optional[torch.Tensor] = None, eps: float = 1e-6,

@@ -113,12 +113,12 @@ __device__ __forceinline__ float gated(float o, const AttendParams& p, long long
   return o / (1.f + __expf(-g));
 }
 
-// A token's size: its step, or 2^-20 of its middle where that is larger (a row of equal elements has no step), or 2^-80;
+// A token's size: its step, or 2^-20 of its middle where that is larger (a row of equal elements has no step), or 2^-94;
 // so p * step and p * mid both keep their range. What it adds to a score in m: the exponent of the next power of two, less
 // the 7 that leave weights room up to 2^7, 2^15 with the lag.
 // m of two parts of a row may differ by some 200 for the tokens' sizes alone: a sum of p takes the factor between them in
 // two halves, since the sum may be as large as the factor is small.
-constexpr float kMinStep = 8.271806e-25f;      // 2^-80
+constexpr float kMinStep = 5.04870979e-29f;      // 2^-94
 __device__ __forceinline__ float token_size(float step, float mid) { return fmaxf(step, fmaxf(fabsf(mid) * 9.5367432e-7f, kMinStep)); }
 __device__ __forceinline__ int exponent_above(float size) { return int((__float_as_uint(size) + 0x007FFFFFu) >> 23) - 127; }
 __device__ __forceinline__ float size_in_m(float size) { return float(exponent_above(size) - 7); }

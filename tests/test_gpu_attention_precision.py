@@ -67,7 +67,7 @@ def test_large_values_of_no_weight(D, Hq, H):
 
 @pytest.mark.parametrize("rows", (1, 4, 60))
 def test_large_and_small_values(rows):
-    for size in (-100, -80, -60, 60, 100, 116):
+    for size in (-112, -106, -100, -80, -60, 60, 100, 116):
         b = Batch([300, 64], [rows, 1], 4, 2, 128, 16, seed=size & 255)
         b.v = [x * 2.0 ** size for x in b.v]
         store(b)
