@@ -700,7 +700,7 @@ int launch(const AttendParams& p, int blocks, bool behind, cudaStream_t st) {
 // other side of that limit, measured with up to 8 heads a key head, 64 requests of 4096 to 8192 tokens (a row tile more
 // for every 8 rows here against one tile of 128 there): 8 rows 139 us here; 16 rows 242 here and 349 there, 24 rows 343
 // and 351, 32 rows 448 and 351 (4 heads of 256); 242 and 519, 351 and 518, 455 and 518, 48 rows 674 and 526 (8 heads of
-// 128); 32 requests of one head of 64: 16 rows 31 and 65, 64 rows 59 and 69. So the tile kernel is the better one from 24,
+// 128); 32 requests of one head of 64: 16 rows 31 and 65, 64 rows 59 and 69. So the tile kernel is the better one from some 24,
 // 32 and 64 rows on; between 9 rows and there a request costs up to twice what two or three items here would.
 int rows_of(int G) { return G <= 8 ? 8 : 16; }
 int row_blocks(int sms, int G) { return G <= 8 ? 2 * sms : sms; }      // Shape::kBlocks
