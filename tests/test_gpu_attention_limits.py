@@ -206,3 +206,27 @@ def test_sizes_that_32_bits_do_not_hold():
     cache = kv.KVCache4(2, 1, 64, page_size=16)
     with pytest.raises(ValueError, match="2\\^31"):
         cache.attend(torch.zeros(1, 1, 64, device="cuda", dtype=torch.bfloat16), wide, i[:1])
+
+
+@pytest.mark.parametrize("Hq,H,D", [(8, 2, 128), (24, 2, 64), (16, 4, 256)])
+def test_the_result_in_the_place_of_the_queries_or_gates(Hq, H, D):
+    for lengths, rows in (([9000, 40, 700], [1, 1, 1]), ([5000, 300, 20], [200, 1, 9])):
+        b = Batch(lengths, rows, Hq, H, D, 32, gate=True)
+        want, q, gate = b.run(), b.q.clone(), b.gate.clone()
+        for _ in range(3):
+            b.q = q.clone()
+            assert b.run(out=b.q) is b.q and torch.equal(b.q, want)
+            b.q, b.gate = q, gate.clone()
+            assert b.run(out=b.gate) is b.gate and torch.equal(b.gate, want)
+            b.gate = gate
+
+
+def test_one_table_for_every_request_and_lengths_with_strides():
+    b = Batch([300], [1], 8, 2, 128, 16)
+    q = b.q.expand(5, 8, 128)                                   # one query, five lengths
+    lengths = torch.tensor([[300, 0], [17, 0], [0, 0], [1, 0], [255, 0]], **INT)[:, 0]
+    y = b.cache.attend(q, b.table.expand(5, -1), lengths)
+    for i, n in enumerate(lengths.tolist()):
+        want, tol = attend64(b.q, values64(b.k[0][:n]), values64(b.v[0][:n]), torch.tensor([n - 1], device="cuda"), 128 ** -0.5)
+        close(y[i:i + 1], want, tol, str(n))
+    assert status() == 0
