@@ -190,10 +190,9 @@ class KVCache4:
         block_table[b] (int32 [B, width]). The row at position p sees the tokens j <= p; with a window those with
         j > p - window, and the first `sinks` tokens besides. Query head h reads key/value head
         h // (n_heads / n_kv_heads). scale: head_dim ** -0.5 unless given. gate: the result is multiplied by
-        sigmoid(gate). out may be q or gate itself. Where nothing is visible the result is zero; rows that belong to no request are not written.
-        A visible token on a page outside the cache counts as hidden and raises the device status (0x6200); pages that
-        no row sees may be given away. The sums over tokens
-        are fp32 and divided at the end."""
+        sigmoid(gate). out may be q or gate itself. Where nothing is visible the result is zero; rows that belong to no
+        request are not written. A visible token on a page outside the cache counts as hidden and raises the device status
+        (0x6200); pages that no row sees may be given away. The sums over tokens are fp32 and divided at the end."""
         done = _lib.host.attend(self._native, q, block_table, kv_len, row_start,
                                 self.head_dim ** -0.5 if scale is None else scale, window, sinks, gate, out)
         if done is not None:
